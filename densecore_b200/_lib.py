@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -16,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdensecore_sdpa.so")
 
 DC_OK, DC_ERR_VALUE, DC_ERR_RUNTIME, DC_ERR_CUDA, DC_ERR_UNSUPPORTED = 0, 1, 2, 3, 4
-DC_F32, DC_BOOL = 0, 1
+DC_F32, DC_BOOL, DC_F16, DC_BF16, DC_I32, DC_I64, DC_F64 = range(7)
 DC_PREC_3XTF32, DC_PREC_TF32, DC_PREC_FP32 = 0, 1, 2
 
 # Every entry point include/densecore_sdpa.h declares.
@@ -24,7 +25,10 @@ EXPORTS = ("dc_sdpa_fwd", "dc_sdpa_bwd_workspace_size", "dc_sdpa_bwd", "dc_sdpa_
            "dc_sdpa_decode_default_splits", "dc_sdpa_decode", "dc_sdpa_decode_noalloc", "dc_attn_merge", "dc_attn_probs",
            "dc_last_error", "dc_abi_version", "dc_sdpa_fwd_path", "dc_kernel_timing", "dc_kernel_timing_report", "dc_device_status",
            "dc_dropout_keep_bits", "dc_rng_skip", "dc_sdpa_fwd_dropout", "dc_sdpa_bwd_dropout", "dc_attn_probs_dropout",
-           "dc_debug_wait_probe", "dc_ring_sdpa_fwd_workspace_size", "dc_ring_sdpa_fwd")
+           "dc_debug_wait_probe", "dc_ring_sdpa_fwd_workspace_size", "dc_ring_sdpa_fwd",
+           "dc_sdpa_window_fwd_workspace_size", "dc_sdpa_window_fwd", "dc_sdpa_window_bwd", "dc_rotary", "dc_qk_norm_rotary",
+           "dc_qk_norm_rotary_bwd_workspace_size", "dc_qk_norm_rotary_bwd", "dc_cache4_append", "dc_cache4_read",
+           "dc_cache4_attention_workspace_size", "dc_cache4_attention")
 
 
 class DcTensor(ctypes.Structure):
@@ -32,7 +36,13 @@ class DcTensor(ctypes.Structure):
                 ("sizes", ctypes.c_int64 * 4), ("strides", ctypes.c_int64 * 4)]
 
 
+class DcCache4(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("num_pages", ctypes.c_int64),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32)]
+
+
 _P = ctypes.POINTER(DcTensor)
+_C4 = ctypes.POINTER(DcCache4)
 _lock = threading.Lock()
 _lib = None
 
@@ -93,6 +103,29 @@ def load():
         L.dc_ring_sdpa_fwd_workspace_size.restype = sz
         L.dc_ring_sdpa_fwd.argtypes = [_P, _P, _P, i, i, d, i, vp, _P, _P, vp, sz, vp]
         L.dc_ring_sdpa_fwd.restype = i
+        L.dc_sdpa_window_fwd_workspace_size.argtypes = [i64] * 8
+        L.dc_sdpa_window_fwd_workspace_size.restype = sz
+        # Tensors of these come as bytes (packed) or references.
+        L.dc_sdpa_window_fwd.argtypes = [vp] * 4 + [i64] * 3 + [vp, i, d, i, vp, vp, vp, sz, vp]
+        L.dc_sdpa_window_fwd.restype = i
+        L.dc_sdpa_window_bwd.argtypes = [vp] * 7 + [i64] * 3 + [i, d, i, vp, vp, vp, vp, sz, vp]
+        L.dc_sdpa_window_bwd.restype = i
+        L.dc_rotary.argtypes = [vp] * 4 + [i, d, i, vp, vp, vp]
+        L.dc_rotary.restype = i
+        L.dc_qk_norm_rotary.argtypes = [vp] * 6 + [d, i, d, vp, vp, vp]
+        L.dc_qk_norm_rotary.restype = i
+        L.dc_qk_norm_rotary_bwd_workspace_size.argtypes = [i64]
+        L.dc_qk_norm_rotary_bwd_workspace_size.restype = sz
+        L.dc_qk_norm_rotary_bwd.argtypes = [vp] * 8 + [d, i, d, vp, vp, vp, vp, vp, sz, vp]
+        L.dc_qk_norm_rotary_bwd.restype = i
+        L.dc_cache4_append.argtypes = [_C4, vp, vp, vp, vp, vp, vp]
+        L.dc_cache4_append.restype = i
+        L.dc_cache4_read.argtypes = [_C4, vp, vp, vp, vp, vp]
+        L.dc_cache4_read.restype = i
+        L.dc_cache4_attention_workspace_size.argtypes = [i64] * 7 + [i]
+        L.dc_cache4_attention_workspace_size.restype = sz
+        L.dc_cache4_attention.argtypes = [_C4, vp, vp, vp, i64, i64, i, d, vp, vp, vp, sz, vp]
+        L.dc_cache4_attention.restype = i
         L.dc_debug_wait_probe.argtypes = [ctypes.c_uint64, i, vp]
         L.dc_debug_wait_probe.restype = i
         L.dc_kernel_timing.argtypes = [i]
@@ -125,6 +158,27 @@ def view(t: torch.Tensor | None):
         v.sizes[n] = s
         v.strides[n] = st
     return v
+
+
+_DTYPES = {torch.float32: DC_F32, torch.bool: DC_BOOL, torch.uint8: DC_BOOL, torch.float16: DC_F16,
+           torch.bfloat16: DC_BF16, torch.int32: DC_I32, torch.int64: DC_I64, torch.float64: DC_F64}
+# dc_tensor_t of a tensor of 0 to 4 dims, packed (sizes and strides padded to 4).
+_PACK = [struct.Struct(f"<Qii{n}q{8 * (4 - n)}x{n}q{8 * (4 - n)}x").pack for n in range(5)]
+
+
+def packed(t: torch.Tensor | None):
+    """A dc_tensor_t describing ``t`` as bytes (a ctypes structure takes three times as long to fill,
+    which shows in single-token calls), for the entry points whose arguments are plain pointers and
+    that take other types than float32 and bool; None stays None."""
+    if t is None:
+        return None
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        raise TypeError(f"densecore_b200: unsupported tensor dtype {t.dtype}")
+    shape = t.shape
+    if len(shape) > 4:
+        raise ValueError("densecore_b200: tensors have at most 4 dims")
+    return _PACK[len(shape)](t.data_ptr(), dt, len(shape), *shape, *t.stride())
 
 
 def ref(v):

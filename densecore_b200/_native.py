@@ -11,6 +11,8 @@ materialised (B, H, L, S) float mask is accepted as one case of it.
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -205,3 +207,162 @@ def _fwd_path(q, k, v, mask=None, causal=False, precision=None):
     prec = precision_code() if precision is None else precision
     vs = [_lib.view(t) for t in (q, k, v, mask)]
     return L.dc_sdpa_fwd_path(*[_lib.ref(x) for x in vs], int(bool(causal)), prec)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(dev):
+    """The context in which ``dev`` is the current device."""
+    return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _device_of(first, *rest):
+    """:func:`_require_cuda` with one integer comparison a tensor while all is well."""
+    index = first.get_device()
+    if index >= 0:
+        for t in rest:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return first.device
+    return _require_cuda(first, *rest)
+
+
+def _refs(*ts):
+    """The tensors as the C entry points take them (None stays None)."""
+    return [_lib.packed(t) for t in ts]
+
+
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _sliding_window(q, k, v, window, sinks, offset, scale=None, mask=None, lengths=None, precision=None):
+    """Forward through a sliding window (dc_sdpa_window_fwd): (out, lse)."""
+    L = _lib.load()
+    dev = _device_of(q, k, v, mask, lengths)
+    B, H, Lq, E = q.shape
+    S, Ev = k.shape[2], v.shape[3]
+    out = torch.empty((B, H, Lq, Ev), device=dev, dtype=torch.float32)
+    lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32)
+    prec = precision_code() if precision is None else precision
+    has, sc = _scale_args(scale)
+    with _on(dev):
+        need = 0
+        if Lq == 1 and k.shape[1] and H % k.shape[1] == 0:
+            need = L.dc_sdpa_window_fwd_workspace_size(B, H, k.shape[1], Lq, S, E, window, sinks)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        r = _refs(q, k, v, mask, lengths, out, lse)
+        st = L.dc_sdpa_window_fwd(*r[:4], window, sinks, offset, r[4], has, sc, prec, r[5], r[6],
+                                  ws.data_ptr() if need else None, need, _stream(dev))
+    _lib.check(st, "sliding window attention failed")
+    return out, lse
+
+
+def _sliding_window_backward(grad_out, q, k, v, out, lse, window, sinks, offset, scale=None, mask=None, precision=None):
+    """Backward of :func:`_sliding_window` (dc_sdpa_window_bwd): (grad_q, grad_k, grad_v)."""
+    L = _lib.load()
+    dev = _device_of(grad_out, q, k, v, out, lse, mask)
+    gq = torch.empty(q.shape, device=dev, dtype=torch.float32)
+    gk = torch.empty(k.shape, device=dev, dtype=torch.float32)
+    gv = torch.empty(v.shape, device=dev, dtype=torch.float32)
+    prec = precision_code() if precision is None else precision
+    has, sc = _scale_args(scale)
+    with _on(dev):
+        nbytes = max(L.dc_sdpa_bwd_workspace_size(q.shape[0], q.shape[1], q.shape[2]), 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        r = _refs(grad_out, q, k, v, out, lse, mask, gq, gk, gv)
+        st = L.dc_sdpa_window_bwd(*r[:7], window, sinks, offset, has, sc, prec, *r[7:], ws.data_ptr(), nbytes,
+                                  _stream(dev))
+    _lib.check(st, "sliding window attention backward failed")
+    return gq, gk, gv
+
+
+def _rotary(q, k, positions, inv_freq, interleaved, amplitude, inverse=False):
+    """Rotary positions of (B, H, L, D) q and k (or None), or the inverse turn (dc_rotary)."""
+    L = _lib.load()
+    dev = _device_of(q, k, positions, inv_freq)
+    yq = torch.empty_like(q)
+    yk = None if k is None else torch.empty_like(k)
+    with _on(dev):
+        r = _refs(q, k, positions, inv_freq, yq, yk)
+        st = L.dc_rotary(*r[:4], int(interleaved), amplitude, int(inverse), r[4], r[5], _stream(dev))
+    _lib.check(st, "rotary positions failed")
+    return yq, yk
+
+
+def _qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, amplitude):
+    """Rotary positions of each head's row over its root mean square (dc_qk_norm_rotary)."""
+    L = _lib.load()
+    dev = _device_of(q, k, wq, wk, positions, inv_freq)
+    yq = torch.empty_like(q)
+    yk = None if k is None else torch.empty_like(k)
+    with _on(dev):
+        r = _refs(q, k, wq, wk, positions, inv_freq, yq, yk)
+        st = L.dc_qk_norm_rotary(*r[:6], eps, int(interleaved), amplitude, r[6], r[7], _stream(dev))
+    _lib.check(st, "normed rotary positions failed")
+    return yq, yk
+
+
+def _qk_norm_rotary_backward(gyq, gyk, q, k, wq, wk, positions, inv_freq, eps, interleaved, amplitude,
+                             weight_grads=(True, True)):
+    """Backward of :func:`_qk_norm_rotary`: (grad_q, grad_k, grad_wq, grad_wk); a weight's gradient is
+    None where there is no weight or ``weight_grads`` says it is not needed."""
+    L = _lib.load()
+    dev = _device_of(gyq, gyk, q, k, wq, wk, positions, inv_freq)
+    gq = torch.empty_like(q)
+    gk = None if k is None else torch.empty_like(k)
+    gws = [torch.empty_like(w) if w is not None and need else None for w, need in zip((wq, wk), weight_grads)]
+    with _on(dev):
+        nbytes = L.dc_qk_norm_rotary_bwd_workspace_size(q.shape[3])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        r = _refs(gyq, gyk, q, k, wq, wk, positions, inv_freq, gq, gk, *gws)
+        st = L.dc_qk_norm_rotary_bwd(*r[:8], eps, int(interleaved), amplitude, *r[8:], ws.data_ptr(), nbytes,
+                                     _stream(dev))
+    _lib.check(st, "normed rotary positions backward failed")
+    return gq, gk, gws[0], gws[1]
+
+
+def _cache4_append(desc, key, value, page_table, start, end=None):
+    """Tokens into a 4-bit cache (dc_cache4_append); ``desc`` is a ``_lib.DcCache4``."""
+    L = _lib.load()
+    dev = _device_of(key, value, page_table, start, end)
+    with _on(dev):
+        st = L.dc_cache4_append(_lib.ref(desc), *_refs(key, value, page_table, start, end), _stream(dev))
+    _lib.check(st, "cache append failed")
+
+
+def _cache4_read(desc, page_table, lengths, max_length):
+    """The first max_length positions of each sequence (dc_cache4_read): (key, value) in float32."""
+    L = _lib.load()
+    dev = _device_of(page_table, lengths)
+    shape = (page_table.shape[0], desc.kv_heads, max_length, desc.head_dim)
+    key = torch.empty(shape, device=dev, dtype=torch.float32)
+    value = torch.empty(shape, device=dev, dtype=torch.float32)
+    with _on(dev):
+        st = L.dc_cache4_read(_lib.ref(desc), *_refs(page_table, lengths, key, value), _stream(dev))
+    _lib.check(st, "cache read failed")
+    return key, value
+
+
+def _cache4_attention(desc, q, page_table, lengths, window=0, sinks=0, scale=None):
+    """One token per sequence over a 4-bit cache (dc_cache4_attention): (out, lse)."""
+    L = _lib.load()
+    dev = _device_of(q, page_table, lengths)
+    B, H = q.shape[:2]
+    out = torch.empty_like(q)
+    lse = torch.empty((B, H, 1), device=dev, dtype=torch.float32)
+    has, sc = _scale_args(scale)
+    with _on(dev):
+        r = _refs(q, page_table, lengths, out, lse)
+        need = 0
+        if H and H % desc.kv_heads == 0:
+            need = L.dc_cache4_attention_workspace_size(B, H, desc.kv_heads, desc.head_dim,
+                                                        page_table.shape[1] * desc.page_size, window, sinks,
+                                                        _lib._DTYPES[q.dtype])
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        st = L.dc_cache4_attention(_lib.ref(desc), *r[:3], window, sinks, has, sc, r[3], r[4],
+                                   ws.data_ptr() if need else None, need, _stream(dev))
+    _lib.check(st, "cache attention failed")
+    return out, lse

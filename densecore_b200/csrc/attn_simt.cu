@@ -70,9 +70,22 @@ __global__ void __launch_bounds__(FW_WARPS *WARP) fwd_simt_kernel(AttnProblem p)
 #pragma unroll
         for (int t = 0; t < T; t++) acc[r][t] = 0.0f;
     }
-    int64_t num_keys = p.S;
+    // One query row of a ragged batch: its sequence's own length and place.
+    if (p.lens) {
+        p.S = max((int64_t)0, min(p.S, (int64_t)p.lens[b * p.lens_stride]));
+        p.offset = p.S - 1;
+    }
+    int64_t num_keys = p.S, skip_to = 0;  // through a window: keys from the sinks up to skip_to are seen by no row
     if (p.causal) num_keys = min(p.S, q0 + FW_BQ);
+    if (p.window) {
+        num_keys = min(p.S, min(q0 + FW_BQ, p.L) + p.offset);
+        skip_to = max((int64_t)0, q0 + p.offset - p.window + 1) / FW_BK * FW_BK;
+    }
     for (int64_t n = 0; n < num_keys; n += FW_BK) {
+        if (n >= p.sinks && n < skip_to) {
+            n = skip_to;
+            if (n >= num_keys) break;
+        }
         __syncthreads();
         for (int idx = threadIdx.x; idx < FW_BK * E; idx += blockDim.x) {
             int j = idx / E, d = idx % E;
@@ -91,12 +104,12 @@ __global__ void __launch_bounds__(FW_WARPS *WARP) fwd_simt_kernel(AttnProblem p)
             const int rr = warp * FW_RPW + r;
             const int64_t i = q0 + rr;
             float s = -INFINITY, z = 1.0f;
-            if (i < p.L && kj < p.S && causal_visible(p.causal, i, kj)) {
+            if (i < p.L && kj < p.S && key_visible(p, i, kj)) {
                 const float *qr = sq + rr * E, *kr = sk + lane * KP;
                 float dot = 0.0f;
                 for (int d = 0; d < E; d++) dot = fmaf(qr[d], kr[d], dot);
                 s = dot * p.scale;
-                if (p.mask_kind) s += mask_value(p, b, h, i, kj);
+                if (p.mask_kind) s = masked_score(p, s, b, h, i, kj);
                 z = keep_factor(p, b, h, i, kj);
             }
             const float m_new = fmaxf(m[r], warp_max(s));
@@ -192,8 +205,9 @@ __global__ void __launch_bounds__(BK_WARPS *WARP) bwd_dkdv_simt_kernel(AttnProbl
         const float *db = g.dout + b * g.dos[0] + h * g.dos[1];
         const float *lb = p.lse + b * p.ls[0] + h * p.ls[1];
         const float *deb = g.delta + (b * p.H + h) * p.L;
-        const int64_t row_start = p.causal ? min(k0, p.L) : 0;
-        for (int64_t r0 = row_start; r0 < p.L; r0 += BK_ROWS) {
+        int64_t row_start = p.causal ? min(k0, p.L) : 0, row_end = p.L;
+        if (p.window) window_rows(p, k0, BK_KEYS, row_start, row_end);
+        for (int64_t r0 = row_start; r0 < row_end; r0 += BK_ROWS) {
             __syncthreads();
             for (int idx = threadIdx.x; idx < BK_ROWS * E; idx += blockDim.x) {
                 int r = idx / E, d = idx % E;
@@ -212,12 +226,12 @@ __global__ void __launch_bounds__(BK_WARPS *WARP) bwd_dkdv_simt_kernel(AttnProbl
             {
                 const int64_t i = r0 + warp;
                 float pr = 0.0f, ds = 0.0f;
-                if (i < p.L && kj < p.S && causal_visible(p.causal, i, kj)) {
+                if (i < p.L && kj < p.S && key_visible(p, i, kj)) {
                     const float *qr = sq + warp * E, *kr = sk + lane * KP;
                     float dot = 0.0f;
                     for (int d = 0; d < E; d++) dot = fmaf(qr[d], kr[d], dot);
                     float s = dot * p.scale;
-                    if (p.mask_kind) s += mask_value(p, b, h, i, kj);
+                    if (p.mask_kind) s = masked_score(p, s, b, h, i, kj);
                     pr = expf(s - srow[2 * warp]);
                     const float *dr = sdo + warp * Ev, *vr = sv + lane * VP;
                     float dp = 0.0f;
@@ -289,9 +303,17 @@ __global__ void __launch_bounds__(BK_WARPS *WARP) bwd_dq_simt_kernel(AttnProblem
     float dq[T];
 #pragma unroll
     for (int t = 0; t < T; t++) dq[t] = 0.0f;
-    int64_t num_keys = p.S;
+    int64_t num_keys = p.S, skip_to = 0;
     if (p.causal) num_keys = min(p.S, q0 + BK_ROWS);
+    if (p.window) {
+        num_keys = min(p.S, min(q0 + BK_ROWS, p.L) + p.offset);
+        skip_to = max((int64_t)0, q0 + p.offset - p.window + 1) / BK_KEYS * BK_KEYS;
+    }
     for (int64_t n = 0; n < num_keys; n += BK_KEYS) {
+        if (n >= p.sinks && n < skip_to) {
+            n = skip_to;
+            if (n >= num_keys) break;
+        }
         __syncthreads();
         for (int idx = threadIdx.x; idx < BK_KEYS * E; idx += blockDim.x) {
             int j = idx / E, d = idx % E;
@@ -304,12 +326,12 @@ __global__ void __launch_bounds__(BK_WARPS *WARP) bwd_dq_simt_kernel(AttnProblem
         __syncthreads();
         const int64_t kj = n + lane;
         float ds = 0.0f;
-        if (i < p.L && kj < p.S && causal_visible(p.causal, i, kj)) {
+        if (i < p.L && kj < p.S && key_visible(p, i, kj)) {
             const float *qr = sq + warp * E, *kr = sk + lane * KP;
             float dot = 0.0f;
             for (int d = 0; d < E; d++) dot = fmaf(qr[d], kr[d], dot);
             float s = dot * p.scale;
-            if (p.mask_kind) s += mask_value(p, b, h, i, kj);
+            if (p.mask_kind) s = masked_score(p, s, b, h, i, kj);
             const float pr = expf(s - lse_i);
             const float *dr = sdo + warp * Ev, *vr = sv + lane * VP;
             float dp = 0.0f;

@@ -194,7 +194,7 @@ __device__ __forceinline__ void row_to_tmem(const uint8_t *raw, uint32_t chunk_b
 // within a head, so that the tiles the hardware runs together share their head's K / V in L2.
 // The same roles and pipelines as the persistent kernel below for a single tile: the raw Q tile
 // waits in the V ring while the K ring fills, and the first V load waits until Q has left.
-template <class C, bool SPLIT, bool MASKED, bool DROP>
+template <class C, bool SPLIT, bool MASKED, bool DROP, bool WIN>
 __global__ void __maxnreg__(128)
     attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                        const __grid_constant__ CUtensorMap tmv, const TcFwdArgs a) {
@@ -208,7 +208,11 @@ __global__ void __maxnreg__(128)
     const int64_t h = blockIdx.y, b = blockIdx.z, hk = h / p.group;
     const int64_t q0 = (int64_t)qt * C::BM;
     const int64_t kv_end = p.causal ? min(p.S, q0 + C::BM) : p.S;
-    const int nblk = (int)((kv_end + C::BN - 1) / C::BN);
+    WindowSpan span{0, 0, (int)((kv_end + C::BN - 1) / C::BN)};
+    if constexpr (WIN) span = window_span<C::BN>(p, q0, C::BM);
+    const int nblk = span.n;
+    // First key of the tile's j-th block.
+    auto key0 = [&](int j) { return (WIN ? span.block(j) : j) * C::BN; };
     auto bar = [&](int i) { return sb + C::OFF_BAR + 8u * (uint32_t)i; };
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sg + C::OFF_MISC);
     volatile int *abort = reinterpret_cast<volatile int *>(sg + C::OFF_MISC + 4);
@@ -274,14 +278,14 @@ __global__ void __maxnreg__(128)
                 mbar_expect_tx(bar(C::K_FULL + ks), C::KV_BYTES);
                 const uint32_t kd = sb + C::OFF_K + ks * C::KV_STAGE;
                 for (int c = 0; c < C::CHUNKS; c++)
-                    tma_load_4d(&tmk, kd + c * C::KV_CHUNK, bar(C::K_FULL + ks), 32 * c, j * C::BN, (int)hk, (int)b);
+                    tma_load_4d(&tmk, kd + c * C::KV_CHUNK, bar(C::K_FULL + ks), 32 * c, key0(j), (int)hk, (int)b);
                 k_issued = j;
                 if (j == 0 && !(ok = mbar_wait(bar(C::Q_READY), 0, abort, err))) break;
                 if (j >= C::VST && !mbar_wait(bar(C::V_EMPTY + vs), ((j / C::VST) - 1) & 1, abort, err)) break;
                 mbar_expect_tx(bar(C::V_FULL + vs), C::KV_BYTES);
                 const uint32_t vd = sb + C::OFF_V + vs * C::KV_STAGE;
                 for (int c = 0; c < C::CHUNKS; c++)
-                    tma_load_4d(&tmv, vd + c * C::KV_CHUNK, bar(C::V_FULL + vs), 32 * c, j * C::BN, (int)hk, (int)b);
+                    tma_load_4d(&tmv, vd + c * C::KV_CHUNK, bar(C::V_FULL + vs), 32 * c, key0(j), (int)hk, (int)b);
                 v_issued = j;
             }
             if (*abort) {
@@ -402,13 +406,16 @@ __global__ void __maxnreg__(128)
         bool ok = true;
         for (int j = 0; j < nblk; j++) {
             const int bb = j & 1;
-            const int64_t k0 = (int64_t)j * C::BN + half * C::HB;
+            const int64_t k0 = (int64_t)key0(j) + half * C::HB;
             // Rows past L (zero-filled by TMA) are computed but never stored. Column c is key
             // k0 + c: valid below S and, under causal masking, up to qrow (one bit per column
             // keeps the edge path as short as the fast one).
-            const bool edge = MASKED || (k0 + C::HB > p.S) || (p.causal && k0 + C::HB - 1 > q0);
+            const bool edge = MASKED || (WIN ? !window_interior(p, q0, C::BM, k0, C::HB)
+                                             : (k0 + C::HB > p.S) || (p.causal && k0 + C::HB - 1 > q0));
             uint32_t vbits = 0xFFFFFFFFu;
-            if (edge) {
+            if (WIN) {
+                if (edge) vbits = row_ok ? window_key_bits(p, qrow, k0) : 0u;
+            } else if (edge) {
                 const int64_t lim = (p.causal ? min(p.S, qrow + 1) : p.S) - k0;
                 const int n = !row_ok || lim <= 0 ? 0 : (lim >= C::HB ? C::HB : (int)lim);
                 vbits = n == 0 ? 0u : (0xFFFFFFFFu >> (32 - n));
@@ -417,6 +424,7 @@ __global__ void __maxnreg__(128)
             // the wait hides their latency.
             float mk[MASKED ? C::HB : 1];
             if constexpr (MASKED) mask_run<C::HB>(p, b, h, qrow, k0, p.ms[3], vbits, mk);
+            if constexpr (MASKED && WIN) vbits = mask_visible(mk, vbits);
             // Dropout: this row's keep bits for these columns (the weights that meet V are
             // P * keep_scale where kept, 0 where dropped; the row sum and lse stay undropped).
             uint32_t kbits = 0;
@@ -596,7 +604,7 @@ __device__ __forceinline__ int64_t fwd_tile_of(int64_t r, int c, int G, int64_t 
 // still work on the current tile; the converters move Q into TMEM once the current tile's last
 // S MMA has read the old Q, and the softmax warps' epilogue (last fold, normalisation, stores)
 // overlaps the next tile's first S MMAs.
-template <class C, bool SPLIT, bool MASKED, bool DROP>
+template <class C, bool SPLIT, bool MASKED, bool DROP, bool WIN>
 __global__ void __maxnreg__(128)
     attn_fwd_tc_persist_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                        const __grid_constant__ CUtensorMap tmv, const TcFwdArgs a) {
@@ -611,6 +619,7 @@ __global__ void __maxnreg__(128)
     constexpr int QS = C::QS, CPS = C::Q_CHUNKS_PER_SLOT;
     // Key blocks of the tile at q0 (causal tiles stop at their last row).
     auto tile_blocks = [&](int64_t q0) {
+        if constexpr (WIN) return window_span<C::BN>(p, q0, C::BM).n;
         const int64_t kv_end = p.causal ? min(p.S, q0 + C::BM) : p.S;
         return (int)((kv_end + C::BN - 1) / C::BN);
     };
@@ -674,6 +683,9 @@ __global__ void __maxnreg__(128)
                 fwd_tile(a, t, q0, h, b);
                 const int64_t hk = h / p.group;
                 const int nblk = tile_blocks(q0);
+                WindowSpan span{};
+                if constexpr (WIN) span = window_span<C::BN>(p, q0, C::BM);
+                auto key0 = [&](int j) { return (WIN ? span.block(j) : j) * C::BN; };
                 // The raw Q tile into the next QS V-ring slots; the converters move it to TMEM.
                 for (int s = 0; s < QS; s++, x++) {
                     const int vs = vslot(x);
@@ -693,7 +705,7 @@ __global__ void __maxnreg__(128)
                     mbar_expect_tx(bar(C::K_FULL + ks), C::KV_BYTES);
                     const uint32_t kd = sb + C::OFF_K + ks * C::KV_STAGE;
                     for (int c = 0; c < C::CHUNKS; c++)
-                        tma_load_4d(&tmk, kd + c * C::KV_CHUNK, bar(C::K_FULL + ks), 32 * c, j * C::BN, (int)hk, (int)b);
+                        tma_load_4d(&tmk, kd + c * C::KV_CHUNK, bar(C::K_FULL + ks), 32 * c, key0(j), (int)hk, (int)b);
                     k_last = kk++;
                     const int vs = vslot(x);
                     if (x >= C::VST && !mbar_wait(bar(C::V_EMPTY + vs), vpar(x - C::VST), abort, err)) {
@@ -703,7 +715,7 @@ __global__ void __maxnreg__(128)
                     mbar_expect_tx(bar(C::V_FULL + vs), C::KV_BYTES);
                     const uint32_t vd = sb + C::OFF_V + vs * C::KV_STAGE;
                     for (int c = 0; c < C::CHUNKS; c++)
-                        tma_load_4d(&tmv, vd + c * C::KV_CHUNK, bar(C::V_FULL + vs), 32 * c, j * C::BN, (int)hk, (int)b);
+                        tma_load_4d(&tmv, vd + c * C::KV_CHUNK, bar(C::V_FULL + vs), 32 * c, key0(j), (int)hk, (int)b);
                     x_last = x++;
                 }
             }
@@ -869,6 +881,9 @@ __global__ void __maxnreg__(128)
             int64_t q0, h, b;
             fwd_tile(a, t, q0, h, b);
             const int nblk = tile_blocks(q0);
+            WindowSpan span{};
+            if constexpr (WIN) span = window_span<C::BN>(p, q0, C::BM);
+            auto key0 = [&](int j) { return (WIN ? span.block(j) : j) * C::BN; };
             const int64_t qrow = q0 + row;
             const bool row_ok = qrow < p.L;
             float m = -INFINITY, l = 0.0f;
@@ -877,13 +892,16 @@ __global__ void __maxnreg__(128)
             for (int x = 0; x < C::HD; x++) o[x] = 0.0f;
             for (int j = 0; j < nblk; j++, jg++) {
                 const int bb = jg & 1;
-                const int64_t k0 = (int64_t)j * C::BN + half * C::HB;
+                const int64_t k0 = (int64_t)key0(j) + half * C::HB;
                 // Rows past L (zero-filled by TMA) are computed but never stored. Column c is key
                 // k0 + c: valid below S and, under causal masking, up to qrow (one bit per column
                 // keeps the edge path as short as the fast one).
-                const bool edge = MASKED || (k0 + C::HB > p.S) || (p.causal && k0 + C::HB - 1 > q0);
+                const bool edge = MASKED || (WIN ? !window_interior(p, q0, C::BM, k0, C::HB)
+                                                 : (k0 + C::HB > p.S) || (p.causal && k0 + C::HB - 1 > q0));
                 uint32_t vbits = 0xFFFFFFFFu;
-                if (edge) {
+                if (WIN) {
+                    if (edge) vbits = row_ok ? window_key_bits(p, qrow, k0) : 0u;
+                } else if (edge) {
                     const int64_t lim = (p.causal ? min(p.S, qrow + 1) : p.S) - k0;
                     const int n = !row_ok || lim <= 0 ? 0 : (lim >= C::HB ? C::HB : (int)lim);
                     vbits = n == 0 ? 0u : (0xFFFFFFFFu >> (32 - n));
@@ -892,6 +910,7 @@ __global__ void __maxnreg__(128)
                 // the wait hides their latency.
                 float mk[MASKED ? C::HB : 1];
                 if constexpr (MASKED) mask_run<C::HB>(p, b, h, qrow, k0, p.ms[3], vbits, mk);
+                if constexpr (MASKED && WIN) vbits = mask_visible(mk, vbits);
                 // Dropout: this row's keep bits for these columns (the weights that meet V are
                 // P * keep_scale where kept, 0 where dropped; the row sum and lse stay undropped).
                 uint32_t kbits = 0;
@@ -1041,16 +1060,24 @@ __global__ void __maxnreg__(128)
     }
 }
 
-// The forward instantiation for (split, masked, dropout): persistent, or one CTA per tile.
+// The forward instantiation for (split, masked, dropout, window): persistent, or one CTA per tile.
+// (Dropout and a window do not meet: sdpa_window has no dropout.)
 template <class C, bool PERSIST>
-decltype(&attn_fwd_tc_kernel<C, true, true, true>) pick_fwd(bool split, bool masked, bool drop) {
-#define DC_FWD(S, M, D) (PERSIST ? attn_fwd_tc_persist_kernel<C, S, M, D> : attn_fwd_tc_kernel<C, S, M, D>)
+decltype(&attn_fwd_tc_kernel<C, true, true, true, false>) pick_fwd(bool split, bool masked, bool drop, bool win) {
+#define DC_FWD(S, M, D) \
+    (PERSIST ? attn_fwd_tc_persist_kernel<C, S, M, D, false> : attn_fwd_tc_kernel<C, S, M, D, false>)
+#define DC_FWD_WIN(S, M) \
+    (PERSIST ? attn_fwd_tc_persist_kernel<C, S, M, false, true> : attn_fwd_tc_kernel<C, S, M, false, true>)
+    if (win)
+        return split ? (masked ? DC_FWD_WIN(true, true) : DC_FWD_WIN(true, false))
+                     : (masked ? DC_FWD_WIN(false, true) : DC_FWD_WIN(false, false));
     if (drop)
         return split ? (masked ? DC_FWD(true, true, true) : DC_FWD(true, false, true))
                      : (masked ? DC_FWD(false, true, true) : DC_FWD(false, false, true));
     return split ? (masked ? DC_FWD(true, true, false) : DC_FWD(true, false, false))
                  : (masked ? DC_FWD(false, true, false) : DC_FWD(false, false, false));
 #undef DC_FWD
+#undef DC_FWD_WIN
 }
 
 template <class C>
@@ -1080,9 +1107,13 @@ int launch_fwd(const AttnProblem &p, int split, cudaStream_t stream) {
     // memory admit one) walking the schedule, so that a tile's start-up overlaps the previous
     // tile's tail; long tiles take one CTA each, which the hardware hands out in schedule order.
     const int64_t sms = device_sm_count();
-    const bool persistent = (p.S + C::BN - 1) / C::BN <= 64 && a.num_tiles < (1ll << 31);
+    // (A window's tiles hold at most its keys, the tile's own and the sinks, each rounded up.)
+    int64_t tile_keys = p.S;
+    if (p.window) tile_keys = min(p.S, min(p.window, p.S) + C::BM + C::BN + min(p.sinks, p.S) + C::BN);
+    const bool persistent = (tile_keys + C::BN - 1) / C::BN <= 64 && a.num_tiles < (1ll << 31);
     const int64_t ctas = persistent && a.num_tiles > sms ? sms : a.num_tiles;
-    auto kernel = persistent ? pick_fwd<C, true>(split, masked, drop) : pick_fwd<C, false>(split, masked, drop);
+    const bool win = p.window != 0;
+    auto kernel = persistent ? pick_fwd<C, true>(split, masked, drop, win) : pick_fwd<C, false>(split, masked, drop, win);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
     if (e != cudaSuccess) return cuda_fail(e, "attn_fwd_tc smem attribute");
     const dim3 grid = persistent ? dim3((unsigned)ctas) : dim3((unsigned)a.num_q_tiles, (unsigned)p.H, (unsigned)p.B);

@@ -372,7 +372,7 @@ struct KvCfg {
 // MMA order per block i: S^T_i, dP^T_i (warp 9), dV_i, dK_i (warp 11). S^T_{i+1} waits for dV_i
 // and runs after dK_i; dP^T_{i+1} waits for dK_i. The softmax warps compute P^T_i while dP^T_i
 // runs and dS^T_i while dV_i runs.
-template <int DD, bool SPLIT, bool MASKED, bool DROP>
+template <int DD, bool SPLIT, bool MASKED, bool DROP, bool WIN>
 __global__ void __maxnreg__(168)
     attn_bwd_dkdv_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                             const __grid_constant__ CUtensorMap tm_qk, const __grid_constant__ CUtensorMap tm_qmn,
@@ -396,9 +396,11 @@ __global__ void __maxnreg__(168)
     const uint32_t bh = (uint32_t)(bhd / C::NH);
     const int64_t hk = bh % (uint32_t)p.Hkv, b = bh / (uint32_t)p.Hkv, k0 = kt * TILE;
     // Query blocks this CTA visits: for each query head of the group, rows [r_begin, L).
-    const int64_t r_begin = p.causal ? min(k0, p.L) : 0;
+    // (through a window, those that see one of this CTA's keys).
+    int64_t r_begin = p.causal ? min(k0, p.L) : 0, r_end = p.L;
+    if constexpr (WIN) window_rows(p, k0, min((int64_t)TILE, p.S - k0), r_begin, r_end);
     const int qb_first = (int)(r_begin / QB);
-    const int qb_per_head = (int)((p.L + QB - 1) / QB) - qb_first;
+    const int qb_per_head = (int)((r_end + QB - 1) / QB) - qb_first;
     const int nblk = qb_per_head * p.group;
     auto bar = [&](int i) { return sb + C::OFF_BAR + 8u * (uint32_t)i; };
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sg + C::OFF_MISC);
@@ -624,12 +626,18 @@ __global__ void __maxnreg__(168)
             if (i + 1 < nblk) colvals(i + 1, nxt_l, nxt_d);
             // Column c is query base + c: valid below L and, under causal masking, from `key` on.
             const int64_t base = q0 + cb;
-            const bool edge = MASKED || !key_ok || q0 + QB > p.L || (p.causal && key > q0);
             uint32_t vbits = 0xFFFFFFFFu;
-            if (edge) vbits = key_ok ? col_bits32(p.causal ? key - base : 0, p.L - base) : 0u;
+            if constexpr (WIN) {  // from key - offset on, up to the window's end (sinks: to the last row)
+                const int64_t last = key < p.sinks ? p.L : min(p.L, key - p.offset + p.window);
+                vbits = key_ok ? col_bits32(key - p.offset - base, last - base) : 0u;
+            } else {
+                const bool edge = MASKED || !key_ok || q0 + QB > p.L || (p.causal && key > q0);
+                if (edge) vbits = key_ok ? col_bits32(p.causal ? key - base : 0, p.L - base) : 0u;
+            }
             // The user mask down this key's column, loaded before the wait for S.
             float mk[MASKED ? CPT : 1];
             if constexpr (MASKED) mask_run<CPT>(p, b, h, base, key, p.ms[2], vbits, mk);
+            if constexpr (MASKED && WIN) vbits = mask_visible(mk, vbits);
             // Dropout: the keep bits of (query base + c, this key). The weights that meet dO are
             // P * Z; dS = P (Z dP - delta), Z = keep_scale where kept, 0 where dropped. The
             // warp's lanes are 32 consecutive keys: one row read per lane, transposed by ballots.
@@ -787,7 +795,7 @@ struct QqCfg {
 // S_j) and dP_{j+1} (once dQ_j has read dS_j); a second issues dQ_j once dS_j is in TMEM. The
 // tensor core thus runs ... dQ_j, dP_{j+1}, S_{j+2}, dQ_{j+1} ... while the softmax warps
 // compute dS_{j+1} under S_{j+2} and P_{j+2} under dQ_{j+1}.
-template <int DD, bool SPLIT, bool MASKED, bool DROP>
+template <int DD, bool SPLIT, bool MASKED, bool DROP, bool WIN>
 __global__ void __maxnreg__(168)
     attn_bwd_dq_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                           const __grid_constant__ CUtensorMap tm_kk, const __grid_constant__ CUtensorMap tm_kmn,
@@ -813,7 +821,11 @@ __global__ void __maxnreg__(168)
     const int64_t h = bh % (uint32_t)p.H, b = bh / (uint32_t)p.H, hk = (uint32_t)h / (uint32_t)p.group;
     const int64_t q0 = qt * TILE;
     const int64_t kv_end = p.causal ? min(p.S, q0 + TILE) : p.S;
-    const int nblk = (int)((kv_end + NB - 1) / NB);
+    WindowSpan span{0, 0, (int)((kv_end + NB - 1) / NB)};
+    if constexpr (WIN) span = window_span<NB>(p, q0, TILE);
+    const int nblk = span.n;
+    // First key of the j-th block.
+    auto key0 = [&](int j) { return (WIN ? span.block(j) : j) * NB; };
     auto bar = [&](int i) { return sb + C::OFF_BAR + 8u * (uint32_t)i; };
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sg + C::OFF_MISC);
     volatile int *abort = reinterpret_cast<volatile int *>(sg + C::OFF_MISC + 4);
@@ -885,8 +897,8 @@ __global__ void __maxnreg__(168)
                 mbar_expect_tx(bar(C::KK_FULL + st), (SPLIT ? 2 : 1) * C::TK_BYTES);
                 for (int c = 0; c < DD / 32; c++) {
                     const uint32_t o = C::OFF_KK + st * C::KSTAGE + c * C::TK_CHUNK;
-                    tma_load_4d(&tm_kk, sb + o, bar(C::KK_FULL + st), 32 * c, j * NB, (int)hk, (int)b);
-                    if (SPLIT) tma_load_4d(&tm_kk_lo, sb + o + C::TK_BYTES, bar(C::KK_FULL + st), 32 * c, j * NB, (int)hk, (int)b);
+                    tma_load_4d(&tm_kk, sb + o, bar(C::KK_FULL + st), 32 * c, key0(j), (int)hk, (int)b);
+                    if (SPLIT) tma_load_4d(&tm_kk_lo, sb + o + C::TK_BYTES, bar(C::KK_FULL + st), 32 * c, key0(j), (int)hk, (int)b);
                 }
                 k_issued = j;
                 if (C::LO_TMEM && j == 0 && !(ok = mbar_wait(bar(C::QD_READY), 0, abort, err))) break;
@@ -894,8 +906,8 @@ __global__ void __maxnreg__(168)
                 mbar_expect_tx(bar(C::VK_FULL + st), (SPLIT ? 2 : 1) * C::TK_BYTES);
                 for (int c = 0; c < DD / 32; c++) {
                     const uint32_t o = C::OFF_VK + st * C::KSTAGE + c * C::TK_CHUNK;
-                    tma_load_4d(&tm_vk, sb + o, bar(C::VK_FULL + st), 32 * c, j * NB, (int)hk, (int)b);
-                    if (SPLIT) tma_load_4d(&tm_vk_lo, sb + o + C::TK_BYTES, bar(C::VK_FULL + st), 32 * c, j * NB, (int)hk, (int)b);
+                    tma_load_4d(&tm_vk, sb + o, bar(C::VK_FULL + st), 32 * c, key0(j), (int)hk, (int)b);
+                    if (SPLIT) tma_load_4d(&tm_vk_lo, sb + o + C::TK_BYTES, bar(C::VK_FULL + st), 32 * c, key0(j), (int)hk, (int)b);
                 }
                 v_issued = j;
             }
@@ -922,8 +934,8 @@ __global__ void __maxnreg__(168)
                 for (int c = 0; c < 2; c++) {
                     const uint32_t o = C::OFF_KMN + st * C::GSTAGE + c * C::TM_CHUNK;
                     const int col = 64 * dh + 32 * c;
-                    tma_load_4d(&tm_kmn, sb + o, bar(C::SG_FULL + st), col, j * NB, (int)hk, (int)b);
-                    if (SPLIT) tma_load_4d(&tm_kmn_lo, sb + o + C::TM_BYTES, bar(C::SG_FULL + st), col, j * NB, (int)hk, (int)b);
+                    tma_load_4d(&tm_kmn, sb + o, bar(C::SG_FULL + st), col, key0(j), (int)hk, (int)b);
+                    if (SPLIT) tma_load_4d(&tm_kmn_lo, sb + o + C::TM_BYTES, bar(C::SG_FULL + st), col, key0(j), (int)hk, (int)b);
                 }
                 issued = j;
                 if (*abort) break;
@@ -1034,14 +1046,18 @@ __global__ void __maxnreg__(168)
         uint32_t zcur = 0;  // its dropout keep bits
         // Reads S_j, releases its columns, and leaves P_j in pv.
         auto load_p = [&](int j) -> bool {
-            const int64_t base = (int64_t)j * NB + cb;
+            const int64_t base = (int64_t)key0(j) + cb;
             // Column c is key base + c: valid below S and, under causal masking, up to q.
-            const bool edge = MASKED || !row_ok || (int64_t)(j + 1) * NB > p.S || (p.causal && (int64_t)(j + 1) * NB - 1 > q0);
             uint32_t vbits = 0xFFFFFFFFu;
-            if (edge) vbits = row_ok ? col_bits32(0, (p.causal ? min(p.S, q + 1) : p.S) - base) : 0u;
+            const bool edge = WIN ? !window_interior(p, q0, TILE, key0(j), NB)
+                                  : MASKED || !row_ok || (int64_t)(j + 1) * NB > p.S || (p.causal && (int64_t)(j + 1) * NB - 1 > q0);
+            if (WIN) {
+                vbits = !row_ok ? 0u : (edge ? window_key_bits(p, q, base) : vbits);
+            } else if (edge) vbits = row_ok ? col_bits32(0, (p.causal ? min(p.S, q + 1) : p.S) - base) : 0u;
             // The user mask along this query's row, loaded before the wait for S.
             float mk[MASKED ? CPT : 1];
             if constexpr (MASKED) mask_run<CPT>(p, b, h, q, base, p.ms[3], vbits, mk);
+            if constexpr (MASKED && WIN) vbits = mask_visible(mk, vbits);
             if constexpr (DROP) zcur = row_ok ? keep_run32(p, b, h, q, base) : 0u;
             if (!warp_wait(bar(C::S_FULL), j & 1, abort, err)) return false;
             tc_fence_after();
@@ -1261,14 +1277,17 @@ int tc_backward_dd(const AttnProblem &p, const AttnGrads &g, int precision, cuda
         if (!st) st = do_maps(tdok, KC::QB, KM);
         if (!st) st = do_maps(tdomn, KC::QB, MN);
         if (st) return st;
-        auto kernel = pick_kernel(split, masked, drop, attn_bwd_dkdv_tc_kernel<DD, true, true, true>,
-                                  attn_bwd_dkdv_tc_kernel<DD, true, true, false>,
-                                  attn_bwd_dkdv_tc_kernel<DD, true, false, true>,
-                                  attn_bwd_dkdv_tc_kernel<DD, true, false, false>,
-                                  attn_bwd_dkdv_tc_kernel<DD, false, true, true>,
-                                  attn_bwd_dkdv_tc_kernel<DD, false, true, false>,
-                                  attn_bwd_dkdv_tc_kernel<DD, false, false, true>,
-                                  attn_bwd_dkdv_tc_kernel<DD, false, false, false>);
+        auto kernel = pick_kernel(split, masked, drop, attn_bwd_dkdv_tc_kernel<DD, true, true, true, false>,
+                                  attn_bwd_dkdv_tc_kernel<DD, true, true, false, false>,
+                                  attn_bwd_dkdv_tc_kernel<DD, true, false, true, false>,
+                                  attn_bwd_dkdv_tc_kernel<DD, true, false, false, false>,
+                                  attn_bwd_dkdv_tc_kernel<DD, false, true, true, false>,
+                                  attn_bwd_dkdv_tc_kernel<DD, false, true, false, false>,
+                                  attn_bwd_dkdv_tc_kernel<DD, false, false, true, false>,
+                                  attn_bwd_dkdv_tc_kernel<DD, false, false, false, false>);
+        if (p.window)  // (dropout and a window do not meet)
+            kernel = split ? (masked ? attn_bwd_dkdv_tc_kernel<DD, true, true, false, true> : attn_bwd_dkdv_tc_kernel<DD, true, false, false, true>)
+                           : (masked ? attn_bwd_dkdv_tc_kernel<DD, false, true, false, true> : attn_bwd_dkdv_tc_kernel<DD, false, false, false, true>);
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)KC::SMEM);
         if (e != cudaSuccess) return cuda_fail(e, "attn_bwd_dkdv_tc smem attribute");
         const unsigned grid = (unsigned)((p.S + TILE - 1) / TILE * p.Hkv * p.B * KC::NH);
@@ -1295,14 +1314,17 @@ int tc_backward_dd(const AttnProblem &p, const AttnGrads &g, int precision, cuda
         if (!st) st = k_maps(tkmn, QC::NB, MN);
         if (!st) st = v_maps(tvk, QC::NB, KM);
         if (st) return st;
-        auto kernel = pick_kernel(split, masked, drop, attn_bwd_dq_tc_kernel<DD, true, true, true>,
-                                  attn_bwd_dq_tc_kernel<DD, true, true, false>,
-                                  attn_bwd_dq_tc_kernel<DD, true, false, true>,
-                                  attn_bwd_dq_tc_kernel<DD, true, false, false>,
-                                  attn_bwd_dq_tc_kernel<DD, false, true, true>,
-                                  attn_bwd_dq_tc_kernel<DD, false, true, false>,
-                                  attn_bwd_dq_tc_kernel<DD, false, false, true>,
-                                  attn_bwd_dq_tc_kernel<DD, false, false, false>);
+        auto kernel = pick_kernel(split, masked, drop, attn_bwd_dq_tc_kernel<DD, true, true, true, false>,
+                                  attn_bwd_dq_tc_kernel<DD, true, true, false, false>,
+                                  attn_bwd_dq_tc_kernel<DD, true, false, true, false>,
+                                  attn_bwd_dq_tc_kernel<DD, true, false, false, false>,
+                                  attn_bwd_dq_tc_kernel<DD, false, true, true, false>,
+                                  attn_bwd_dq_tc_kernel<DD, false, true, false, false>,
+                                  attn_bwd_dq_tc_kernel<DD, false, false, true, false>,
+                                  attn_bwd_dq_tc_kernel<DD, false, false, false, false>);
+        if (p.window)  // (dropout and a window do not meet)
+            kernel = split ? (masked ? attn_bwd_dq_tc_kernel<DD, true, true, false, true> : attn_bwd_dq_tc_kernel<DD, true, false, false, true>)
+                           : (masked ? attn_bwd_dq_tc_kernel<DD, false, true, false, true> : attn_bwd_dq_tc_kernel<DD, false, false, false, true>);
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)QC::SMEM);
         if (e != cudaSuccess) return cuda_fail(e, "attn_bwd_dq_tc smem attribute");
         const unsigned grid = (unsigned)((p.L + TILE - 1) / TILE * p.H * p.B * QC::NH);

@@ -14,6 +14,7 @@
 #include <mutex>
 #include <string>
 
+#include "capi.h"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -42,13 +43,21 @@ int check_launch(const char *what) {
     return e == cudaSuccess ? DC_OK : cuda_fail(e, what);
 }
 
-namespace {
-
 std::string shape_str(const dc_tensor_t *t) {
     std::string s = "(";
     for (int i = 0; i < t->ndim; i++) s += (i ? ", " : "") + std::to_string(t->sizes[i]);
     return s + ")";
 }
+
+int device_ok() {
+    int n = 0;
+    cudaError_t e = cudaGetDeviceCount(&n);
+    if (e != cudaSuccess) return cuda_fail(e, "no CUDA device");
+    if (n == 0) return fail(DC_ERR_CUDA, "no CUDA device");
+    return DC_OK;
+}
+
+namespace {
 
 bool is_f32(const dc_tensor_t *t, int ndim) {
     return t && t->dtype == DC_F32 && t->ndim == ndim;
@@ -61,10 +70,6 @@ bool sizes_are(const dc_tensor_t *t, std::initializer_list<int64_t> want) {
         i++;
     }
     return i == t->ndim;
-}
-
-void copy_strides(const dc_tensor_t *t, int64_t *dst, int n) {
-    for (int i = 0; i < n; i++) dst[i] = t->strides[i];
 }
 
 // attention_dims (src/lib.rs:555-580), generalised to Ev != E.
@@ -143,39 +148,6 @@ int check_precision(int precision) {
         return fail(DC_ERR_VALUE, "unknown precision mode " + std::to_string(precision));
     return DC_OK;
 }
-
-int device_ok() {
-    int n = 0;
-    cudaError_t e = cudaGetDeviceCount(&n);
-    if (e != cudaSuccess) return cuda_fail(e, "no CUDA device");
-    if (n == 0) return fail(DC_ERR_CUDA, "no CUDA device");
-    return DC_OK;
-}
-
-struct ScopedWorkspace {
-    void *ptr = nullptr;
-    bool owned = false;
-    cudaStream_t stream = nullptr;
-    ~ScopedWorkspace() {
-        if (owned && ptr) cudaFreeAsync(ptr, stream);
-    }
-    int get(void *given, size_t given_bytes, size_t need, cudaStream_t s, const char *what) {
-        stream = s;
-        if (need == 0) return DC_OK;
-        if (given) {
-            if (given_bytes < need)
-                return fail(DC_ERR_VALUE, std::string(what) + ": workspace of " +
-                                              std::to_string(given_bytes) + " bytes, " +
-                                              std::to_string(need) + " needed");
-            ptr = given;
-            return DC_OK;
-        }
-        cudaError_t e = cudaMallocAsync(&ptr, need, s);
-        if (e != cudaSuccess) return cuda_fail(e, what);
-        owned = true;
-        return DC_OK;
-    }
-};
 
 int pick_forward_path(const AttnProblem &p, int precision) {
     if (p.L == 1 && decode_supported(p)) return 2;
@@ -315,15 +287,22 @@ size_t dc_sdpa_bwd_workspace_size(int64_t batch, int64_t heads, int64_t q_len) {
     return ((n * sizeof(float) + 255) / 256) * 256;
 }
 
+// A sliding window's arguments (null: none).
+struct WindowArgs {
+    int64_t window, sinks, offset;
+};
+static int fill_window(AttnProblem &p, int64_t window, int64_t sinks, int64_t offset, const dc_tensor_t *lengths);
+
 static int sdpa_bwd_impl(const dc_tensor_t *grad_out, const dc_tensor_t *q, const dc_tensor_t *k,
                          const dc_tensor_t *v, const dc_tensor_t *out, const dc_tensor_t *lse,
                          const dc_tensor_t *mask, int causal, int has_scale, double scale, int precision,
-                         const uint32_t *keep_bits, float keep_scale, bool dropout, dc_tensor_t *grad_q,
-                         dc_tensor_t *grad_k, dc_tensor_t *grad_v, void *workspace, size_t workspace_bytes,
-                         void *stream) {
+                         const uint32_t *keep_bits, float keep_scale, bool dropout, const WindowArgs *win,
+                         dc_tensor_t *grad_q, dc_tensor_t *grad_k, dc_tensor_t *grad_v, void *workspace,
+                         size_t workspace_bytes, void *stream) {
     AttnProblem p;
     int st = fill_problem(q, k, v, causal, has_scale, scale, p);
     if (!st) st = fill_mask(mask, p);
+    if (!st && win) st = fill_window(p, win->window, win->sinks, win->offset, nullptr);
     if (!st) st = check_precision(precision);
     if (!st && dropout) st = set_keep(p, keep_bits, keep_scale);
     if (st) return st;
@@ -369,7 +348,7 @@ int dc_sdpa_bwd(const dc_tensor_t *grad_out, const dc_tensor_t *q, const dc_tens
                 dc_tensor_t *grad_q, dc_tensor_t *grad_k, dc_tensor_t *grad_v, void *workspace,
                 size_t workspace_bytes, void *stream) {
     return sdpa_bwd_impl(grad_out, q, k, v, out, lse, mask, causal, has_scale, scale, precision, nullptr, 0.0f,
-                         false, grad_q, grad_k, grad_v, workspace, workspace_bytes, stream);
+                         false, nullptr, grad_q, grad_k, grad_v, workspace, workspace_bytes, stream);
 }
 
 int dc_sdpa_bwd_dropout(const dc_tensor_t *grad_out, const dc_tensor_t *q, const dc_tensor_t *k,
@@ -378,7 +357,7 @@ int dc_sdpa_bwd_dropout(const dc_tensor_t *grad_out, const dc_tensor_t *q, const
                         const uint32_t *keep_bits, float keep_scale, dc_tensor_t *grad_q, dc_tensor_t *grad_k,
                         dc_tensor_t *grad_v, void *workspace, size_t workspace_bytes, void *stream) {
     return sdpa_bwd_impl(grad_out, q, k, v, out, lse, mask, causal, has_scale, scale, precision, keep_bits,
-                         keep_scale, true, grad_q, grad_k, grad_v, workspace, workspace_bytes, stream);
+                         keep_scale, true, nullptr, grad_q, grad_k, grad_v, workspace, workspace_bytes, stream);
 }
 
 int dc_dropout_keep_bits(const uint32_t *state_in, uint32_t *state_out, int64_t n, double keep_prob,
@@ -473,6 +452,80 @@ int dc_sdpa_decode_noalloc(const dc_tensor_t *q, const dc_tensor_t *k, const dc_
     void *scratch = nullptr;
     if ((st = decode_scratch(&scratch))) return st;
     return decode_forward(p, splits, scratch, static_cast<cudaStream_t>(stream));
+}
+
+// The window arguments of a problem: key distances and offsets beyond the lengths act alike.
+static int fill_window(AttnProblem &p, int64_t window, int64_t sinks, int64_t offset, const dc_tensor_t *lengths) {
+    if (window < 1) return fail(DC_ERR_VALUE, "sliding window attention: the window must be at least 1");
+    if (sinks < 0) return fail(DC_ERR_VALUE, "sliding window attention: sinks must not be negative");
+    const int64_t far = 1ll << 32;
+    if (offset > far || offset < -far)
+        return fail(DC_ERR_VALUE, "sliding window attention: the offset must lie within 2^32 of 0");
+    p.causal = 0;
+    p.window = window < far ? window : far;
+    p.sinks = sinks < far ? sinks : far;
+    p.offset = offset;
+    if (!lengths) return DC_OK;
+    if (lengths->dtype != DC_I32 || lengths->ndim != 1 || lengths->sizes[0] != p.B)
+        return fail(DC_ERR_VALUE, "sliding window attention: lengths must be int32 (B)");
+    if (p.L != 1) return fail(DC_ERR_VALUE, "sliding window attention: lengths take a query length of 1");
+    p.lens = static_cast<const int32_t *>(lengths->data);
+    p.lens_stride = lengths->strides[0];
+    return DC_OK;
+}
+
+size_t dc_sdpa_window_fwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                         int64_t head_dim, int64_t window, int64_t sinks) {
+    if (q_len != 1 || batch <= 0 || kv_heads <= 0 || heads < kv_heads || kv_len <= 0 || (head_dim != 64 && head_dim != 128))
+        return 0;
+    const int splits = window_decode_splits(batch, heads, kv_heads, kv_len, window, sinks);
+    return split_rows_bytes(batch * heads, splits, head_dim);
+}
+
+int dc_sdpa_window_fwd(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *v, const dc_tensor_t *mask,
+                       int64_t window, int64_t sinks, int64_t offset, const dc_tensor_t *lengths, int has_scale,
+                       double scale, int precision, dc_tensor_t *out, dc_tensor_t *lse, void *workspace,
+                       size_t workspace_bytes, void *stream) {
+    AttnProblem p;
+    int st = fill_problem(q, k, v, 0, has_scale, scale, p);
+    if (!st) st = fill_mask(mask, p);
+    if (!st) st = fill_window(p, window, sinks, offset, lengths);
+    if (!st) st = check_out(out, lse, p);
+    if (!st) st = check_precision(precision);
+    if (st) return st;
+    p.out = static_cast<float *>(out->data);
+    p.lse = static_cast<float *>(lse->data);
+    copy_strides(out, p.os, 4);
+    copy_strides(lse, p.ls, 3);
+    if (p.B == 0 || p.H == 0 || p.L == 0) return DC_OK;
+    if ((st = device_ok())) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (precision != DC_PREC_FP32 && !p.lens && p.L > 1 && tc_forward_supported(p)) return tc_forward(p, precision, s);
+    if (!window_decode_supported(p) || p.S == 0) return simt_forward(p, s);
+    SplitRows rows{};
+    rows.splits = window_decode_splits(p.B, p.H, p.Hkv, p.S, p.window, p.sinks);
+    rows.D = (int)p.E;
+    rows.out_dtype = DC_F32;
+    rows.rows = p.B * p.H;
+    rows.H = p.H;
+    rows.out = p.out;
+    rows.lse = p.lse;
+    copy_strides(out, rows.os, 4);
+    copy_strides(lse, rows.ls, 3);
+    ScopedWorkspace ws;
+    if ((st = ws.get(workspace, workspace_bytes, split_rows_bytes(rows.rows, rows.splits, rows.D), s, "window decode workspace")))
+        return st;
+    rows.part = static_cast<float *>(ws.ptr);
+    return window_decode(p, rows, s);
+}
+
+int dc_sdpa_window_bwd(const dc_tensor_t *grad_out, const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *v,
+                       const dc_tensor_t *out, const dc_tensor_t *lse, const dc_tensor_t *mask, int64_t window,
+                       int64_t sinks, int64_t offset, int has_scale, double scale, int precision, dc_tensor_t *grad_q,
+                       dc_tensor_t *grad_k, dc_tensor_t *grad_v, void *workspace, size_t workspace_bytes, void *stream) {
+    const WindowArgs w{window, sinks, offset};
+    return sdpa_bwd_impl(grad_out, q, k, v, out, lse, mask, 0, has_scale, scale, precision, nullptr, 0.0f, false, &w,
+                         grad_q, grad_k, grad_v, workspace, workspace_bytes, stream);
 }
 
 int dc_attn_merge(dc_tensor_t *out_acc, dc_tensor_t *lse_acc, const dc_tensor_t *out_part,

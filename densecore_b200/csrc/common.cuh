@@ -29,6 +29,12 @@ struct AttnProblem {
     // and by 0 otherwise.
     const uint32_t *keep;
     float keep_scale;
+    // Sliding window (0 = none): query row i stands at t = i + offset and sees the keys j <= t
+    // with t - j < window or j < sinks. lens (one query row per sequence only; null = none): the
+    // keys of sequence b are the first lens[b * lens_stride], and its row stands at the last.
+    int64_t window, sinks, offset;
+    const int32_t *lens;
+    int64_t lens_stride;
 };
 
 // Backward extras: grad_out (B,H,L,Ev), dq (B,H,L,E), dk (B,Hkv,S,E), dv (B,Hkv,S,Ev),
@@ -150,6 +156,76 @@ __device__ __forceinline__ uint32_t transpose_bits32(uint32_t w, int lane) {
 // Whether key j is visible to query row i under top-left causal alignment.
 __device__ __forceinline__ bool causal_visible(int causal, int64_t i, int64_t j) {
     return !causal || j <= i;
+}
+
+// Through a window, an additive mask value at or below this hides its key as -inf does, so that
+// masks filled with a type's lowest value act alike in every kernel (times log2(e) that value would
+// overflow to -inf in some of them and not in others).
+constexpr float MASK_HIDES = -1e30f;
+
+// Score s of (i, j) with the user's mask value added.
+__device__ __forceinline__ float masked_score(const AttnProblem &p, float s, int64_t b, int64_t h, int64_t i, int64_t j) {
+    const float mv = mask_value(p, b, h, i, j);
+    return p.window && mv <= MASK_HIDES ? -INFINITY : s + mv;
+}
+
+// Through a window: bit c cleared where mask value mk[c] hides its key (whose score may be a NaN).
+template <int N>
+__device__ __forceinline__ uint32_t mask_visible(const float (&mk)[N], uint32_t bits) {
+#pragma unroll
+    for (int c = 0; c < N; c++)
+        if (mk[c] <= MASK_HIDES) bits &= ~(1u << c);
+    return bits;
+}
+
+// Whether key j is visible to query row i: causal, or through the sliding window.
+__device__ __forceinline__ bool key_visible(const AttnProblem &p, int64_t i, int64_t j) {
+    if (p.window == 0) return causal_visible(p.causal, i, j);
+    const int64_t t = i + p.offset;
+    return j <= t && (t - j < p.window || j < p.sinks);
+}
+
+// The key blocks of BN keys that the query rows [q0, q0 + rows) see through a sliding window:
+// `sink_blocks` blocks from the start, then blocks from `first` on; n of them in all. A tile that
+// sees no key gets one block, whose columns are all masked.
+struct WindowSpan {
+    int sink_blocks, first, n;
+    __device__ __forceinline__ int block(int j) const { return j < sink_blocks ? j : first + j - sink_blocks; }
+};
+
+template <int BN>
+__device__ __forceinline__ WindowSpan window_span(const AttnProblem &p, int64_t q0, int64_t rows) {
+    const int64_t t0 = q0 + p.offset, t1 = min(q0 + rows, p.L) + p.offset;  // [t0, t1)
+    const int64_t hi = max((int64_t)0, min(t1, p.S)), lo = max((int64_t)0, min(t0 - p.window + 1, p.S));
+    WindowSpan s;
+    s.first = (int)(lo / BN);
+    s.sink_blocks = min((int)((min(p.sinks, hi) + BN - 1) / BN), s.first);
+    s.n = s.sink_blocks + max((int)((hi + BN - 1) / BN) - s.first, 0);
+    if (s.n < 1) s.sink_blocks = s.first = 0, s.n = 1;
+    return s;
+}
+
+// Bit c set for c < n, c = 0..31.
+__device__ __forceinline__ uint32_t bits_below(int64_t n) {
+    return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << (int)n) - 1u);
+}
+
+// The keys k0 + c, c = 0..31, that query row i sees through the window, as bits.
+__device__ __forceinline__ uint32_t window_key_bits(const AttnProblem &p, int64_t i, int64_t k0) {
+    const int64_t t = i + p.offset;
+    return bits_below(min(p.S, t + 1) - k0) & (~bits_below(t - p.window + 1 - k0) | bits_below(p.sinks - k0));
+}
+
+// Whether every row of [q0, q0 + rows) below L sees all of the keys [k0, k0 + keys).
+__device__ __forceinline__ bool window_interior(const AttnProblem &p, int64_t q0, int64_t rows, int64_t k0, int64_t keys) {
+    return k0 + keys <= p.S && k0 + keys - 1 <= q0 + p.offset &&
+           (k0 + keys <= p.sinks || min(q0 + rows, p.L) - 1 + p.offset - k0 < p.window);
+}
+
+// The query rows [begin, end) that see some key of [k0, k0 + keys) through the window.
+__device__ __forceinline__ void window_rows(const AttnProblem &p, int64_t k0, int64_t keys, int64_t &begin, int64_t &end) {
+    begin = max((int64_t)0, min(k0 - p.offset, p.L));
+    end = k0 < p.sinks ? p.L : max(begin, min(p.L, k0 + keys - 1 + p.window - p.offset));
 }
 
 // Host side: the thread's last error message and a setter that returns the status.

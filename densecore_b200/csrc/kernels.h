@@ -27,6 +27,77 @@ int decode_pick_splits(const AttnProblem &p);
 size_t decode_workspace_bytes(int64_t B, int64_t H, int64_t Ev, int splits);
 int decode_forward(const AttnProblem &p, int splits, void *workspace, cudaStream_t stream);
 
+// Rows whose keys are split over CTAs (window_decode.cu, cache4.cu): row (b, h) of out (B, H, 1, D)
+// and lse (B, H, 1). With one split the CTA writes its row; otherwise the partial results go to
+// `part` -- per row and split D accumulators, the maximum in base 2 and the sum, both relative to
+// that maximum -- and split_combine joins them in order.
+struct SplitRows {
+    float *part;
+    int splits, D, out_dtype;  // out: float32, float16 or bfloat16
+    int64_t rows, H;
+    void *out;
+    float *lse;
+    int64_t os[4], ls[3];
+};
+size_t split_rows_bytes(int64_t rows, int splits, int64_t D);
+int split_combine(const SplitRows &r, cudaStream_t stream);
+
+// One query row per sequence through a sliding window (window_decode.cu): head dim 64 or 128.
+bool window_decode_supported(const AttnProblem &p);
+int window_decode_splits(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t window, int64_t sinks);
+int window_decode(const AttnProblem &p, const SplitRows &rows, cudaStream_t stream);
+
+// Rotary positions (rotary.cu). op[0] is the queries, op[1] the keys (x null: none); per operand
+// x, y and (norm backward) the upstream gradient g are (B, H, L, D) views of one type, w the norm's
+// weight and gw its gradient (float32 or that type; either may be null).
+struct RotaryOperand {
+    const void *x, *g, *w;
+    void *y, *gw;
+    float *wpart;  // norm backward: the blocks' parts of gw
+    int64_t xs[4], gs[4], ys[4], ws, gws;
+    int H, w_dtype, gw_dtype, heads_per_item, chunks;
+};
+struct RotaryArgs {
+    RotaryOperand op[2];
+    int64_t B, L;
+    int D, rot, lpr_log, blocks_q;
+    const void *positions;
+    int pos64;
+    int64_t ps[2];  // (batch, token) strides of the positions
+    const double *freq;
+    int64_t freq_stride;
+    float amplitude, eps, inv_D;
+    int inverse;
+};
+enum RotaryMode { ROTARY_ROTATE = 0, ROTARY_NORM = 1, ROTARY_NORM_BWD = 2 };
+size_t rotary_bwd_workspace_bytes(int64_t D);
+int rotary_launch(RotaryArgs &a, int dtype, bool interleaved, int mode, cudaStream_t stream);
+
+// The 4-bit key/value cache (cache4.cu).
+struct Cache4 {
+    uint8_t *codes;    // (pages, 2, Hkv, page_size, D / 2)
+    uint32_t *scales;  // (pages, 2, Hkv, page_size, D / 32): scale | low << 16, bfloat16 each
+    int64_t pages;
+    int Hkv, D, page_size;
+};
+struct Cache4Args {
+    Cache4 c;
+    const int32_t *table, *lens, *starts, *ends;  // (B, P) page ids, (B) lengths / first / end positions
+    int64_t ts[2], lens_stride, starts_stride, ends_stride;
+    int64_t B, H, T, P;  // P: page table entries per sequence; T: tokens of an append or read
+    const void *x[2];    // append: key, value; attention: x[0] the queries
+    float *y[2];         // read: key, value
+    int64_t xs[2][4], ys[2][4];
+    int dtype;
+    float scale;
+    int64_t window, sinks;
+    int *err;
+};
+int cache4_append(const Cache4Args &a, cudaStream_t stream);
+int cache4_read(const Cache4Args &a, cudaStream_t stream);
+int cache4_splits(int64_t B, int64_t H, int64_t Hkv, int64_t capacity, int64_t window, int64_t sinks, int dtype);
+int cache4_attention(const Cache4Args &a, const SplitRows &rows, cudaStream_t stream);
+
 // tcgen05 tensor-core kernels (attn_tc.cu, attn_tc_bwd.cu). Forward: head dim 64 or 128,
 // E == Ev, unit-stride rows on 16-byte boundaries. Backward: E == Ev == 64, any strides (its
 // pre-pass copies the operands into contiguous TF32 hi / lo buffers); it also writes delta.

@@ -13,6 +13,7 @@ import numbers
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 from . import random as _random
@@ -177,6 +178,232 @@ def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.
     else:
         out, _lse = flash_attention(q, k, v, is_causal, float(scale), mask)
     return out.squeeze(1) if rank == 3 else out
+
+
+def _whole_number(name, value, least=None):
+    if isinstance(value, (bool, np.bool_)) or not isinstance(value, numbers.Integral):
+        raise TypeError(f"{name} must be a whole number")
+    if least is not None and value < least:
+        raise ValueError(f"{name} must be at least {least}")
+    if abs(int(value)) >= 1 << 62:
+        raise ValueError(f"{name} is out of range")
+    return int(value)
+
+
+class _SlidingWindow(torch.autograd.Function):
+    """Attention through a sliding window; saves q, k, v, out, lse."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, offset, scale, mask):
+        out, lse = _native._sliding_window(q, k, v, window, sinks, offset, scale, mask)
+        ctx.save_for_backward(q, k, v, out, lse, *(() if mask is None else (mask,)))
+        ctx.window, ctx.sinks, ctx.offset, ctx.scale = window, sinks, offset, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, *mask = ctx.saved_tensors
+        gq, gk, gv = _native._sliding_window_backward(grad, q, k, v, out, lse, ctx.window, ctx.sinks, ctx.offset,
+                                                      ctx.scale, mask[0] if mask else None)
+        return gq, gk, gv, None, None, None, None, None
+
+
+def sliding_window_attention(query, key, value, window, sinks=0, attn_mask=None, lengths=None, offset=None, scale=None,
+                             enable_gqa=False):
+    """Causal attention in which each query sees the last ``window`` keys and the first ``sinks``.
+
+    query (B, H, L, E), key (B, H, S, E), value (B, H, S, Ev), or rank 3 without the head dim, float32 as
+    :func:`scaled_dot_product_attention`; with ``enable_gqa`` key and value may have H / n heads. Query
+    row i stands at position t = i + ``offset`` (default S - L: the queries are the last L of the S
+    tokens) and sees the keys j <= t with t - j < window or j < sinks, where ``attn_mask`` (bool, True
+    may attend, or float32, added to the scores; a value of -1e30 or less hides its key as -inf does)
+    lets it. ``lengths`` (int32 (B), L == 1, no gradient) are the keys that each sequence of a padded cache holds:
+    its row stands at the last of them. A row that sees no key gives 0 and zero gradients. scale
+    defaults to 1/sqrt(E). Not in DenseCore; the rules are those of its SDPA (functional.py:276-340).
+    """
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"attention {name} must be a Tensor")
+    rank = query.dim()
+    if rank not in (3, 4) or key.dim() != rank or value.dim() != rank:
+        raise ValueError("attention query, key and value must all be rank 3 or all rank 4")
+    q, k, v = (t.unsqueeze(1) for t in (query, key, value)) if rank == 3 else (query, key, value)
+    b, heads, length, embed = q.shape
+    kv, source = k.shape[1], k.shape[2]
+    grouped = enable_gqa and kv > 0 and heads % kv == 0
+    if (k.shape[0] != b or v.shape[0] != b or v.shape[1] != kv or not (kv == heads or grouped) or k.shape[3] != embed
+            or v.shape[2] != source):
+        raise ValueError("attention shapes must be (..., L, E), (..., S, E), (..., S, Ev)")
+    window, sinks = _whole_number("window", window, 1), _whole_number("sinks", sinks, 0)
+    if scale is None:
+        scale = 1.0 / math.sqrt(embed) if embed else 1.0
+    elif isinstance(scale, (bool, np.bool_)) or not isinstance(scale, numbers.Real):
+        raise TypeError("scale must be real")
+    for t in (query, key, value):
+        if t.dtype != torch.float32:
+            raise TypeError(f"attention tensors must be float32, got {t.dtype}")
+    if lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32:
+            raise TypeError("lengths must be an int32 Tensor")
+        if tuple(lengths.shape) != (b,):
+            raise ValueError(f"lengths must be ({b},), got {tuple(lengths.shape)}")
+        if length != 1 or offset is not None:
+            raise ValueError("lengths take a query length of 1 and no offset")
+    offset = source - length if offset is None else _whole_number("offset", offset)
+    mask = _flash_mask(_as_mask(attn_mask, query.device), rank)
+    grad = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)
+    if grad:
+        if lengths is not None:
+            raise NotImplementedError("sliding window attention with lengths has no gradient")
+        out = _SlidingWindow.apply(q, k, v, window, sinks, offset, float(scale), mask)
+    else:
+        out, _lse = _native._sliding_window(q, k, v, window, sinks, offset, float(scale), mask, lengths)
+    return out.squeeze(1) if rank == 3 else out
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_length=None, fast=32.0, slow=1.0,
+                       device=None):
+    """(inv_freq, amplitude) for :func:`rotary_embedding`: the float64 angles per position of the
+    ``rotary_dim // 2`` pairs, base^(-2i/rotary_dim), and the factor of the rotated channels.
+
+    ``scaling`` for contexts ``factor`` times longer than those trained on: None; "linear" (positions
+    interpolated: every frequency over factor); "ntk" (the base raised to base * factor^(d/(d-2)), so
+    that the fastest frequency stays and the slowest is interpolated); "yarn" (frequencies that make
+    more than ``fast`` turns over ``original_length`` stay, those below ``slow`` are interpolated, linear
+    in between; amplitude 0.1 ln(factor) + 1).
+    """
+    d = _whole_number("rotary_dim", rotary_dim, 2)
+    if d % 2:
+        raise ValueError("rotary_dim must be even")
+    if not (base > 0 and factor > 0):
+        raise ValueError("base and factor must be positive")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError('scaling must be None, "linear", "ntk" or "yarn"')
+    if scaling == "ntk":
+        if d < 4:
+            raise ValueError("ntk scaling needs a rotary_dim of at least 4")
+        base = base * factor ** (d / (d - 2))
+    freq = float(base) ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    amplitude = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if original_length is None or not fast > slow:
+            raise ValueError("yarn scaling needs original_length, and fast above slow")
+        keep = ((original_length * freq / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        freq = freq * keep + freq / factor * (1.0 - keep)
+        amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    return freq.to(device), amplitude
+
+
+_ROTARY_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _rotary_args(what, query, key, positions, inv_freq, interleaved, amplitude):
+    """Checks of the rotary operators; query and key as (B, H, L, D)."""
+    for name, t in (("query", query), ("key", key)):
+        if name == "key" and t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what} {name} must be a Tensor")
+        if t.dtype not in _ROTARY_TYPES:
+            raise TypeError(f"{what} tensors must be float32, float16 or bfloat16, got {t.dtype}")
+        if t.dtype != query.dtype:
+            raise TypeError(f"{what} query and key must have one type")
+        if t.dim() not in (3, 4) or t.dim() != query.dim():
+            raise ValueError(f"{what} query and key must both be rank 3 or both rank 4")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be an int32 or int64 Tensor")
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64:
+        raise TypeError("inv_freq must be a float64 Tensor")
+    if type(interleaved) is not bool:
+        raise TypeError("interleaved must be a bool")
+    if isinstance(amplitude, (bool, np.bool_)) or not isinstance(amplitude, numbers.Real):
+        raise TypeError("amplitude must be real")
+    if query.dim() == 3:
+        return query.unsqueeze(1), None if key is None else key.unsqueeze(1)
+    return query, key
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, amplitude):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.interleaved, ctx.amplitude = interleaved, amplitude
+        return _native._rotary(q, k, positions, inv_freq, interleaved, amplitude)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        positions, inv_freq = ctx.saved_tensors
+        gq, gk = _native._rotary(gq, gk, positions, inv_freq, ctx.interleaved, ctx.amplitude, inverse=True)
+        return gq, gk, None, None, None, None
+
+
+def rotary_embedding(query, key, positions, inv_freq, *, interleaved=False, amplitude=1.0):
+    """(query, key) with the first ``2 * len(inv_freq)`` channels of every head turned by their position.
+
+    query (B, H, L, D) and key (B, Hkv, L, D; or None), or rank 3 without the head dim, in float32,
+    float16 or bfloat16, any strides, D even and at most 256; positions int32 or int64, (L) or (B, L);
+    inv_freq float64 (:func:`rotary_frequencies`). Pair i of channels, (i, i + len(inv_freq)) or, with
+    ``interleaved``, (2i, 2i + 1), turns by positions * inv_freq[i]; ``amplitude`` multiplies the turned
+    channels and the others pass through. Not in DenseCore, whose nanoGPT path adds learned positions.
+    """
+    q, k = _rotary_args("rotary", query, key, positions, inv_freq, interleaved, amplitude)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        q, k = _Rotary.apply(q, k, positions, inv_freq, interleaved, float(amplitude))
+    else:
+        q, k = _native._rotary(q, k, positions, inv_freq, interleaved, float(amplitude))
+    if query.dim() == 3:
+        return q.squeeze(1), None if k is None else k.squeeze(1)
+    return q, k
+
+
+class _QKNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, positions, inv_freq, eps, interleaved, amplitude):
+        ctx.save_for_backward(q, k, wq, wk, positions, inv_freq)
+        ctx.rest = (eps, interleaved, amplitude)
+        return _native._qk_norm_rotary(q, k, wq, wk, positions, inv_freq, eps, interleaved, amplitude)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        gq, gk, gwq, gwk = _native._qk_norm_rotary_backward(gq, gk, *ctx.saved_tensors, *ctx.rest,
+                                                            weight_grads=ctx.needs_input_grad[2:4])
+        return gq, gk, gwq, gwk, None, None, None, None, None
+
+
+def qk_norm_rotary(query, key, query_weight, key_weight, positions, inv_freq, *, eps=1e-6, interleaved=False,
+                   amplitude=1.0):
+    """:func:`rotary_embedding` of each head's row over its root mean square, x / sqrt(mean(x^2) + eps) *
+    weight, in one pass. Weights are (D), float32 or of the inputs' type, or None for ones; their
+    gradients are summed over every row in a fixed order."""
+    q, k = _rotary_args("normed rotary", query, key, positions, inv_freq, interleaved, amplitude)
+    for w in (query_weight, key_weight):
+        if w is None:
+            continue
+        if not isinstance(w, torch.Tensor):
+            raise TypeError("norm weights must be Tensors")
+        if w.dtype not in (torch.float32, query.dtype):
+            raise TypeError(f"norm weights must be float32 or {query.dtype}, got {w.dtype}")
+        if tuple(w.shape) != (query.shape[-1],):
+            raise ValueError(f"norm weights must be ({query.shape[-1]},), got {tuple(w.shape)}")
+    if key is None and key_weight is not None:
+        raise ValueError("a key weight needs a key")
+    if isinstance(eps, (bool, np.bool_)) or not isinstance(eps, numbers.Real):
+        raise TypeError("eps must be real")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    args = (q, k, query_weight, key_weight, positions, inv_freq, float(eps), interleaved, float(amplitude))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        q, k = _QKNormRotary.apply(*args)
+    else:
+        q, k = _native._qk_norm_rotary(*args)
+    if query.dim() == 3:
+        return q.squeeze(1), None if k is None else k.squeeze(1)
+    return q, k
 
 
 def _float_mask(mask):

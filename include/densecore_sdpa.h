@@ -19,6 +19,9 @@
  *                    src/torch_random.rs:242-254) as a device bit mask
  *   dc_sdpa_fwd_dropout / dc_sdpa_bwd_dropout / dc_attn_probs_dropout  SDPA and MHA with
  *                    dropout_p > 0 (functional.py:312-340, :450-451), fused
+ *   dc_sdpa_window_fwd / _bwd, dc_rotary, dc_qk_norm_rotary / _bwd, dc_cache4_*
+ *                    sliding windows, rotary positions, normed queries and keys, and a key/value
+ *                    cache in 4 bits around that path (no reference counterpart)
  *   dc_rng_skip      host-side skip-ahead of the generator state (no reference counterpart)
  *   dc_last_error    the message of the last failure on this thread (PyErr text in lib.rs)
  *
@@ -74,7 +77,9 @@ enum dc_status {
     DC_ERR_UNSUPPORTED = 4  /* valid request this build does not implement */
 };
 
-enum dc_dtype { DC_F32 = 0, DC_BOOL = 1 };
+/* The attention entry points take DC_F32 (and DC_BOOL masks); the others of this list are for the
+ * entry points that name them. */
+enum dc_dtype { DC_F32 = 0, DC_BOOL = 1, DC_F16 = 2, DC_BF16 = 3, DC_I32 = 4, DC_I64 = 5, DC_F64 = 6 };
 
 enum dc_precision { DC_PREC_3XTF32 = 0, DC_PREC_TF32 = 1, DC_PREC_FP32 = 2 };
 
@@ -154,6 +159,117 @@ DC_API int dc_sdpa_decode_noalloc(const dc_tensor_t *q, const dc_tensor_t *k, co
  * reference has no sequence parallelism). */
 DC_API int dc_attn_merge(dc_tensor_t *out_acc, dc_tensor_t *lse_acc, const dc_tensor_t *out_part,
                   const dc_tensor_t *lse_part, void *stream);
+
+/* ---- Sliding-window attention (no counterpart in the reference) ----
+ * Query row i stands at position t = i + offset among the S keys (offset = S - L puts the queries
+ * at the end, as prefill and decode do; 0 is the reference's top-left alignment) and sees the keys
+ * j <= t with t - j < window or j < sinks. lengths (nullable; q_len 1 only): int32 (B), the keys of
+ * sequence b are its first lengths[b] (clamped to 0..S) and its row stands at the last of them;
+ * offset is then not used. mask, scale, precision, out, lse and rows that see no key are as in
+ * dc_sdpa_fwd, with one difference: a float mask value of -1e30 or less hides its key as -inf does.
+ * Keys that no row of a 128-row query tile sees are not read; key and value are taken as finite
+ * where a tile sees them. Shapes the tensor-core kernels do not cover run the CUDA-core kernels. */
+
+/* Bytes of scratch dc_sdpa_window_fwd needs (0 unless q_len is 1 and the keys are split). */
+DC_API size_t dc_sdpa_window_fwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                int64_t q_len, int64_t kv_len, int64_t head_dim,
+                                                int64_t window, int64_t sinks);
+
+/* Forward: out (B,H,L,Ev) and lse (B,H,L); window >= 1, sinks >= 0. workspace may be NULL (then
+ * the library takes stream-ordered memory). */
+DC_API int dc_sdpa_window_fwd(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *v,
+                              const dc_tensor_t *mask, int64_t window, int64_t sinks,
+                              int64_t offset, const dc_tensor_t *lengths, int has_scale,
+                              double scale, int precision, dc_tensor_t *out, dc_tensor_t *lse,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
+/* Backward of dc_sdpa_window_fwd (without lengths); arguments and workspace as dc_sdpa_bwd. */
+DC_API int dc_sdpa_window_bwd(const dc_tensor_t *grad_out, const dc_tensor_t *q,
+                              const dc_tensor_t *k, const dc_tensor_t *v, const dc_tensor_t *out,
+                              const dc_tensor_t *lse, const dc_tensor_t *mask, int64_t window,
+                              int64_t sinks, int64_t offset, int has_scale, double scale,
+                              int precision, dc_tensor_t *grad_q, dc_tensor_t *grad_k,
+                              dc_tensor_t *grad_v, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
+/* ---- Rotary positions, alone or behind a norm of each head (no counterpart in the reference) ----
+ * q (B, H, L, D) and k (B, Hkv, L, D; nullable) of one type, float32, float16 or bfloat16, any
+ * strides, D even and at most 256; positions int32 or int64, (L) or (B, L), any value; inv_freq
+ * float64 (r), the angle per position of the r pairs: channels (i, r + i), or (2 i, 2 i + 1) when
+ * interleaved. A pair (a, b) becomes amplitude * (a cos - b sin, b cos + a sin); channels from 2 r on
+ * pass through. Arithmetic is in 32 bits (angles in 64), rounded once. Outputs have the inputs'
+ * shapes and type, any strides, and may be the inputs themselves. */
+
+/* inverse != 0 turns by the negative angles: the gradient of the inputs from the outputs'. */
+DC_API int dc_rotary(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *positions,
+                     const dc_tensor_t *inv_freq, int interleaved, double amplitude, int inverse,
+                     dc_tensor_t *q_out, dc_tensor_t *k_out, void *stream);
+
+/* rotary(x / sqrt(mean(x^2) + eps) * weight) over each head's D channels. Weights (D), float32 or of
+ * the inputs' type; null means ones. */
+DC_API int dc_qk_norm_rotary(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *q_weight,
+                             const dc_tensor_t *k_weight, const dc_tensor_t *positions,
+                             const dc_tensor_t *inv_freq, double eps, int interleaved,
+                             double amplitude, dc_tensor_t *q_out, dc_tensor_t *k_out, void *stream);
+
+/* Its backward: q_grad, k_grad are the outputs' gradients; writes the inputs' gradients to q_out,
+ * k_out (not the same memory as q_grad, k_grad, q or k) and the weights' (nullable; float32 or of
+ * the inputs' type), summed over all rows in a fixed order. workspace: nullable, of
+ * dc_qk_norm_rotary_bwd_workspace_size() bytes. */
+DC_API size_t dc_qk_norm_rotary_bwd_workspace_size(int64_t head_dim);
+DC_API int dc_qk_norm_rotary_bwd(const dc_tensor_t *q_grad, const dc_tensor_t *k_grad,
+                                 const dc_tensor_t *q, const dc_tensor_t *k,
+                                 const dc_tensor_t *q_weight, const dc_tensor_t *k_weight,
+                                 const dc_tensor_t *positions, const dc_tensor_t *inv_freq,
+                                 double eps, int interleaved, double amplitude, dc_tensor_t *q_out,
+                                 dc_tensor_t *k_out, dc_tensor_t *q_weight_grad,
+                                 dc_tensor_t *k_weight_grad, void *workspace,
+                                 size_t workspace_bytes, void *stream);
+
+/* ---- Paged key/value cache in 4 bits (no counterpart in the reference) ----
+ * Position p of a sequence lies in slot p % page_size of page page_table[b][p / page_size]. Each
+ * group of 32 channels of a token and head is held as low = its least value rounded down to
+ * bfloat16, scale = (its largest - low) / 15 rounded up to bfloat16, and codes = (x - low) / scale
+ * rounded to nearest even, in 32-bit arithmetic; it stands for low + scale * code. A group with an
+ * infinity or a NaN stands for NaN.
+ *  codes   num_pages * 2 * kv_heads * page_size * head_dim / 2 bytes, scales 4 bytes per group;
+ *          16-byte aligned device memory of the caller's. All zero is a cache of zeros.
+ *  Page tables (B, P), lengths, start and end positions (B) are int32 device tensors. A position
+ *  outside the table, a length outside 0..P * page_size or a page id outside 0..num_pages - 1 sets
+ *  dc_device_status() to 3; it is then not written, reads as zero, or is left out of the attention
+ *  (lengths are clamped). Entries behind a sequence's length are not read. */
+typedef struct dc_cache4 {
+    void *codes;
+    void *scales;
+    int64_t num_pages;
+    int32_t kv_heads, head_dim, page_size; /* head_dim 64, 128 or 256; page_size a multiple of 16 */
+} dc_cache4_t;
+
+/* Token i of key, value (B, kv_heads, T, head_dim; one of float32, float16, bfloat16; any strides)
+ * goes to position start[b] + i, where that is below end[b] (nullable). One call must not write a
+ * slot twice: two sequences of it must not append to a page that they share. */
+DC_API int dc_cache4_append(const dc_cache4_t *cache, const dc_tensor_t *key,
+                            const dc_tensor_t *value, const dc_tensor_t *page_table,
+                            const dc_tensor_t *start, const dc_tensor_t *end, void *stream);
+
+/* The first T positions of each sequence as float32 (B, kv_heads, T, head_dim), zeros from
+ * lengths[b] on. */
+DC_API int dc_cache4_read(const dc_cache4_t *cache, const dc_tensor_t *page_table,
+                          const dc_tensor_t *lengths, dc_tensor_t *key, dc_tensor_t *value,
+                          void *stream);
+
+/* Attention of one token per sequence over its first lengths[b] positions, standing at the last:
+ * q (B, H, 1, head_dim) float32, float16 or bfloat16, H a multiple of kv_heads; window == 0 sees all
+ * of them, window >= 1 those less than `window` back and the first `sinks`. out has q's type; lse
+ * (B, H, 1) float32. An empty sequence gives out = 0, lse = 0. */
+DC_API size_t dc_cache4_attention_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                 int64_t head_dim, int64_t capacity,
+                                                 int64_t window, int64_t sinks, int dtype);
+DC_API int dc_cache4_attention(const dc_cache4_t *cache, const dc_tensor_t *q,
+                               const dc_tensor_t *page_table, const dc_tensor_t *lengths,
+                               int64_t window, int64_t sinks, int has_scale, double scale,
+                               dc_tensor_t *out, dc_tensor_t *lse, void *workspace,
+                               size_t workspace_bytes, void *stream);
 
 /* ---- Ring attention (sequence parallelism over an NCCL communicator) ----
  * NCCL's communicator type: ncclComm_t in nccl.h is `struct ncclComm *`. */
@@ -261,7 +377,8 @@ DC_API int dc_kernel_timing_report(char *buf, size_t len, int reset);
 /* Device-side status of the library's kernels: 0; 1 when a tensor-core kernel gave up on a
  * wait that did not complete within its bound (1 s) -- that CTA then unwound without writing
  * its outputs; 2 when dc_dropout_keep_bits read a generator state whose `left` word is not in
- * 1..624 -- it then wrote neither mask nor state. Synchronises with the device. reset != 0
+ * 1..624 -- it then wrote neither mask nor state; 3 when a cache entry point met a length, a
+ * position or a page id out of range. Synchronises with the device. reset != 0
  * clears the status. -1 on a CUDA error. */
 DC_API int dc_device_status(int reset);
 

@@ -1,0 +1,214 @@
+"""Sliding-window attention against the formula in 64 bits.
+
+Tolerance: the bar of the other attention kernels, max|delta| <= 1e-5 max|ref| (3xTF32 products are off
+by about 2^-21 of their absolute terms, the fp32 kernels by less; scores here stay below 10, so weights
+are off by a few 1e-6). Single-pass TF32 rounds operands to 11 bits: 2^-11 of the absolute terms of a
+score, sums of D products of random sign; 1e-2."""
+import math
+
+import pytest
+import torch
+
+import densecore_b200 as dc
+from densecore_b200 import functional as F
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(q, k, v, window, sinks, offset, mask=None, lens=None, scale=None):
+    q, k, v = q.double(), k.double(), v.double()
+    h, kv = q.shape[1], k.shape[1]
+    k, v = (t.repeat_interleave(h // kv, 1) for t in (k, v))
+    s = q @ k.transpose(2, 3) * (1 / math.sqrt(q.shape[3]) if scale is None else scale)
+    i, j = torch.arange(q.shape[2], device="cuda")[:, None], torch.arange(k.shape[2], device="cuda")
+    t = (i + offset)[None] if lens is None else (lens.clamp(0, k.shape[2]).long() - 1)[:, None, None]
+    vis = (j <= t) & ((t - j < window) | (j < sinks))
+    vis = vis[:, None]
+    if mask is not None:
+        if mask.dtype == torch.bool:
+            vis = vis & mask
+        else:
+            vis = vis & (mask > -1e30)
+            s = s + mask.clamp_min(-1e30).double()
+    s = torch.where(vis, s, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    p = (s - torch.where(top == -math.inf, 0.0, top)).exp()
+    total = p.sum(-1, keepdim=True)
+    return (p / torch.where(total == 0, 1.0, total)) @ v
+
+
+def rel(got, ref):
+    assert torch.isfinite(got).all()
+    scale = ref.abs().max().item() if ref.numel() else 0.0
+    return (got.double() - ref).abs().max().item() / (scale or 1.0) if ref.numel() else 0.0
+
+
+def make(b, h, kv, l, s, d, layout, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *x: torch.randn(x, generator=g, device="cuda")
+    if layout == "bshd":
+        return r(b, l, h, d).transpose(1, 2), r(b, s, kv, d).transpose(1, 2), r(b, s, kv, d).transpose(1, 2)
+    if layout == "odd":  # no TMA: rows at odd strides
+        return r(b, h, l, d + 1)[..., 1:], r(b, kv, s, d + 1)[..., 1:], r(b, kv, s, d + 3)[..., :d]
+    return r(b, h, l, d), r(b, kv, s, d), r(b, kv, s, d)
+
+
+def check(q, k, v, window, sinks, offset=None, mask=None, tol=1e-5, scale=None):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = F.sliding_window_attention(*leaves, window, sinks, attn_mask=mask, offset=offset, scale=scale, enable_gqa=True)
+    go = torch.randn(out.shape, device="cuda")
+    grads = torch.autograd.grad(out, leaves, go)
+    refs = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    ro = reference(*refs, window, sinks, k.shape[2] - q.shape[2] if offset is None else offset, mask, scale=scale)
+    rg = torch.autograd.grad(ro, refs, go.double())
+    for name, a, r in zip(("out", "dq", "dk", "dv"), (out, *grads), (ro, *rg)):
+        assert rel(a.detach(), r.detach()) <= tol, (name, rel(a.detach(), r.detach()))
+    assert dc._lib.load().dc_device_status(1) == 0
+    return out.detach(), grads
+
+
+CASES = [  # b, h, kv, l, s, d, window, sinks, offset
+    (1, 1, 1, 1, 1, 64, 1, 0, None), (2, 3, 3, 17, 17, 64, 5, 2, None), (1, 2, 2, 129, 129, 64, 64, 0, None),
+    (2, 4, 2, 300, 300, 64, 33, 4, None), (1, 2, 1, 257, 257, 128, 100, 1, None), (1, 2, 2, 640, 640, 64, 128, 130, None),
+    (1, 2, 2, 100, 700, 64, 200, 3, None), (1, 1, 1, 64, 1000, 128, 1, 1, None), (2, 2, 2, 200, 90, 64, 20, 2, None),
+    (1, 2, 2, 200, 200, 64, 20, 2, 0), (1, 2, 2, 150, 150, 128, 40, 0, 70), (1, 2, 2, 150, 150, 64, 40, 5, -60),
+    (1, 1, 1, 50, 50, 64, 10, 2, -200), (1, 1, 1, 50, 50, 64, 10, 2, 400), (1, 1, 1, 50, 50, 64, 10, 0, 400),
+    (1, 2, 2, 130, 130, 64, 10 ** 12, 0, None), (1, 1, 1, 130, 130, 64, 7, 10 ** 12, None), (1, 8, 1, 70, 333, 64, 90, 64, None),
+    (1, 2, 2, 40, 40, 32, 9, 3, None), (1, 2, 1, 75, 130, 20, 17, 40, None), (1, 1, 1, 33, 70, 256, 12, 3, None),
+    (1, 2, 2, 1, 500, 64, 100, 4, None), (2, 4, 2, 1, 500, 128, 100, 4, None)]
+
+
+@pytest.mark.parametrize("layout", ["plain", "bshd", "odd"])
+@pytest.mark.parametrize("case", CASES)
+def test_forward_and_backward(case, layout):
+    b, h, kv, l, s, d, window, sinks, offset = case
+    check(*make(b, h, kv, l, s, d, layout), window, sinks, offset)
+
+
+@pytest.mark.parametrize("d", [64, 128, 48])
+@pytest.mark.parametrize("kind", ["padding", "left", "rows", "bias", "lowest", "inf", "full"])
+def test_masks(kind, d):
+    b, h, s = 2, 4, 200
+    q, k, v = make(b, h, 2, s, s, d, "bshd", 3)
+    j = torch.arange(s, device="cuda")
+    mask = {
+        "padding": lambda: (j < torch.tensor([150, 60], device="cuda")[:, None])[:, None, None],
+        "left": lambda: (j >= torch.tensor([150, 0], device="cuda")[:, None])[:, None, None],  # empty first rows
+        "rows": lambda: (torch.arange(s, device="cuda") % 3 != 0)[:, None].expand(s, s),  # every third row empty
+        "bias": lambda: torch.randn(1, h, s, s, device="cuda"),
+        "lowest": lambda: torch.where(j % 2 == 0, torch.finfo(torch.float32).min, 0.5).expand(1, 1, s, s).clone(),
+        "inf": lambda: torch.where(j < 120, -math.inf, 0.0).expand(s, s).clone(),
+        "full": lambda: torch.rand(b, h, s, s, device="cuda") < 0.5,
+    }[kind]()
+    out, grads = check(q, k, v, 40, 0 if kind in ("inf", "left") else 4, mask=mask)
+    if kind == "rows":
+        assert (out[:, :, ::3] == 0).all() and (grads[0][:, :, ::3] == 0).all()
+    if kind == "lowest":  # a row of lowest values only sees nothing: row 0 of a window of one
+        low = torch.full((s, s), torch.finfo(torch.float32).min, device="cuda")
+        assert (F.sliding_window_attention(q, k, v, 40, 4, attn_mask=low, enable_gqa=True) == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 32])
+def test_hidden_keys_may_hold_anything(d):
+    # Infinities and NaN in keys that a bool or -inf mask hides do not reach the scores; masked values
+    # must be finite.
+    s = 150
+    q, k, v = make(1, 2, 2, s, s, d, "plain", 4)
+    hide = torch.zeros(s, dtype=torch.bool, device="cuda")
+    hide[10:30] = True
+    bad = k.clone()
+    bad[:, :, 10:20], bad[:, :, 20:30] = math.nan, math.inf
+    clean = F.sliding_window_attention(q, k, v, 50, 4, attn_mask=~hide.expand(s, s))
+    assert torch.equal(F.sliding_window_attention(q, bad, v, 50, 4, attn_mask=~hide.expand(s, s)), clean)
+    minus = torch.where(hide, -math.inf, 0.0).expand(s, s).clone()
+    assert rel(F.sliding_window_attention(q, bad, v, 50, 4, attn_mask=minus), clean.double()) <= 1e-6
+
+
+def test_long_windows_take_the_one_tile_kernel():
+    # window + tile + sinks over 64 key blocks at head dim 128
+    q, k, v = make(1, 1, 1, 4000, 4000, 128, "bshd", 5)
+    check(q, k, v, 2500, 4)
+    q, k, v = make(1, 2, 2, 6000, 6000, 64, "bshd", 6)
+    check(q, k, v, 5000, 70)
+
+
+def test_whole_window_is_causal_attention():
+    q, k, v = make(2, 3, 3, 333, 333, 64, "bshd", 7)
+    causal = dc.scaled_dot_product_attention(q, k, v, is_causal=True)
+    assert torch.equal(F.sliding_window_attention(q, k, v, 333), causal)
+
+
+@pytest.mark.parametrize("mode,tol", [("fp32", 1e-5), ("tf32", 1e-2)])
+def test_precisions(mode, tol):
+    dc.set_sdpa_precision(mode)
+    try:
+        for d in (64, 128):
+            check(*make(1, 2, 1, 200, 260, d, "bshd", 8), 64, 3, tol=tol)
+    finally:
+        dc.set_sdpa_precision(None)
+
+
+def test_negative_and_zero_scale():
+    q, k, v = make(1, 2, 2, 140, 140, 64, "bshd", 9)
+    for scale in (-0.2, 0.0, 1.0):
+        check(q, k, v, 30, 2, scale=scale)
+
+
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("heads", [(4, 4), (4, 2), (8, 2), (12, 4), (8, 1), (5, 1)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (64, 4), (700, 100), (10 ** 6, 0)])
+def test_single_token_with_lengths(d, heads, window, sinks):
+    h, kv = heads
+    s = 777
+    lens = torch.tensor([0, 1, 5, 64, 300, 776, 777, 12], dtype=torch.int32, device="cuda")
+    b = len(lens)
+    q, k, v = make(b, h, kv, 1, s, d, "plain", 11)
+    for i, n in enumerate(lens.tolist()):  # what lies behind a sequence's end is never used
+        k[i, :, n:], v[i, :, n:] = math.nan, math.nan
+    got = F.sliding_window_attention(q, k, v, window, sinks, lengths=lens, enable_gqa=True)
+    ref = reference(q, torch.nan_to_num(k), torch.nan_to_num(v), window, sinks, 0, lens=lens)
+    assert rel(got, ref) <= 1e-5
+    assert (got[0] == 0).all()
+    strided = F.sliding_window_attention(q, k, v, window, sinks, lengths=lens.repeat_interleave(3)[::3], enable_gqa=True)
+    assert torch.equal(strided, got)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_single_token_masks_and_batch_of_one(d):
+    q, k, v = make(1, 8, 2, 1, 5000, d, "bshd", 12)
+    ref = reference(q, k, v, 3000, 8, 4999)
+    got = F.sliding_window_attention(q, k, v, 3000, 8, enable_gqa=True)
+    assert rel(got, ref) <= 1e-5
+    bias = torch.randn(1, 8, 1, 5000, device="cuda")
+    assert rel(F.sliding_window_attention(q, k, v, 3000, 8, attn_mask=bias, enable_gqa=True),
+               reference(q, k, v, 3000, 8, 4999, bias)) <= 1e-5
+    hide = (torch.arange(5000, device="cuda") < 4990)
+    assert rel(F.sliding_window_attention(q, k, v, 5, 0, attn_mask=hide.view(1, 1, 1, -1), enable_gqa=True),
+               reference(q, k, v, 5, 0, 4999, hide.view(1, 1, 1, -1))) == 0.0  # a row that sees nothing
+    low = torch.full((1, 1, 1, 5000), torch.finfo(torch.float32).min, device="cuda")
+    low[..., 4999] = 0
+    assert rel(F.sliding_window_attention(q, k, v, 100, 4, attn_mask=low, enable_gqa=True),
+               reference(q, k, v, 100, 4, 4999, low)) <= 1e-5
+    lse = dc._native._sliding_window(q, k, v, 3000, 8, 4999)[1]
+    x = (q.double().view(2, 4, d) @ k[0].double().transpose(1, 2)) / math.sqrt(d)
+    x = torch.cat((x[..., :8], x[..., 2000:]), -1)
+    assert (lse.view(2, 4).double() - x.logsumexp(-1)).abs().max() <= 1e-5
+
+
+def test_rank_three_and_empty():
+    q = torch.randn(2, 9, 64, device="cuda")
+    got = F.sliding_window_attention(q, q, q, 4, 1)
+    assert rel(got[:, None], reference(q[:, None], q[:, None], q[:, None], 4, 1, 0)) <= 1e-5
+    for shape_q, shape_k in (((0, 2, 3, 64), (0, 2, 3, 64)), ((1, 2, 0, 64), (1, 2, 5, 64)), ((1, 2, 4, 64), (1, 2, 0, 64)),
+                             ((1, 2, 1, 64), (1, 2, 0, 64))):
+        a, c = torch.randn(shape_q, device="cuda", requires_grad=True), torch.randn(shape_k, device="cuda", requires_grad=True)
+        y = F.sliding_window_attention(a, c, c, 3, 1)
+        y.sum().backward()
+        assert y.shape == a.shape and (y == 0).all() and (c.grad == 0).all()
+
+
+def test_repeats_bit_for_bit():
+    q, k, v = make(2, 4, 2, 500, 500, 64, "bshd", 13)
+    first = check(q, k, v, 60, 4)[0]
+    for _ in range(3):
+        assert torch.equal(F.sliding_window_attention(q, k, v, 60, 4, enable_gqa=True), first)
