@@ -81,104 +81,124 @@ __device__ __forceinline__ void load4(const T *p, int64_t inner, bool vec, float
     }
 }
 
-// Where four channels of a token live: halfword `half` of row `row` of `page`.
+// Row of `slot` of `page` in the codes and scales.
 __device__ __forceinline__ int64_t cache_row(const Cache4 &c, int64_t page, int which, int head, int slot) {
     return (((page * 2 + which) * c.Hkv + head) * c.page_size + slot);
 }
 
-// The page of position pos of sequence b, or -1 (and the device status) where the table has none.
-__device__ __forceinline__ int64_t page_of(const Cache4Args &a, int64_t b, int64_t pos) {
-    const int64_t entry = pos / a.c.page_size;
-    if (pos >= 0 && entry < a.P) {
+// The row of position pos of sequence b, or -1 (and the device status) where the table has none.
+__device__ __forceinline__ int64_t row_of(const Cache4Args &a, int64_t b, int64_t pos, int which, int head) {
+    if (pos >= 0 && pos < a.P * a.c.page_size) {
+        const uint32_t entry = (uint32_t)pos / (uint32_t)a.c.page_size, slot = (uint32_t)pos - entry * (uint32_t)a.c.page_size;
         const int64_t page = a.table[b * a.ts[0] + entry * a.ts[1]];
-        if (page >= 0 && page < a.c.pages) return page;
+        if (page >= 0 && page < a.c.pages) return cache_row(a.c, page, which, head, (int)slot);
     }
     atomicExch(a.err, BAD_TABLE);
     return -1;
 }
 
-// A thread takes four channels of one (sequence, token, head); eight neighbours make a group.
-// blockIdx.y: keys or values.
+// Filling and reading back are bound by HBM. A block takes a run of tokens of one (sequence, head) of
+// the keys or the values (grid: token runs, 2 Hkv, B); a thread four channels of ROWS tokens, whose
+// loads are issued together; eight neighbours make a group of 32.
+constexpr int ROWS = 4;
+
+// rint(d / scale) of the correctly rounded quotient, by a product with the reciprocal where that
+// cannot round the other way (the product is off by less than 1e-5 for quotients up to 15).
+__device__ __forceinline__ float code_of(float d, float scale, float inv) {
+    const float q = d * inv;
+    float c = rintf(q);
+    if (!(fabsf(q - c) < 0.4999f)) c = rintf(__fdiv_rn(d, scale));
+    return fminf(fmaxf(c, 0.0f), 15.0f);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Args a, bool vec) {
-    const int which = blockIdx.y, lanes = a.c.D / 4;
-    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, row = idx / lanes;
-    const int quad = (int)(idx - row * lanes), g = quad / 8, r = quad % 8;
-    const int64_t rows = a.B * a.T * a.c.Hkv;
-    const bool live = row < rows;
-    const int64_t bt = (live ? row : 0) / a.c.Hkv, b = bt / a.T, t = bt - b * a.T;
-    const int head = (int)((live ? row : 0) - bt * a.c.Hkv);
-    const int64_t pos = a.starts[b * a.starts_stride] + t;
-    float x[4] = {};
-    const bool wanted = live && !(a.ends && pos >= a.ends[b * a.ends_stride]);
-    if (wanted) {
-        const T *src = static_cast<const T *>(a.x[which]) + b * a.xs[which][0] + head * a.xs[which][1] + t * a.xs[which][2] +
-                       (int64_t)(4 * quad) * a.xs[which][3];
-        load4(src, a.xs[which][3], vec, x);
-    }
-    float mn = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    bool finite = true;
+    const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
+    const int64_t b = blockIdx.z;
+    const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes;
+    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS) + threadIdx.x / lanes, start = a.starts[b * a.starts_stride];
+    const int64_t last = min(a.T, a.ends ? a.ends[b * a.ends_stride] - start : a.T);  // tokens from here on stay out
+    const T *src = static_cast<const T *>(a.x[which]) + b * a.xs[which][0] + head * a.xs[which][1] + (int64_t)(4 * quad) * a.xs[which][3];
+    float x[ROWS][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) finite = finite && fabsf(x[i]) <= 3.402823466e38f;
-    if (!finite) mx = INFINITY;
+    for (int i = 0; i < ROWS; i++) {
+        const int64_t t = t0 + i * pass;
+        if (t < last) {
+            load4(src + t * a.xs[which][2], a.xs[which][3], vec, x[i]);
+        } else {
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-        mn = fminf(mn, __shfl_xor_sync(ALL, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(ALL, mx, o));
-    }
-    if (!wanted) return;
-    // low: bits below bfloat16 cut, one step further down for a negative value that had some.
-    uint32_t lb = __float_as_uint(mn);
-    if ((lb >> 31) && (lb & 0xFFFFu)) lb += 0x10000u;
-    lb &= 0xFFFF0000u;
-    const float low = __uint_as_float(lb);
-    const float width = __fdiv_rn(__fsub_rn(mx, low), 15.0f);
-    uint32_t sb = (__float_as_uint(width) + 0xFFFFu) & 0xFFFF0000u;  // up to bfloat16 (width >= 0)
-    uint32_t codes = 0;
-    if (!(fabsf(low) <= 3.402823466e38f) || !(width <= 3.3e38f)) {
-        lb = sb = 0x7FC00000u;  // NaN
-    } else if (sb) {
-        const float scale = __uint_as_float(sb);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], low), scale)), 0.0f), 15.0f);
-            codes |= (uint32_t)c << (4 * i);
+            for (int e = 0; e < 4; e++) x[i][e] = 0.0f;
         }
     }
-    const int64_t page = page_of(a, b, pos);
-    if (page < 0) return;
-    const int ng = a.c.D / GROUP;
-    const int64_t at = cache_row(a.c, page, which, head, (int)(pos % a.c.page_size));
-    reinterpret_cast<uint16_t *>(a.c.codes + at * (a.c.D / 2))[r * ng + g] = (uint16_t)codes;
-    if (r == 0) a.c.scales[at * ng + g] = (sb >> 16) | lb;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const int64_t t = t0 + i * pass;
+        float mn = fminf(fminf(x[i][0], x[i][1]), fminf(x[i][2], x[i][3]));
+        float mx = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
+        bool finite = true;
+#pragma unroll
+        for (int e = 0; e < 4; e++) finite = finite && fabsf(x[i][e]) <= 3.402823466e38f;
+        if (!finite) mx = INFINITY;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            mn = fminf(mn, __shfl_xor_sync(ALL, mn, o));
+            mx = fmaxf(mx, __shfl_xor_sync(ALL, mx, o));
+        }
+        if (t >= last) continue;
+        // low: bits below bfloat16 cut, one step further down for a negative value that had some.
+        uint32_t lb = __float_as_uint(mn);
+        if ((lb >> 31) && (lb & 0xFFFFu)) lb += 0x10000u;
+        lb &= 0xFFFF0000u;
+        const float low = __uint_as_float(lb);
+        const float width = __fdiv_rn(__fsub_rn(mx, low), 15.0f);
+        uint32_t sb = (__float_as_uint(width) + 0xFFFFu) & 0xFFFF0000u;  // up to bfloat16 (width >= 0)
+        uint32_t codes = 0;
+        if (!(fabsf(low) <= 3.402823466e38f) || !(width <= 3.3e38f)) {
+            lb = sb = 0x7FC00000u;  // NaN
+        } else if (sb) {
+            const float scale = __uint_as_float(sb);
+            const float inv = scale > 1e-37f && scale < 1e37f ? __frcp_rn(scale) : NAN;  // NaN: divide
+#pragma unroll
+            for (int e = 0; e < 4; e++) codes |= (uint32_t)code_of(__fsub_rn(x[i][e], low), scale, inv) << (4 * e);
+        }
+        const int64_t at = row_of(a, b, start + t, which, head);
+        if (at < 0) continue;
+        reinterpret_cast<uint16_t *>(a.c.codes + at * (a.c.D / 2))[r * ng + g] = (uint16_t)codes;
+        if (r == 0) a.c.scales[at * ng + g] = (sb >> 16) | lb;
+    }
 }
 
 // Token t of sequence b from the cache, in float32; zeros from the sequence's length on.
 __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bool vec) {
-    const int which = blockIdx.y, lanes = a.c.D / 4, ng = a.c.D / GROUP;
-    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, row = idx / lanes;
-    const int quad = (int)(idx - row * lanes), g = quad / 8, r = quad % 8;
-    if (row >= a.B * a.T * a.c.Hkv) return;
-    const int64_t bh = row / a.T, t = row - bh * a.T, b = bh / a.c.Hkv;
-    const int head = (int)(bh - b * a.c.Hkv);
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (t < a.lens[b * a.lens_stride]) {
-        const int64_t page = page_of(a, b, t);
-        if (page >= 0) {
-            const int64_t at = cache_row(a.c, page, which, head, (int)(t % a.c.page_size));
-            const uint32_t codes = reinterpret_cast<const uint16_t *>(a.c.codes + at * (a.c.D / 2))[r * ng + g];
-            const uint32_t sl = a.c.scales[at * ng + g];
-            const float scale = bf16_low(sl), low = bf16_high(sl);
-            y = make_float4(fmaf(scale, (float)(codes & 15u), low), fmaf(scale, (float)((codes >> 4) & 15u), low),
-                            fmaf(scale, (float)((codes >> 8) & 15u), low), fmaf(scale, (float)(codes >> 12), low));
+    const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
+    const int64_t b = blockIdx.z;
+    const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes;
+    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS) + threadIdx.x / lanes, len = a.lens[b * a.lens_stride];
+    uint32_t codes[ROWS], sl[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const int64_t t = t0 + i * pass;
+        codes[i] = sl[i] = 0u;  // a zero
+        const int64_t at = t < a.T && t < len ? row_of(a, b, t, which, head) : -1;
+        if (at >= 0) {
+            codes[i] = reinterpret_cast<const uint16_t *>(a.c.codes + at * (a.c.D / 2))[r * ng + g];
+            sl[i] = a.c.scales[at * ng + g];
         }
     }
-    float *dst = a.y[which] + b * a.ys[which][0] + head * a.ys[which][1] + t * a.ys[which][2] + (int64_t)(4 * quad) * a.ys[which][3];
-    if (vec) {
-        *reinterpret_cast<float4 *>(dst) = y;
-    } else {
-        const int64_t s = a.ys[which][3];
-        dst[0] = y.x, dst[s] = y.y, dst[2 * s] = y.z, dst[3 * s] = y.w;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const int64_t t = t0 + i * pass;
+        if (t >= a.T) continue;
+        const float scale = bf16_low(sl[i]), low = bf16_high(sl[i]);
+        const float4 y = make_float4(fmaf(scale, (float)(codes[i] & 15u), low), fmaf(scale, (float)((codes[i] >> 4) & 15u), low),
+                                     fmaf(scale, (float)((codes[i] >> 8) & 15u), low), fmaf(scale, (float)(codes[i] >> 12), low));
+        float *dst = a.y[which] + b * a.ys[which][0] + head * a.ys[which][1] + t * a.ys[which][2] + (int64_t)(4 * quad) * a.ys[which][3];
+        if (vec) {
+            *reinterpret_cast<float4 *>(dst) = y;
+        } else {
+            const int64_t s = a.ys[which][3];
+            dst[0] = y.x, dst[s] = y.y, dst[2 * s] = y.z, dst[3 * s] = y.w;
+        }
     }
 }
 
@@ -569,27 +589,26 @@ bool vec4(const void *ptr, const int64_t *st, int size) {
 
 }  // namespace
 
+// Grid of the fill and read kernels.
+dim3 token_grid(const Cache4Args &a) {
+    const int64_t run = 256 / (a.c.D / 4) * ROWS;
+    return dim3((unsigned)((a.T + run - 1) / run), (unsigned)(2 * a.c.Hkv), (unsigned)a.B);
+}
+
 int cache4_append(const Cache4Args &a, cudaStream_t stream) {
-    const int64_t threads = a.B * a.T * a.c.Hkv * (a.c.D / 4), blocks = (threads + 255) / 256;
-    if (blocks == 0) return DC_OK;
-    if (blocks >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "cache append: more than 2^31 blocks of tokens");
     const int size = a.dtype == DC_F32 ? 4 : 2;
     const bool vec = vec4(a.x[0], a.xs[0], size) && vec4(a.x[1], a.xs[1], size);
-    const dim3 grid((unsigned)blocks, 2);
     KernelTrace tr("cache4_append", stream);
-    if (a.dtype == DC_F32) cache4_append_kernel<float><<<grid, 256, 0, stream>>>(a, vec);
-    else if (a.dtype == DC_F16) cache4_append_kernel<__half><<<grid, 256, 0, stream>>>(a, vec);
-    else cache4_append_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a, vec);
+    if (a.dtype == DC_F32) cache4_append_kernel<float><<<token_grid(a), 256, 0, stream>>>(a, vec);
+    else if (a.dtype == DC_F16) cache4_append_kernel<__half><<<token_grid(a), 256, 0, stream>>>(a, vec);
+    else cache4_append_kernel<__nv_bfloat16><<<token_grid(a), 256, 0, stream>>>(a, vec);
     return check_launch("cache4_append");
 }
 
 int cache4_read(const Cache4Args &a, cudaStream_t stream) {
-    const int64_t threads = a.B * a.T * a.c.Hkv * (a.c.D / 4), blocks = (threads + 255) / 256;
-    if (blocks == 0) return DC_OK;
-    if (blocks >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "cache read: more than 2^31 blocks of tokens");
     const bool vec = vec4(a.y[0], a.ys[0], 4) && vec4(a.y[1], a.ys[1], 4);
     KernelTrace tr("cache4_read", stream);
-    cache4_read_kernel<<<dim3((unsigned)blocks, 2), 256, 0, stream>>>(a, vec);
+    cache4_read_kernel<<<token_grid(a), 256, 0, stream>>>(a, vec);
     return check_launch("cache4_read");
 }
 

@@ -87,8 +87,8 @@ int fill_cache(const dc_cache4_t *cache, Cache4 &c) {
     if (!cache || !cache->codes || !cache->scales) return fail(DC_ERR_VALUE, "cache: codes and scales are required");
     if ((reinterpret_cast<uintptr_t>(cache->codes) & 15u) || (reinterpret_cast<uintptr_t>(cache->scales) & 15u))
         return fail(DC_ERR_VALUE, "cache: codes and scales must be 16-byte aligned");
-    if (cache->num_pages < 1 || cache->num_pages > 0x7fffffff || cache->kv_heads < 1)
-        return fail(DC_ERR_VALUE, "cache: pages and heads must be at least 1, pages below 2^31");
+    if (cache->num_pages < 1 || cache->num_pages > 0x7fffffff || cache->kv_heads < 1 || cache->kv_heads > 32767)
+        return fail(DC_ERR_VALUE, "cache: pages and heads must be at least 1, pages below 2^31, heads below 2^15");
     if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
         return fail(DC_ERR_UNSUPPORTED, "cache: the head dim must be 64, 128 or 256");
     if (cache->page_size < 16 || cache->page_size % 16) return fail(DC_ERR_VALUE, "cache: the page size must be a multiple of 16");
@@ -211,7 +211,7 @@ int dc_qk_norm_rotary_bwd(const dc_tensor_t *q_grad, const dc_tensor_t *k_grad, 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ScopedWorkspace scratch;
     if ((st = scratch.get(workspace, workspace_bytes, rotary_bwd_workspace_bytes(a.D), s, "normed rotary backward workspace"))) return st;
-    a.op[0].wpart = static_cast<float *>(scratch.ptr);
+    a.wpart = static_cast<float *>(scratch.ptr);
     return rotary_launch(a, q->dtype, interleaved != 0, ROTARY_NORM_BWD, s);
 }
 
@@ -227,6 +227,7 @@ int dc_cache4_append(const dc_cache4_t *cache, const dc_tensor_t *key, const dc_
         key->sizes[0] != a.B || key->sizes[1] != a.c.Hkv || key->sizes[3] != a.c.D)
         return fail(DC_ERR_VALUE, "cache append: keys and values must be (B, kv heads, T, head dim) of one float type");
     a.T = key->sizes[2];
+    if (a.T >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "cache append: 2^31 tokens and more");
     a.dtype = key->dtype;
     a.x[0] = key->data;
     a.x[1] = value->data;
@@ -248,6 +249,7 @@ int dc_cache4_read(const dc_cache4_t *cache, const dc_tensor_t *page_table, cons
         key->sizes[0] != a.B || key->sizes[1] != a.c.Hkv || key->sizes[3] != a.c.D || overlaps(key) || overlaps(value))
         return fail(DC_ERR_VALUE, "cache read: keys and values must be float32 (B, kv heads, T, head dim)");
     a.T = key->sizes[2];
+    if (a.T >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "cache read: 2^31 tokens and more");
     a.y[0] = static_cast<float *>(key->data);
     a.y[1] = static_cast<float *>(value->data);
     copy_strides(key, a.ys[0], 4);

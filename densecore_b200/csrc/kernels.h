@@ -53,14 +53,14 @@ int window_decode(const AttnProblem &p, const SplitRows &rows, cudaStream_t stre
 struct RotaryOperand {
     const void *x, *g, *w;
     void *y, *gw;
-    float *wpart;  // norm backward: the blocks' parts of gw
     int64_t xs[4], gs[4], ys[4], ws, gws;
-    int H, w_dtype, gw_dtype, heads_per_item, chunks;
+    int H, w_dtype, gw_dtype;
 };
 struct RotaryArgs {
     RotaryOperand op[2];
     int64_t B, L;
-    int D, rot, lpr_log, blocks_q;
+    int D, rot, lpr_log, heads_per_item, chunks;
+    float *wpart;  // norm backward: the blocks' parts of the weight gradients, queries then keys
     const void *positions;
     int pos64;
     int64_t ps[2];  // (batch, token) strides of the positions

@@ -12,14 +12,17 @@
 //              gx = r (gn - n mean(gn n)), with r recomputed from x
 //
 // Bound: HBM. Each element is read once and written once (the backward of the norm reads x and g),
-// and about ten instructions an element are far below what the loads allow, so the design is about
-// wide loads and about not paying for the angles:
-//   * a row is held by D / (2 V) lanes (V = 16 bytes of elements): a lane owns both members of its
-//     V pairs, so the rotation needs no exchange and the norm one butterfly over the row's lanes;
-//   * a warp takes one token and a run of its heads, and computes each lane's V sines and cosines
-//     once for the run. The angle is reduced to a fraction of a turn in 64 bits (position 10^6 in
-//     32 bits would already be 0.06 rad off), its sine and cosine taken in 32. No table: nothing
-//     bounds the positions, and nothing else is read;
+// and some seven instructions an element are below what the loads allow, as long as the angles cost
+// little beside them:
+//   * a row is held by D / 8 lanes, two pieces of four channels each: a lane owns both members of its
+//     four pairs, so the rotation needs no exchange and the norm one butterfly over the row's lanes.
+//     (Pieces of 16 bytes in the 16-bit types, eight channels, cost twice the registers and spilled:
+//     the norm of 40 heads of 8188 tokens took 101 us against the 26 of its bytes.)
+//   * a warp takes one token and a run of its heads, queries then keys. The run's sines and cosines
+//     are computed once, two or four to a lane, and handed out through shared memory. The angle is
+//     reduced to a fraction of a turn in 64 bits (position 10^6 in 32 bits would already be 0.06 rad
+//     off), its sine and cosine taken in 32. No table: nothing bounds the positions, and nothing
+//     else is read;
 //   * runs are cut short (down to one row a lane group) when a call has too few tokens to fill the
 //     GPU, as in a decode step;
 //   * the weight gradients are summed in fixed order: per lane over its rows, then over the warps
@@ -31,6 +34,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -41,18 +45,10 @@ namespace {
 
 constexpr int WPB = 8;  // warps per block
 constexpr unsigned ALL = 0xffffffffu;
-constexpr int BWD_BLOCKS = 592;  // blocks of the norm's backward: 4 of 8 warps on each of 148 SMs
+constexpr int MAX_BWD_BLOCKS = 296;  // blocks of the norm's backward: 2 of 8 warps on each of 148 SMs
+constexpr int MAX_PAIRS = 128;
 
 constexpr int ROTATE = ROTARY_ROTATE, NORM = ROTARY_NORM, NORM_BWD = ROTARY_NORM_BWD;
-
-template <typename T>
-__device__ __forceinline__ float to_f(T x);
-template <>
-__device__ __forceinline__ float to_f<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 template <typename T>
 __device__ __forceinline__ T from_f(float x);
@@ -63,32 +59,49 @@ __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// One piece of a row: V elements as loaded.
+// One piece of a row, V elements as loaded: kept as words until they are used (as separate 16-bit
+// elements they took a register each, and the loads in flight spilled).
 template <typename T, int V>
 struct Piece {
-    T e[V];
+    static constexpr int WORDS = V == 1 ? 1 : V * (int)sizeof(T) / 4;
+    uint32_t w[WORDS];
+
+    // V == 1 reads at any element stride; pieces of four elements lie on a boundary of their size.
+    __device__ __forceinline__ void load(const T *row, int at, int64_t inner) {
+        if constexpr (V == 1) {
+            if constexpr (sizeof(T) == 4) w[0] = __float_as_uint(row[at * inner]);
+            else w[0] = reinterpret_cast<const uint16_t *>(row)[at * inner];
+        } else if constexpr (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(row + at);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(row + at);
+            w[0] = v.x, w[1] = v.y;
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i & 1)))));
+        else return __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+    }
 };
 
-// V == 1 reads at any element stride; wider pieces are 16 bytes on a 16-byte boundary.
-template <typename T, int V>
-__device__ __forceinline__ Piece<T, V> load(const T *row, int at, int64_t inner) {
-    Piece<T, V> p;
-    if constexpr (V == 1) {
-        p.e[0] = row[at * inner];
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
     } else {
-        static_assert(V * sizeof(T) == 16, "a piece is 16 bytes");
-        *reinterpret_cast<uint4 *>(p.e) = *reinterpret_cast<const uint4 *>(row + at);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
     }
-    return p;
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store(T *row, int at, int64_t inner, const float *f) {
-    Piece<T, V> p;
-#pragma unroll
-    for (int i = 0; i < V; i++) p.e[i] = from_f<T>(f[i]);
-    if constexpr (V == 1) row[at * inner] = p.e[0];
-    else *reinterpret_cast<uint4 *>(row + at) = *reinterpret_cast<const uint4 *>(p.e);
+    if constexpr (V == 1) row[at * inner] = from_f<T>(f[0]);
+    else if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(row + at) = make_float4(f[0], f[1], f[2], f[3]);
+    else *reinterpret_cast<uint2 *>(row + at) = make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]));
 }
 
 __device__ __forceinline__ float weight_at(const RotaryOperand &o, int at) {
@@ -106,13 +119,13 @@ constexpr int rows_ahead() {
 }
 
 // UPL units (two pieces of V elements: V pairs, or 2 V channels that pass through) per lane; a row
-// takes 1 << lpr_log lanes. Blocks below a.blocks_q work on the queries, the others on the keys.
+// takes 1 << lpr_log lanes. An item is a token and a run of heads_per_item of its rows, the query
+// heads first, then the keys'.
 template <typename T, int V, int UPL, int MODE, bool INTER>
 __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_kernel(const RotaryArgs a) {
     constexpr int R = rows_ahead<MODE, UPL>();
-    const bool key = (int)blockIdx.x >= a.blocks_q;
-    const RotaryOperand &o = a.op[key];
-    const int blk = (int)blockIdx.x - (key ? a.blocks_q : 0), nblk = key ? (int)gridDim.x - a.blocks_q : a.blocks_q;
+    constexpr int NW = MODE == ROTATE ? 1 : UPL, NG = MODE == NORM_BWD ? UPL : 1;
+    __shared__ __align__(16) float s_cos[WPB][MAX_PAIRS], s_sin[WPB][MAX_PAIRS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int lpr = 1 << a.lpr_log, sub = lane >> a.lpr_log, rpw = 32 >> a.lpr_log, ul = lane & (lpr - 1);
     const int nrot = INTER ? a.rot / (2 * V) : a.rot / 2 / V, nunit = a.D / (2 * V);
@@ -136,160 +149,203 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
             e1[u] = e0[u] + V;
         }
     }
-    float w[MODE == ROTATE ? 1 : UPL][2 * V], gw[MODE == NORM_BWD ? UPL : 1][2 * V];
-    if constexpr (MODE != ROTATE) {
+    float gw[2][NG][2 * V];
+    if constexpr (MODE == NORM_BWD) {
 #pragma unroll
-        for (int u = 0; u < UPL; u++)
+        for (int k = 0; k < 2; k++)
 #pragma unroll
-            for (int i = 0; i < 2 * V; i++) {
-                w[u][i] = has[u] ? weight_at(o, (i < V ? e0[u] : e1[u]) + i % V) : 0.0f;
-                if constexpr (MODE == NORM_BWD) gw[u][i] = 0.0f;
-            }
+            for (int u = 0; u < UPL; u++)
+#pragma unroll
+                for (int i = 0; i < 2 * V; i++) gw[k][u][i] = 0.0f;
     }
-    const int64_t items = a.B * a.L * o.chunks;
-    for (int64_t item = (int64_t)blk * WPB + warp; item < items; item += (int64_t)nblk * WPB) {
-        const int64_t token = item / o.chunks, b = token / a.L, l = token - b * a.L;
-        const int h0 = (int)(item - token * o.chunks) * o.heads_per_item, h1 = min(o.H, h0 + o.heads_per_item);
-        const int64_t at = b * a.ps[0] + l * a.ps[1];
+    // The weights, in 32 bits, for every item of the block.
+    __shared__ __align__(16) float s_w[2][MODE == ROTATE ? 4 : 2 * MAX_PAIRS];
+    if constexpr (MODE != ROTATE) {
+        for (int i = threadIdx.x; i < 2 * a.D; i += WPB * 32) {
+            const int k = i >= a.D;
+            s_w[k][i - k * a.D] = weight_at(a.op[k], i - k * a.D);
+        }
+        __syncthreads();
+    }
+    const int64_t items = a.B * a.L * a.chunks;
+    for (int64_t item = (int64_t)blockIdx.x * WPB + warp; item < items; item += (int64_t)gridDim.x * WPB) {
+        int64_t token, b;
+        int chunk;
+        if (items < (1ll << 31)) {  // 32-bit divisions
+            const uint32_t t32 = (uint32_t)item / (uint32_t)a.chunks, b32 = t32 / (uint32_t)a.L;
+            token = t32, b = b32;
+            chunk = (int)((uint32_t)item - t32 * (uint32_t)a.chunks);
+        } else {
+            token = item / a.chunks, b = token / a.L;
+            chunk = (int)(item - token * a.chunks);
+        }
+        const int64_t l = token - b * a.L, at = b * a.ps[0] + l * a.ps[1];
         const double t = a.pos64 ? (double)static_cast<const int64_t *>(a.positions)[at]
                                  : (double)static_cast<const int32_t *>(a.positions)[at];
+        __syncwarp();
+        for (int i = lane; i < a.rot / 2; i += 32) {
+            double turn = t * (a.freq[i * a.freq_stride] * 0.15915494309189535);
+            turn -= rint(turn);
+            float sn, cs;
+            sincospif(2.0f * (float)turn, &sn, &cs);
+            s_cos[warp][i] = cs * a.amplitude;
+            s_sin[warp][i] = (a.inverse ? -sn : sn) * a.amplitude;
+        }
+        __syncwarp();
         float cs[UPL][V], sn[UPL][V];
 #pragma unroll
         for (int u = 0; u < UPL; u++)
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                cs[u][i] = 1.0f;
-                sn[u][i] = 0.0f;
-                if (has[u] && turns[u]) {
-                    double turn = t * a.freq[((ul + u * lpr) * V + i) * a.freq_stride] * 0.15915494309189535;
-                    turn -= rint(turn);
-                    sincospif(2.0f * (float)turn, &sn[u][i], &cs[u][i]);
-                    cs[u][i] *= a.amplitude;
-                    sn[u][i] *= a.amplitude;
-                    if (a.inverse) sn[u][i] = -sn[u][i];
-                }
+                const int pair = (ul + u * lpr) * V + i;
+                cs[u][i] = turns[u] ? s_cos[warp][pair] : 1.0f;
+                sn[u][i] = turns[u] ? s_sin[warp][pair] : 0.0f;
             }
-        const T *xb = static_cast<const T *>(o.x) + b * o.xs[0] + l * o.xs[2];
-        const T *gb = MODE == NORM_BWD ? static_cast<const T *>(o.g) + b * o.gs[0] + l * o.gs[2] : nullptr;
-        T *yb = static_cast<T *>(o.y) + b * o.ys[0] + l * o.ys[2];
-        for (int hb = h0; hb < h1; hb += rpw * R) {
-            Piece<T, V> x[R][UPL][2], g[MODE == NORM_BWD ? R : 1][UPL][2];
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int h = hb + r * rpw + sub;
-#pragma unroll
-                for (int u = 0; u < UPL; u++)
-                    if (h < h1 && has[u]) {
-                        const T *row = xb + h * o.xs[1];
-                        x[r][u][0] = load<T, V>(row, e0[u], o.xs[3]);
-                        x[r][u][1] = load<T, V>(row, e1[u], o.xs[3]);
-                        if constexpr (MODE == NORM_BWD) {
-                            const T *gr = gb + h * o.gs[1];
-                            g[r][u][0] = load<T, V>(gr, e0[u], o.gs[3]);
-                            g[r][u][1] = load<T, V>(gr, e1[u], o.gs[3]);
-                        }
-                    }
-            }
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int h = hb + r * rpw + sub;
-                const bool live = h < h1;
-                float f[UPL][2 * V], v[MODE == NORM_BWD ? UPL : 1][2 * V];
-                float ss = 0.0f;
+        // Rows h0 .. h1 - 1 of operand K.
+        auto rows = [&](auto operand, int h0, int h1) {
+            constexpr int K = decltype(operand)::value;
+            if (h0 >= h1) return;
+            const RotaryOperand &o = a.op[K];
+            float w[NW][2 * V];
+            if constexpr (MODE != ROTATE) {
 #pragma unroll
                 for (int u = 0; u < UPL; u++)
 #pragma unroll
-                    for (int i = 0; i < 2 * V; i++) {
-                        const bool in = live && has[u];
-                        f[u][i] = in ? to_f(x[r][u][i / V].e[i % V]) : 0.0f;
-                        if constexpr (MODE != ROTATE) ss = fmaf(f[u][i], f[u][i], ss);
-                        if constexpr (MODE == NORM_BWD) v[u][i] = in ? to_f(g[r][u][i / V].e[i % V]) : 0.0f;
-                    }
-                float rinv = 1.0f;
-                if constexpr (MODE != ROTATE) {
-                    for (int s = lpr >> 1; s > 0; s >>= 1) ss += __shfl_xor_sync(ALL, ss, s);
-                    rinv = 1.0f / sqrtf(ss * a.inv_D + a.eps);
-                }
-                if constexpr (MODE == NORM) {
+                    for (int i = 0; i < 2 * V; i++) w[u][i] = has[u] ? s_w[K][(i < V ? e0[u] : e1[u]) + i % V] : 0.0f;
+            }
+            const T *xb = static_cast<const T *>(o.x) + b * o.xs[0] + l * o.xs[2];
+            const T *gb = MODE == NORM_BWD ? static_cast<const T *>(o.g) + b * o.gs[0] + l * o.gs[2] : nullptr;
+            T *yb = static_cast<T *>(o.y) + b * o.ys[0] + l * o.ys[2];
+            for (int hb = h0; hb < h1; hb += rpw * R) {
+                Piece<T, V> x[R][UPL][2], g[MODE == NORM_BWD ? R : 1][UPL][2];
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const int h = hb + r * rpw + sub;
 #pragma unroll
                     for (int u = 0; u < UPL; u++)
-#pragma unroll
-                        for (int i = 0; i < 2 * V; i++) f[u][i] = f[u][i] * rinv * w[u][i];
-                }
-                // The rotation: of the row, or (backward) transposed, of the gradient.
-#pragma unroll
-                for (int u = 0; u < UPL; u++) {
-                    float *z = MODE == NORM_BWD ? v[MODE == NORM_BWD ? u : 0] : f[u];
-                    if (turns[u]) {
-#pragma unroll
-                        for (int i = 0; i < V; i++) {
-                            const int ia = INTER ? 2 * i : i, ib = INTER ? 2 * i + 1 : V + i;
-                            const float za = z[ia], zb = z[ib];
-                            z[ia] = fmaf(za, cs[u][i], -zb * sn[u][i]);
-                            z[ib] = fmaf(zb, cs[u][i], za * sn[u][i]);
+                        if (h < h1 && has[u]) {
+                            const T *row = xb + h * o.xs[1];
+                            x[r][u][0].load(row, e0[u], o.xs[3]);
+                            x[r][u][1].load(row, e1[u], o.xs[3]);
+                            if constexpr (MODE == NORM_BWD) {
+                                const T *gr = gb + h * o.gs[1];
+                                g[r][u][0].load(gr, e0[u], o.gs[3]);
+                                g[r][u][1].load(gr, e1[u], o.gs[3]);
+                            }
                         }
-                    }
                 }
-                if constexpr (MODE == NORM_BWD) {
-                    float dot = 0.0f;
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const int h = hb + r * rpw + sub;
+                    const bool live = h < h1;
+                    float f[UPL][2 * V], v[NG][2 * V];
+                    float ss = 0.0f;
 #pragma unroll
                     for (int u = 0; u < UPL; u++)
 #pragma unroll
                         for (int i = 0; i < 2 * V; i++) {
-                            const float n = f[u][i] * rinv;
-                            gw[u][i] = fmaf(v[u][i], n, gw[u][i]);
-                            f[u][i] = n;
-                            v[u][i] *= w[u][i];
-                            dot = fmaf(v[u][i], n, dot);
+                            const bool in = live && has[u];
+                            f[u][i] = in ? x[r][u][i / V].at(i % V) : 0.0f;
+                            if constexpr (MODE != ROTATE) ss = fmaf(f[u][i], f[u][i], ss);
+                            if constexpr (MODE == NORM_BWD) v[u][i] = in ? g[r][u][i / V].at(i % V) : 0.0f;
                         }
-                    for (int s = lpr >> 1; s > 0; s >>= 1) dot += __shfl_xor_sync(ALL, dot, s);
-                    dot *= a.inv_D;
+                    float rinv = 1.0f;
+                    if constexpr (MODE != ROTATE) {
+                        for (int s = lpr >> 1; s > 0; s >>= 1) ss += __shfl_xor_sync(ALL, ss, s);
+                        rinv = 1.0f / sqrtf(ss * a.inv_D + a.eps);
+                    }
+                    if constexpr (MODE == NORM) {
 #pragma unroll
-                    for (int u = 0; u < UPL; u++)
+                        for (int u = 0; u < UPL; u++)
 #pragma unroll
-                        for (int i = 0; i < 2 * V; i++) f[u][i] = rinv * fmaf(-f[u][i], dot, v[u][i]);
-                }
-                if (live) {
-                    T *row = yb + h * o.ys[1];
+                            for (int i = 0; i < 2 * V; i++) f[u][i] = f[u][i] * rinv * w[u][i];
+                    }
+                    // The rotation: of the row, or (backward) transposed, of the gradient. Channels that
+                    // pass through are left alone, not multiplied by 1: an infinity beside them would
+                    // come back as NaN.
 #pragma unroll
-                    for (int u = 0; u < UPL; u++)
-                        if (has[u]) {
-                            store<T, V>(row, e0[u], o.ys[3], f[u]);
-                            store<T, V>(row, e1[u], o.ys[3], f[u] + V);
+                    for (int u = 0; u < UPL; u++) {
+                        float *z = MODE == NORM_BWD ? v[MODE == NORM_BWD ? u : 0] : f[u];
+                        if (turns[u]) {
+#pragma unroll
+                            for (int i = 0; i < V; i++) {
+                                const int ia = INTER ? 2 * i : i, ib = INTER ? 2 * i + 1 : V + i;
+                                const float za = z[ia], zb = z[ib];
+                                z[ia] = fmaf(za, cs[u][i], -zb * sn[u][i]);
+                                z[ib] = fmaf(zb, cs[u][i], za * sn[u][i]);
+                            }
                         }
+                    }
+                    if constexpr (MODE == NORM_BWD) {
+                        float dot = 0.0f;
+#pragma unroll
+                        for (int u = 0; u < UPL; u++)
+#pragma unroll
+                            for (int i = 0; i < 2 * V; i++) {
+                                const float n = f[u][i] * rinv;
+                                gw[K][u][i] = fmaf(v[u][i], n, gw[K][u][i]);
+                                f[u][i] = n;
+                                v[u][i] *= w[u][i];
+                                dot = fmaf(v[u][i], n, dot);
+                            }
+                        for (int s = lpr >> 1; s > 0; s >>= 1) dot += __shfl_xor_sync(ALL, dot, s);
+                        dot *= a.inv_D;
+#pragma unroll
+                        for (int u = 0; u < UPL; u++)
+#pragma unroll
+                            for (int i = 0; i < 2 * V; i++) f[u][i] = rinv * fmaf(-f[u][i], dot, v[u][i]);
+                    }
+                    if (live) {
+                        T *row = yb + h * o.ys[1];
+#pragma unroll
+                        for (int u = 0; u < UPL; u++)
+                            if (has[u]) {
+                                store<T, V>(row, e0[u], o.ys[3], f[u]);
+                                store<T, V>(row, e1[u], o.ys[3], f[u] + V);
+                            }
+                    }
                 }
             }
-        }
+        };
+        const int r0 = chunk * a.heads_per_item, r1 = r0 + a.heads_per_item, hq = a.op[0].H;
+        rows(std::integral_constant<int, 0>{}, r0, min(r1, hq));
+        rows(std::integral_constant<int, 1>{}, max(r0 - hq, 0), min(r1 - hq, a.op[1].H));
     }
     if constexpr (MODE == NORM_BWD) {
-        // This block's part of the weight gradient: over the warp's lane groups, then its warps.
-        __shared__ float part[WPB][256];
+        // This block's part of the weight gradients: over the warp's lane groups, then its warps.
+        __shared__ float part[WPB][2 * MAX_PAIRS];
 #pragma unroll
-        for (int u = 0; u < UPL; u++)
+        for (int k = 0; k < 2; k++) {
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 2 * V; i++) {
-                float s = gw[u][i];
-                for (int m = lpr; m < 32; m <<= 1) s += __shfl_xor_sync(ALL, s, m);
-                if (has[u] && sub == 0) part[warp][(i < V ? e0[u] : e1[u]) + i % V] = s;
+            for (int u = 0; u < UPL; u++)
+#pragma unroll
+                for (int i = 0; i < 2 * V; i++) {
+                    float s = gw[k][u][i];
+                    for (int m = lpr; m < 32; m <<= 1) s += __shfl_xor_sync(ALL, s, m);
+                    if (has[u] && sub == 0) part[warp][(i < V ? e0[u] : e1[u]) + i % V] = s;
+                }
+            __syncthreads();
+            for (int d = threadIdx.x; d < a.D; d += WPB * 32) {
+                float s = 0.0f;
+#pragma unroll
+                for (int x = 0; x < WPB; x++) s += part[x][d];
+                a.wpart[((int64_t)k * gridDim.x + blockIdx.x) * a.D + d] = s;
             }
-        __syncthreads();
-        for (int d = threadIdx.x; d < a.D; d += WPB * 32) {
-            float s = 0.0f;
-#pragma unroll
-            for (int x = 0; x < WPB; x++) s += part[x][d];
-            o.wpart[(int64_t)blk * a.D + d] = s;
         }
     }
 }
 
 // gw[d] = sum over the blocks' parts, 32 columns a block, in a fixed order.
-__global__ void __launch_bounds__(1024) weight_grad_kernel(const RotaryArgs a, int blocks_k) {
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const RotaryArgs a, int blocks) {
     __shared__ float sums[32][33];
+    griddep_wait();
     const RotaryOperand &o = a.op[blockIdx.y];
-    const int n = blockIdx.y ? blocks_k : a.blocks_q, d = blockIdx.x * 32 + threadIdx.x;
+    const int d = blockIdx.x * 32 + threadIdx.x;
+    const float *part = a.wpart + (int64_t)blockIdx.y * blocks * a.D;
     float s = 0.0f;
     if (d < a.D)
-        for (int i = threadIdx.y; i < n; i += 32) s += o.wpart[(int64_t)i * a.D + d];
+        for (int i = threadIdx.y; i < blocks; i += 32) s += part[(int64_t)i * a.D + d];
     sums[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && d < a.D && o.gw) {
@@ -303,44 +359,27 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const RotaryArgs a, i
     }
 }
 
-// Whether every row of the tensor can be read in 16-byte pieces.
-bool vec_rows(const void *ptr, const int64_t *st, int v, int64_t D) {
-    return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && (st[3] == 1 || D == 1) && st[0] % v == 0 && st[1] % v == 0 &&
-           st[2] % v == 0;
+// Whether every row of the tensor can be read in pieces of four elements.
+bool vec_rows(const void *ptr, const int64_t *st, int size) {
+    return (reinterpret_cast<uintptr_t>(ptr) & (4 * size - 1)) == 0 && st[3] == 1 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
 }
 
 template <typename T, int V, int UPL, int MODE>
 int launch(RotaryArgs &a, bool interleaved, const char *name, cudaStream_t stream) {
-    const int units = (int)(a.D / (2 * V)), lanes = (units + UPL - 1) / UPL;
+    const int units = a.D / (2 * V), lanes = (units + UPL - 1) / UPL;
     a.lpr_log = 0;
     while ((1 << a.lpr_log) < lanes) a.lpr_log++;
-    const int rpw = 32 >> a.lpr_log, sms = device_sm_count();
-    // A run of heads per warp: as long as the call still gives every SM 16 warps, at most 8 rows a
-    // lane group (the angles then cost an eighth of a row's work); short calls get one row each.
-    int64_t blocks[2] = {0, 0};
-    for (int i = 0; i < 2; i++) {
-        RotaryOperand &o = a.op[i];
-        if (!o.x || o.H == 0) continue;
-        int run = 8;
-        while (run > 1 && a.B * a.L * ((o.H + rpw * run - 1) / (rpw * run)) < 16ll * sms) run >>= 1;
-        o.heads_per_item = rpw * run;
-        o.chunks = (o.H + o.heads_per_item - 1) / o.heads_per_item;
-        blocks[i] = (a.B * a.L * o.chunks + WPB - 1) / WPB;
-    }
-    if (MODE == NORM_BWD) {
-        // At most BWD_BLOCKS blocks (their parts are summed by the second kernel), shared between
-        // queries and keys by their work.
-        const int64_t total = blocks[0] + blocks[1];
-        if (total > BWD_BLOCKS) {
-            const int64_t k = blocks[1] ? std::max<int64_t>(1, blocks[1] * BWD_BLOCKS / total) : 0;
-            blocks[1] = std::min(blocks[1], k);
-            blocks[0] = std::min(blocks[0], BWD_BLOCKS - blocks[1]);
-        }
-        a.op[1].wpart = a.op[0].wpart + blocks[0] * a.D;
-    }
-    if (blocks[0] + blocks[1] >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "rotary: more than 2^31 blocks of rows");
-    a.blocks_q = (int)blocks[0];
-    const unsigned grid = (unsigned)(blocks[0] + blocks[1]);
+    const int rpw = 32 >> a.lpr_log, sms = device_sm_count(), heads = a.op[0].H + a.op[1].H;
+    const int64_t tokens = a.B * a.L;
+    // A run of all of a token's rows, or as much of it as still gives every SM 32 warps.
+    int chunks = 1;
+    while (heads > rpw * chunks && tokens * chunks < 32ll * sms) chunks++;
+    a.heads_per_item = heads ? ((heads + chunks - 1) / chunks + rpw - 1) / rpw * rpw : rpw;
+    a.chunks = heads ? (heads + a.heads_per_item - 1) / a.heads_per_item : 0;
+    int64_t blocks = (tokens * a.chunks + WPB - 1) / WPB;
+    if (MODE == NORM_BWD) blocks = std::min<int64_t>(blocks, MAX_BWD_BLOCKS);
+    if (blocks >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "rotary: more than 2^31 blocks of rows");
+    const unsigned grid = (unsigned)blocks;
     if (grid > 0) {
         KernelTrace tr(name, stream);
         if (interleaved) rotary_kernel<T, V, UPL, MODE, true><<<grid, WPB * 32, 0, stream>>>(a);
@@ -350,22 +389,22 @@ int launch(RotaryArgs &a, bool interleaved, const char *name, cudaStream_t strea
     }
     if (MODE == NORM_BWD && (a.op[0].gw || a.op[1].gw)) {
         KernelTrace tr("qk_norm_weight_grad", stream);
-        weight_grad_kernel<<<dim3((unsigned)((a.D + 31) / 32), 2), dim3(32, 32), 0, stream>>>(a, (int)blocks[1]);
-        return check_launch("qk_norm_weight_grad");
+        const cudaError_t e = launch_dependent(weight_grad_kernel, dim3((unsigned)((a.D + 31) / 32), 2), dim3(32, 32), 0, stream, a, (int)grid);
+        if (e != cudaSuccess) return cuda_fail(e, "qk_norm_weight_grad");
     }
     return DC_OK;
 }
 
 template <typename T, int MODE>
 int dispatch(RotaryArgs &a, bool interleaved, const char *name, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    // 16-byte pieces where the pairs, the passing channels and every row come in whole ones;
-    // otherwise single elements at any stride.
-    bool vec = interleaved ? (a.rot % (2 * V) == 0 && a.D % (2 * V) == 0) : (a.rot % (2 * V) == 0 && (a.D - a.rot) % (2 * V) == 0);
+    constexpr int V = 4, S = (int)sizeof(T);
+    // Pieces of four where the pairs, the passing channels and every row come in whole ones; otherwise
+    // single elements at any stride.
+    bool vec = a.rot % (2 * V) == 0 && a.D % (2 * V) == 0;
     for (int i = 0; i < 2 && vec; i++) {
         const RotaryOperand &o = a.op[i];
         if (!o.x) continue;
-        vec = vec_rows(o.x, o.xs, V, a.D) && vec_rows(o.y, o.ys, V, a.D) && (MODE != NORM_BWD || vec_rows(o.g, o.gs, V, a.D));
+        vec = vec_rows(o.x, o.xs, S) && vec_rows(o.y, o.ys, S) && (MODE != NORM_BWD || vec_rows(o.g, o.gs, S));
     }
     return vec ? launch<T, V, 1, MODE>(a, interleaved, name, stream) : launch<T, 1, 4, MODE>(a, interleaved, name, stream);
 }
@@ -379,7 +418,7 @@ int by_type(RotaryArgs &a, int dtype, bool interleaved, const char *name, cudaSt
 
 }  // namespace
 
-size_t rotary_bwd_workspace_bytes(int64_t D) { return (size_t)BWD_BLOCKS * D * sizeof(float); }
+size_t rotary_bwd_workspace_bytes(int64_t D) { return (size_t)2 * MAX_BWD_BLOCKS * D * sizeof(float); }
 
 int rotary_launch(RotaryArgs &a, int dtype, bool interleaved, int mode, cudaStream_t stream) {
     if (mode == ROTATE) return by_type<ROTATE>(a, dtype, interleaved, "rotary", stream);
