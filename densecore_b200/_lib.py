@@ -37,7 +37,7 @@ class DcTensor(ctypes.Structure):
 
 
 class DcCache4(ctypes.Structure):
-    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("num_pages", ctypes.c_int64),
+    _fields_ = [("data", ctypes.c_void_p), ("num_pages", ctypes.c_int64),
                 ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32)]
 
 

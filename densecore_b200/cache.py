@@ -57,12 +57,10 @@ class KVCache4:
         if page_size % 16:
             raise ValueError("page_size must be a multiple of 16")
         self.num_pages, self.kv_heads, self.head_dim, self.page_size = num_pages, kv_heads, int(head_dim), page_size
-        shape = (num_pages, 2, kv_heads, page_size)
-        self.codes = torch.zeros(shape + (head_dim // 2,), dtype=torch.uint8, device=device)
-        self.scales = torch.zeros(shape + (head_dim // 32,), dtype=torch.int32, device=device)
-        self.device = self.codes.device
-        self._desc = _lib.DcCache4(self.codes.data_ptr(), self.scales.data_ptr(), num_pages, kv_heads, self.head_dim,
-                                   page_size)
+        # A page is contiguous: copying one is copying data[page].
+        self.data = torch.zeros((num_pages, kv_heads, page_size // 16, 20 * self.head_dim), dtype=torch.uint8, device=device)
+        self.device = self.data.device
+        self._desc = _lib.DcCache4(self.data.data_ptr(), num_pages, kv_heads, self.head_dim, page_size)
 
     def _table(self, page_table):
         _counts("page_table", page_table)

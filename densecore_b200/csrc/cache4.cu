@@ -9,9 +9,11 @@
 // in 32-bit arithmetic; the group stands for low + scale * code. low and scale are rounded outward,
 // so no value is clipped, and bfloat16 has the range of every input type. A group with an infinity
 // or a NaN stands for NaN. 20 bytes per 32 values: 5 bits a value, against 32 in the fp32 cache.
-// A row of D channels is stored as halfwords of four codes, halfword r * D/32 + g holding channels
-// 32 g + 4 r .. + 3 in ascending nibbles (r = 0..7): the order in which both tensor-core products of
-// the attention kernel want them, so that a lane's codes are one wide load.
+// Sixteen tokens of a head lie together, 20 D bytes: the keys' codes (8 D bytes) and scales (16 rows of
+// D / 32 words, scale | low << 16), then the values'; so a warp fetches them with one bulk copy. The
+// codes are halfwords of four channels, 32 g + 4 r .. + 3 in ascending nibbles (r = 0..7), placed so
+// that the words of a lane's wide load are pairs as the attention kernel's products take them: for the
+// keys r and r + 1 of a token, for the values tokens s and s + 8 (code_at).
 //
 // Attention. Bound: HBM, 2 * 20/32 D bytes per key and head, and close behind it the integer work
 // of unpacking: so both products run on the tensor cores with the codes as they are, and the scales
@@ -27,9 +29,10 @@
 // product takes 16 keys, 4 heads and both parts. mma.sync, not tcgen05: at one query row per head the
 // products fill an eighth of even these tiles, their time is far from the bound, and their operands
 // come straight from registers (4-bit codes would have to be expanded into shared memory first).
-// A warp works alone: blocks of 16 keys (never across a page) with the next block's loads in flight
-// and the page after that looked up, its own running maximum, which moves only when it grows by more
-// than 2^8 (sum, lows and accumulators share it), joined with the other warps' at the end.
+// A warp works alone on blocks of 16 keys (never across a page), which bulk copies bring into a ring of
+// its own in shared memory a few blocks ahead; its own running maximum, which moves only when it grows
+// by more than 2^8 (sum, mids and accumulators share it), is joined with the other warps' at the end.
+// (With the blocks fetched into registers one ahead the warps waited on loads 2.2 cycles per issue.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -39,6 +42,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "sm100.cuh"
 #include "split_rows.cuh"
 #include "trace.h"
 
@@ -81,20 +85,30 @@ __device__ __forceinline__ void load4(const T *p, int64_t inner, bool vec, float
     }
 }
 
-// Row of `slot` of `page` in the codes and scales.
-__device__ __forceinline__ int64_t cache_row(const Cache4 &c, int64_t page, int which, int head, int slot) {
-    return (((page * 2 + which) * c.Hkv + head) * c.page_size + slot);
+// Bytes of a block of 16 tokens of a head, keys and values.
+__host__ __device__ constexpr int block_bytes(int D) { return 20 * D; }
+
+// Where halfword (group g, r) of token `slot` (0..15) lies among a block's codes of keys or values.
+__device__ __forceinline__ int code_at(int which, int slot, int r, int g, int ng) {
+    return which ? 2 * (((slot % 8) * 8 + r) * ng + g) + slot / 8 : 2 * ((slot * 4 + r / 2) * ng + g) + r % 2;
 }
 
-// The row of position pos of sequence b, or -1 (and the device status) where the table has none.
-__device__ __forceinline__ int64_t row_of(const Cache4Args &a, int64_t b, int64_t pos, int which, int head) {
+// The keys or values of the block of 16 tokens that holds position pos of sequence b, and its slot
+// there; null (and the device status) where the table has no page for it.
+struct Place {
+    uint8_t *half;
+    int slot;
+};
+__device__ __forceinline__ Place place_of(const Cache4Args &a, int64_t b, int64_t pos, int which, int head) {
     if (pos >= 0 && pos < a.P * a.c.page_size) {
         const uint32_t entry = (uint32_t)pos / (uint32_t)a.c.page_size, slot = (uint32_t)pos - entry * (uint32_t)a.c.page_size;
         const int64_t page = a.table[b * a.ts[0] + entry * a.ts[1]];
-        if (page >= 0 && page < a.c.pages) return cache_row(a.c, page, which, head, (int)slot);
+        if (page >= 0 && page < a.c.pages)
+            return {a.c.data + ((page * a.c.Hkv + head) * (a.c.page_size / 16) + slot / 16) * block_bytes(a.c.D) + which * 10 * a.c.D,
+                    (int)(slot % 16)};
     }
     atomicExch(a.err, BAD_TABLE);
-    return -1;
+    return {nullptr, 0};
 }
 
 // Filling and reading back are bound by HBM. A block takes a run of tokens of one (sequence, head) of
@@ -161,10 +175,10 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Args a, 
 #pragma unroll
             for (int e = 0; e < 4; e++) codes |= (uint32_t)code_of(__fsub_rn(x[i][e], low), scale, inv) << (4 * e);
         }
-        const int64_t at = row_of(a, b, start + t, which, head);
-        if (at < 0) continue;
-        reinterpret_cast<uint16_t *>(a.c.codes + at * (a.c.D / 2))[r * ng + g] = (uint16_t)codes;
-        if (r == 0) a.c.scales[at * ng + g] = (sb >> 16) | lb;
+        const Place at = place_of(a, b, start + t, which, head);
+        if (!at.half) continue;
+        reinterpret_cast<uint16_t *>(at.half)[code_at(which, at.slot, r, g, ng)] = (uint16_t)codes;
+        if (r == 0) reinterpret_cast<uint32_t *>(at.half + 8 * a.c.D)[at.slot * ng + g] = (sb >> 16) | lb;
     }
 }
 
@@ -179,10 +193,12 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bo
     for (int i = 0; i < ROWS; i++) {
         const int64_t t = t0 + i * pass;
         codes[i] = sl[i] = 0u;  // a zero
-        const int64_t at = t < a.T && t < len ? row_of(a, b, t, which, head) : -1;
-        if (at >= 0) {
-            codes[i] = reinterpret_cast<const uint16_t *>(a.c.codes + at * (a.c.D / 2))[r * ng + g];
-            sl[i] = a.c.scales[at * ng + g];
+        if (t < a.T && t < len) {
+            const Place at = place_of(a, b, t, which, head);
+            if (at.half) {
+                codes[i] = reinterpret_cast<const uint16_t *>(at.half)[code_at(which, at.slot, r, g, ng)];
+                sl[i] = reinterpret_cast<const uint32_t *>(at.half + 8 * a.c.D)[at.slot * ng + g];
+            }
         }
     }
 #pragma unroll
@@ -231,13 +247,16 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
-// Pair i of codes, less 8, as fp16 and as bfloat16.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t y, int i) {
-    const uint32_t z = ((y >> (4 * i)) & 0x000F000Fu) | 0x64006400u;  // 1024 + code
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(z), "r"(0x64086408u));
-    return r;
+// The four pairs of codes of y, less 8, as fp16: pairs 0 and 2 as they are, 1 and 3 times 16 (their
+// bits lie four higher in the mantissa, which saves a shift; q is divided by 16 there).
+__device__ __forceinline__ void codes_f16(uint32_t y, uint32_t (&c)[4]) {
+    const uint32_t z = y >> 8;
+    const uint32_t w[4] = {(y & 0x000F000Fu) | 0x64006400u, (y & 0x00F000F0u) | 0x64006400u,  // 1024 + code, 1024 + 16 code
+                           (z & 0x000F000Fu) | 0x64006400u, (z & 0x00F000F0u) | 0x64006400u};
+#pragma unroll
+    for (int i = 0; i < 4; i++) asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(c[i]) : "r"(w[i]), "r"((i & 1) ? 0x64806480u : 0x64086408u));
 }
+// Pair i of codes, less 8, as bfloat16.
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t y, int i) {
     const uint32_t z = ((y >> (4 * i)) & 0x000F000Fu) | 0x43004300u;  // 128 + code
     uint32_t r;
@@ -245,38 +264,51 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t y, int i) {
     return r;
 }
 
+// N words from shared memory, on a boundary of their size (at most 16 bytes at a time).
 template <int N>
-__device__ __forceinline__ void load_words(const void *p, uint32_t *w) {
+__device__ __forceinline__ void read_words(const uint8_t *p, uint32_t *w) {
     if constexpr (N == 1) {
-        asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
     } else if constexpr (N == 2) {
-        asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+        const uint2 x = *reinterpret_cast<const uint2 *>(p);
+        w[0] = x.x, w[1] = x.y;
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i += 4)
-            asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
-                         : "l"(reinterpret_cast<const uint32_t *>(p) + i));
+        for (int i = 0; i < N; i += 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(p + 4 * i);
+            w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+        }
     }
 }
 
-// A block of 16 keys as a lane holds it (lane = 4 r + t): the codes of keys r and r + 8 (its
-// quarter of each group) with their scales, and those of values t, t + 8, t + 4, t + 12 (its eighth
-// of each group) with the scales of values r and r + 8.
-template <int NG>
-struct Block {
-    uint32_t k[2][NG], ks[2][NG], v[4][NG / 2], vs[2][NG];
-};
+// A contiguous copy from global to shared memory, completing on the mbarrier (16-byte multiples).
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
 
-template <int D, int PARTS, int NT>
+// HEADS query heads of one key/value head per CTA: 1, 4 or 8.
+//   4, 8  head t (and t + 4) of a lane; a group's product is a head's two parts per column pair, and the
+//         lane applies every group's scales for its heads;
+//   1     the column pairs are the groups instead: lane t gets group t's dots and applies that group's
+//         scales alone, keys and values, and the groups are added up by two shuffles. (With the
+//         columns left to absent heads a block of 16 keys took 722 instructions.)
+template <int D, int PARTS, int HEADS>
 struct AttnCfg {
-    static constexpr int NG = D / GROUP, HC = 4 * NT;  // groups; query heads per CTA
-    static constexpr int ROWS = HC * PARTS;            // rows of the second product in use
+    static constexpr int NG = D / GROUP;
+    static constexpr bool ONE = HEADS == 1;
+    static constexpr int NT = ONE ? 1 : HEADS / 4;              // heads of a lane
+    static constexpr int NS = ONE ? (NG + 3) / 4 : NG;          // groups of a lane
+    static constexpr int ROWS = HEADS * PARTS;                  // rows of the second product in use
     static_assert(ROWS <= 16, "the parts of the weights fill one product's rows");
-    static constexpr int ROW_BYTES = 48;               // 16 weights of a row, padded against bank conflicts
-    // Shared memory: q fragments | the warps' weight tiles; after the loop the accumulators.
-    static constexpr int Q_BYTES = NT * NG * 32 * 16, W_BYTES = NG * 16 * ROW_BYTES;
-    static constexpr int LOOP_BYTES = Q_BYTES + WARPS * W_BYTES;
+    static constexpr int ROW_BYTES = 48;                        // 16 weights of a row, padded against bank conflicts
+    static constexpr int STAGES = D == 64 ? 4 : (D == 128 ? 3 : 2);  // blocks of a warp's ring
+    // Shared memory: the warps' rings | q fragments | the warps' weight tiles; after the loop the
+    // accumulators.
+    static constexpr int BLOCK = block_bytes(D), RING = STAGES * BLOCK;
+    static constexpr int Q_BYTES = NT * NG * 32 * 16, W_BYTES = NG * ROWS * ROW_BYTES;
+    static constexpr int OFF_Q = WARPS * RING, OFF_W = OFF_Q + Q_BYTES, LOOP_BYTES = OFF_W + WARPS * W_BYTES;
     static constexpr int ACC_BYTES = WARPS * ROWS * D * 4;
     static constexpr int SMEM = LOOP_BYTES > ACC_BYTES ? LOOP_BYTES : ACC_BYTES;
 };
@@ -287,66 +319,91 @@ __device__ __forceinline__ float load_q(const Cache4Args &a, int64_t at) {
     return __bfloat162float(static_cast<const __nv_bfloat16 *>(a.x[0])[at]);
 }
 
-template <int D, int PARTS, int NT>
-__global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention_kernel(const Cache4Args a, const SplitRows rows) {
-    using C = AttnCfg<D, PARTS, NT>;
-    constexpr int NG = C::NG, HC = C::HC;
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float s_qsum[HC][NG], s_exp[HC], s_m[WARPS][HC], s_l[WARPS][HC], s_low[WARPS][HC][NG];
+template <int D, int PARTS, int HEADS>
+__global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4))
+    cache4_attention_kernel(const Cache4Args a, const SplitRows rows) {
+    using C = AttnCfg<D, PARTS, HEADS>;
+    constexpr int NG = C::NG, NT = C::NT, NS = C::NS;
+    constexpr bool ONE = C::ONE;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t s_full[WARPS][C::STAGES];
+    __shared__ int s_abort;
+    __shared__ float s_qsum[HEADS][NG], s_exp[HEADS], s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_low[WARPS][HEADS][NG];
     griddep_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-    const int group = (int)(a.H / a.c.Hkv), chunks = (group + HC - 1) / HC;
+    const int group = (int)(a.H / a.c.Hkv), chunks = (group + HEADS - 1) / HEADS;
     const int64_t b = blockIdx.z;
     const int hk = blockIdx.y / chunks;
-    const int64_t h0 = (int64_t)hk * group + (blockIdx.y % chunks) * HC;
-    const int nh = min(HC, group - (int)(blockIdx.y % chunks) * HC);
+    const int64_t h0 = (int64_t)hk * group + (blockIdx.y % chunks) * HEADS;
+    const int nh = min(HEADS, group - (int)(blockIdx.y % chunks) * HEADS);
 
     // The sequence's visible keys: [0, sinks) and [lo, len), in blocks of 16.
     const int64_t capacity = a.P * a.c.page_size;
-    int64_t len = a.lens[b * a.lens_stride];
-    if (len < 0 || len > capacity) {
+    int64_t len64 = a.lens[b * a.lens_stride];
+    if (len64 < 0 || len64 > capacity) {
         if (threadIdx.x == 0) atomicExch(a.err, BAD_TABLE);
-        len = len < 0 ? 0 : capacity;
+        len64 = len64 < 0 ? 0 : capacity;
     }
-    const int64_t lo = a.window ? max((int64_t)0, len - a.window) : 0, sinks = min(a.sinks, lo);
-    const int first = (int)(lo / 16), sink_blocks = min((int)((sinks + 15) / 16), first);
-    const int total = len == 0 ? 0 : sink_blocks + (int)((len + 15) / 16) - first;
+    const int len = (int)len64;
+    const int lo = a.window ? (int)max((int64_t)0, len64 - a.window) : 0, sinks = (int)min(a.sinks, (int64_t)lo);
+    const int first = lo / 16, sink_blocks = min((sinks + 15) / 16, first);
+    const int total = len == 0 ? 0 : sink_blocks + (len + 15) / 16 - first;
     const int per = (total + rows.splits - 1) / rows.splits, v0 = blockIdx.x * per, v1 = min(total, v0 + per);
-    const int page16 = a.c.page_size / 16;
+    const uint32_t page16 = (uint32_t)a.c.page_size / 16;
     auto block_of = [&](int v) { return v < sink_blocks ? v : first + v - sink_blocks; };
-    // Page ids are read a block ahead of the page; -1 where the table's entry is out of range.
-    auto page_id = [&](int v) -> int {
+    // The pool's block numbers of this warp's next 32 blocks, one to a lane (-1: the table's entry is out
+    // of range), and of the 32 after those: the division by the page size and the table's latency are
+    // paid once in 32 blocks.
+    const int32_t *table = a.table + b * a.ts[0];
+    auto numbers = [&](int v) -> int {
+        v += lane * WARPS;
         if (v >= v1) return -1;
-        const int id = a.table[b * a.ts[0] + (int64_t)(block_of(v) / page16) * a.ts[1]];
-        return id;
+        const uint32_t at = (uint32_t)block_of(v), entry = at / page16;
+        const int id = table[entry * a.ts[1]];
+        return (uint32_t)id < (uint32_t)a.c.pages ? (int)(((uint32_t)id * (uint32_t)a.c.Hkv + hk) * page16 + (at - entry * page16)) : -1;
     };
-    const int64_t half_page = (int64_t)a.c.Hkv * a.c.page_size;  // rows from a page's keys to its values
-    auto load_block = [&](int v, int id, Block<NG> &x) -> bool {
-        if ((unsigned)id >= (unsigned)min(a.c.pages, (int64_t)0x7fffffff)) {
-            atomicExch(a.err, BAD_TABLE);
-            return false;
+    // This warp's ring. A block whose page id is out of range is not copied: its stage completes empty
+    // and its keys are left out (stage_ok).
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * C::RING;
+    const uint32_t full = (uint32_t)__cvta_generic_to_shared(&s_full[warp][0]);
+    volatile int *abort = &s_abort;
+    uint32_t stage_ok = 0;
+    int v = v0 + warp, fetched = 0;
+    int numbers_now = numbers(v), numbers_next = numbers(v + 32 * WARPS);
+    auto fetch = [&](int stage) {  // the warp's block number `fetched`
+        const int number = __shfl_sync(ALL, numbers_now, fetched & 31);
+        if ((++fetched & 31) == 0) {
+            numbers_now = numbers_next;
+            numbers_next = numbers(v0 + warp + (fetched + 32) * WARPS);
         }
-        const int64_t krow = ((int64_t)id * 2 * a.c.Hkv + hk) * a.c.page_size + (block_of(v) % page16) * 16, vrow = krow + half_page;
-        const uint8_t *kc = a.c.codes + krow * (D / 2), *vc = a.c.codes + vrow * (D / 2);
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            load_words<NG>(kc + (r + 8 * i) * (D / 2) + t * 4 * NG, x.k[i]);
-            load_words<NG>(a.c.scales + (krow + r + 8 * i) * NG, x.ks[i]);
-            load_words<NG>(a.c.scales + (vrow + r + 8 * i) * NG, x.vs[i]);
+        stage_ok = (stage_ok & ~(1u << stage)) | ((uint32_t)(number >= 0) << stage);
+        if (lane == 0) {
+            if (number >= 0) {
+                sm100::mbar_expect_tx(full + 8 * stage, C::BLOCK);
+                bulk_copy(ring + stage * C::BLOCK, a.c.data + (int64_t)number * C::BLOCK, C::BLOCK, full + 8 * stage);
+            } else {
+                atomicExch(a.err, BAD_TABLE);
+                sm100::mbar_arrive(full + 8 * stage);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) load_words<NG / 2>(vc + (t + 4 * ((i >> 1) + 2 * (i & 1))) * (D / 2) + r * 2 * NG, x.v[i]);
-        return true;
     };
-    Block<NG> cur;
-    bool cur_ok = false;
-    int v = v0 + warp;
-    int next_id = page_id(v + WARPS);
-    if (v < v1) cur_ok = load_block(v, page_id(v), cur);
+    if (lane == 0) {
+        for (int i = 0; i < C::STAGES; i++) sm100::mbar_init(full + 8 * i, 1);
+        sm100::fence_mbar_init();
+    }
+    if (threadIdx.x == 0) s_abort = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < C::STAGES; i++)
+        if (v + i * WARPS < v1) fetch(i);
 
     // q: per head a power of two that brings its largest channel below 1, the sums of its groups,
     // and the two fp16 parts in the order of the products' B fragments.
-    for (int h = warp; h < HC; h += WARPS) {
+    if constexpr (ONE) {  // the other groups' columns of a group's fragment are zero
+        for (int i = threadIdx.x; i < C::Q_BYTES / 16; i += WARPS * 32) reinterpret_cast<uint4 *>(smem + C::OFF_Q)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    for (int h = warp; h < HEADS; h += WARPS) {
         float x[NG], top = 0.0f;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
@@ -364,13 +421,13 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(ALL, s, o);
             if (lane == 0) s_qsum[h][g] = s * (a.scale * LOG2E);
             // Channel 32 g + lane = 4 r' + i of a group: k-pair member r' & 1 of lane t' = r' / 2, pair i.
-            const float y = ldexpf(x[g], -e);
-            const __half hi = __float2half_rn(y), lo16 = __float2half_rn(y - __half2float(hi));
             const int rr = lane >> 2, i = lane & 3;
+            const float y = ldexpf(x[g], (i & 1) ? -e - 4 : -e);
+            const __half hi = __float2half_rn(y), lo16 = __float2half_rn(y - __half2float(hi));
 #pragma unroll
             for (int part = 0; part < 2; part++) {
-                const int col = (h & 3) * 2 + part;
-                __half *frag = reinterpret_cast<__half *>(smem + (((h >> 2) * NG + g) * 32 + col * 4 + (rr >> 1)) * 16);
+                const int col = (ONE ? g & 3 : h & 3) * 2 + part, tile = ONE ? 0 : h >> 2;
+                __half *frag = reinterpret_cast<__half *>(smem + C::OFF_Q + ((tile * NG + g) * 32 + col * 4 + (rr >> 1)) * 16);
                 frag[i * 2 + (rr & 1)] = part ? lo16 : hi;
             }
         }
@@ -378,16 +435,19 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention
     }
     __syncthreads();
 
-    float mul[NT], qsum[NT][NG], m[NT], l[NT], low[NT][NG];
+    // Heads n * 4 + t (one head: head 0), groups g (one head: t + 4 g) of this lane.
+    // m: the running maximum; base: what the weights are relative to (m, or 0 before there is one).
+    float mul[NT], qsum[NT][NS], m[NT], base[NT], l[NT], low[NT][NS];
     float acc[4 * NG][4];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        mul[n] = s_exp[n * 4 + t];
+        mul[n] = s_exp[ONE ? 0 : n * 4 + t];
         m[n] = -INFINITY;
-        l[n] = 0.0f;
+        base[n] = l[n] = 0.0f;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            qsum[n][g] = s_qsum[n * 4 + t][g];
+        for (int g = 0; g < NS; g++) {
+            const int own = ONE ? t + 4 * g : g;
+            qsum[n][g] = own < NG ? s_qsum[ONE ? 0 : n * 4 + t][own] : 0.0f;
             low[n][g] = 0.0f;
         }
     }
@@ -395,55 +455,116 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention
     for (int i = 0; i < 4 * NG; i++)
 #pragma unroll
         for (int c = 0; c < 4; c++) acc[i][c] = 0.0f;
-    uint8_t *wt = smem + C::Q_BYTES + warp * C::W_BYTES;
-    const uint32_t wt_addr = (uint32_t)__cvta_generic_to_shared(wt) + (lane & 15) * C::ROW_BYTES + (lane >> 4) * 16;
+    uint8_t *wt = smem + C::OFF_W + warp * C::W_BYTES;
+    // (Rows past the tile's are read as its last: what they give is never looked at.)
+    const uint32_t wt_addr = (uint32_t)__cvta_generic_to_shared(wt) + min(lane & 15, C::ROWS - 1) * C::ROW_BYTES + (lane >> 4) * 16;
 
+    // This lane's places in a block: codes of keys r and r + 8 (its quarter of each group), of values
+    // (t, t + 8) and (t + 4, t + 12) (its eighth of each group), and of both the scales of places r and
+    // r + 8.
+    const uint8_t *blk = smem + warp * C::RING;
+    const uint32_t koff = r * (D / 2) + t * 4 * NG, voff = 10 * D + (t * 8 + r) * 4 * NG;
+    const uint32_t soff = 8 * D + (r * NG + (ONE ? (NG < 4 ? t % NG : t) : 0)) * 4;
+    int stage = 0;
+    uint32_t parity = 0;
     for (; v < v1; v += WARPS) {
-        Block<NG> nxt;
-        bool nxt_ok = false;
-        if (v + WARPS < v1) nxt_ok = load_block(v + WARPS, next_id, nxt);
-        next_id = page_id(v + 2 * WARPS);
-        const int64_t j0 = (int64_t)block_of(v) * 16 + r, j1 = j0 + 8;
-        const bool ok0 = cur_ok && j0 < len && (j0 >= lo || j0 < sinks), ok1 = cur_ok && j1 < len && (j1 >= lo || j1 < sinks);
-        // Scores of keys r and r + 8 for head t of each tile.
+        if (!sm100::mbar_wait_warp(full + 8 * stage, parity, abort, a.err)) break;
+        const uint8_t *cur = blk + stage * C::BLOCK;
+        const bool cur_ok = (stage_ok >> stage) & 1u;
+        // Which of keys r and r + 8 are seen; all of them in most blocks.
+        const int k0 = block_of(v) * 16;
+        bool ok0 = true, ok1 = true;
+        const bool edge = !cur_ok || k0 + 16 > len || (k0 < lo && k0 + 16 > sinks);
+        if (edge) {
+            const int j0 = k0 + r, j1 = j0 + 8;
+            ok0 = cur_ok && j0 < len && (j0 >= lo || j0 < sinks);
+            ok1 = cur_ok && j1 < len && (j1 >= lo || j1 < sinks);
+        }
+        uint32_t kc[2][NG], ks[2][NS];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            read_words<NG>(cur + koff + 8 * i * (D / 2), kc[i]);
+            if constexpr (ONE) {
+#pragma unroll
+                for (int j = 0; j < NS; j++) read_words<1>(cur + soff + 8 * i * NG * 4 + 16 * j, &ks[i][j]);
+            } else {
+                read_words<NG>(cur + soff + 8 * i * NG * 4, ks[i]);
+            }
+        }
+        // Scores of keys r and r + 8.
         float s0[NT], s1[NT];
+        if constexpr (ONE) {
+            float c[NS][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++) s0[n] = s1[n] = 0.0f;
-        float b0[NT], b1[NT];
+            for (int i = 0; i < NS; i++) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NT; n++) b0[n] = b1[n] = 0.0f;
+            for (int g = 0; g < NG; g++) {
+                uint32_t y0[4], y1[4];
+                codes_f16(kc[0][g], y0);
+                codes_f16(kc[1][g], y1);
+                const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + (g * 32 + lane) * 16);
+                const uint32_t a0[4] = {y0[0], y1[0], y0[1], y1[1]}, a1[4] = {y0[2], y1[2], y0[3], y1[3]};
+                mma_f16(c[g / 4], a0, q.x, q.y);
+                mma_f16(c[g / 4], a1, q.z, q.w);
+            }
+            float x0 = 0.0f, x1 = 0.0f;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
-            const uint32_t y0 = __byte_perm(cur.k[0][g / 2], cur.k[0][NG / 2 + g / 2], sel);
-            const uint32_t y1 = __byte_perm(cur.k[1][g / 2], cur.k[1][NG / 2 + g / 2], sel);
-            const uint32_t a0[4] = {codes_f16(y0, 0), codes_f16(y1, 0), codes_f16(y0, 1), codes_f16(y1, 1)};
-            const uint32_t a1[4] = {codes_f16(y0, 2), codes_f16(y1, 2), codes_f16(y0, 3), codes_f16(y1, 3)};
+            for (int i = 0; i < NS; i++) {
+                x0 = fmaf(bf16_low(ks[0][i]) * mul[0], c[i][0] + c[i][1], fmaf(mid(ks[0][i]), qsum[0][i], x0));
+                x1 = fmaf(bf16_low(ks[1][i]) * mul[0], c[i][2] + c[i][3], fmaf(mid(ks[1][i]), qsum[0][i], x1));
+            }
+            if (NG < 4 && t >= NG) x0 = x1 = 0.0f;  // head dim 64: two groups for four lanes
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                x0 += __shfl_xor_sync(ALL, x0, o);
+                x1 += __shfl_xor_sync(ALL, x1, o);
+            }
+            s0[0] = x0;
+            s1[0] = x1;
+        } else {
+            float b0[NT], b1[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) s0[n] = s1[n] = b0[n] = b1[n] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                uint32_t y0[4], y1[4];
+                codes_f16(kc[0][g], y0);
+                codes_f16(kc[1][g], y1);
+                const uint32_t a0[4] = {y0[0], y1[0], y0[1], y1[1]}, a1[4] = {y0[2], y1[2], y0[3], y1[3]};
+                const float sc0 = bf16_low(ks[0][g]), sc1 = bf16_low(ks[1][g]), mid0 = mid(ks[0][g]), mid1 = mid(ks[1][g]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + ((n * NG + g) * 32 + lane) * 16);
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_f16(c, a0, q.x, q.y);
+                    mma_f16(c, a1, q.z, q.w);
+                    s0[n] = fmaf(sc0, c[0] + c[1], s0[n]);
+                    s1[n] = fmaf(sc1, c[2] + c[3], s1[n]);
+                    b0[n] = fmaf(mid0, qsum[n][g], b0[n]);
+                    b1[n] = fmaf(mid1, qsum[n][g], b1[n]);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(smem + ((n * NG + g) * 32 + lane) * 16);
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma_f16(c, a0, q.x, q.y);
-                mma_f16(c, a1, q.z, q.w);
-                s0[n] = fmaf(bf16_low(cur.ks[0][g]), c[0] + c[1], s0[n]);
-                s1[n] = fmaf(bf16_low(cur.ks[1][g]), c[2] + c[3], s1[n]);
-                b0[n] = fmaf(mid(cur.ks[0][g]), qsum[n][g], b0[n]);
-                b1[n] = fmaf(mid(cur.ks[1][g]), qsum[n][g], b1[n]);
+                s0[n] = fmaf(s0[n], mul[n], b0[n]);
+                s1[n] = fmaf(s1[n], mul[n], b1[n]);
             }
         }
         float corr[NT];
         bool moved = false;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            s0[n] = ok0 ? fmaf(s0[n], mul[n], b0[n]) : -INFINITY;
-            s1[n] = ok1 ? fmaf(s1[n], mul[n], b1[n]) : -INFINITY;
+            if (edge) {
+                s0[n] = ok0 ? s0[n] : -INFINITY;
+                s1[n] = ok1 ? s1[n] : -INFINITY;
+            }
             float top = fmaxf(s0[n], s1[n]);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(ALL, top, o));
             corr[n] = 1.0f;
             if (top > m[n] + 8.0f || (m[n] == -INFINITY && top > m[n])) {
                 corr[n] = exp2_fast(m[n] - top);
-                m[n] = top;
+                m[n] = base[n] = top;
                 moved = true;
             }
         }
@@ -452,16 +573,20 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention
             for (int n = 0; n < NT; n++) {
                 l[n] *= corr[n];
 #pragma unroll
-                for (int g = 0; g < NG; g++) low[n][g] *= corr[n];
+                for (int g = 0; g < NS; g++) low[n][g] *= corr[n];
             }
-            float f[2];
+            float f[2];  // the factors of accumulator rows r and r + 8
+            if constexpr (ONE) {
+                f[0] = f[1] = corr[0];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {  // the factors of accumulator rows r and r + 8
-                const int h = min((r + 8 * i) / PARTS, HC - 1);
-                f[i] = __shfl_sync(ALL, corr[0], h & 3);
-                if constexpr (NT == 2) {
-                    const float other = __shfl_sync(ALL, corr[NT - 1], h & 3);
-                    if (h >= 4) f[i] = other;
+                for (int i = 0; i < 2; i++) {
+                    const int h = min((r + 8 * i) / PARTS, HEADS - 1);
+                    f[i] = __shfl_sync(ALL, corr[0], h & 3);
+                    if constexpr (NT == 2) {
+                        const float other = __shfl_sync(ALL, corr[NT - 1], h & 3);
+                        if (h >= 4) f[i] = other;
+                    }
                 }
             }
 #pragma unroll
@@ -474,42 +599,68 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention
         }
         // Weights times the values' scales, in bfloat16 parts, to the warp's tile: row head * PARTS
         // + part, slots 2 r and 2 r + 1 for keys r and r + 8.
-        __syncwarp();
+        uint32_t vs[2][NS];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            // No key yet: every score is -inf (weight 0) or a NaN.
-            const bool none = m[n] == -INFINITY;
-            const float p0 = none ? (s0[n] != s0[n] ? s0[n] : 0.0f) : exp2_fast(s0[n] - m[n]);
-            const float p1 = none ? (s1[n] != s1[n] ? s1[n] : 0.0f) : exp2_fast(s1[n] - m[n]);
-            l[n] += p0 + p1;
+        for (int i = 0; i < 2; i++) {
+            if constexpr (ONE) {
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                // A place behind the sequence's end may hold anything.
-                const uint32_t z0 = ok0 ? cur.vs[0][g] : 0u, z1 = ok1 ? cur.vs[1][g] : 0u;
-                low[n][g] = fmaf(p0, mid(z0), fmaf(p1, mid(z1), low[n][g]));
-                float w0 = p0 * bf16_low(z0), w1 = p1 * bf16_low(z1);
+                for (int j = 0; j < NS; j++) read_words<1>(cur + 10 * D + soff + 8 * i * NG * 4 + 16 * j, &vs[i][j]);
+            } else {
+                read_words<NG>(cur + 10 * D + soff + 8 * i * NG * 4, vs[i]);
+            }
+        }
+        if (edge) {  // a place behind the sequence's end may hold anything
 #pragma unroll
-                for (int part = 0; part < PARTS; part++) {
-                    const uint32_t w = pack_bf16(w0, w1);
-                    *reinterpret_cast<uint32_t *>(wt + (g * 16 + (n * 4 + t) * PARTS + part) * C::ROW_BYTES + 4 * r) = w;
-                    w0 -= bf16_low(w);
-                    w1 -= bf16_high(w);
-                }
+            for (int g = 0; g < NS; g++) {
+                if (!ok0) vs[0][g] = 0u;
+                if (!ok1) vs[1][g] = 0u;
             }
         }
         __syncwarp();
 #pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float p0 = exp2_fast(s0[n] - base[n]), p1 = exp2_fast(s1[n] - base[n]);
+            l[n] += p0 + p1;
+#pragma unroll
+            for (int g = 0; g < NS; g++) {
+                const uint32_t z0 = vs[0][g], z1 = vs[1][g];
+                low[n][g] = fmaf(p0, mid(z0), fmaf(p1, mid(z1), low[n][g]));
+                float w0 = p0 * bf16_low(z0), w1 = p1 * bf16_low(z1);
+                const int own = ONE ? t + 4 * g : g, row = ONE ? 0 : (n * 4 + t) * PARTS;
+                if (own < NG) {
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++) {
+                        const uint32_t w = pack_bf16(w0, w1);
+                        *reinterpret_cast<uint32_t *>(wt + (own * C::ROWS + row + part) * C::ROW_BYTES + 4 * r) = w;
+                        w0 -= bf16_low(w);
+                        w1 -= bf16_high(w);
+                    }
+                }
+            }
+        }
+        uint32_t vc[2][NG];
+#pragma unroll
+        for (int i = 0; i < 2; i++) read_words<NG>(cur + voff + i * 4 * 8 * 4 * NG, vc[i]);
+        __syncwarp();
+        // Every lane holds its part of the block: the stage takes the block STAGES further on.
+        if (v + C::STAGES * WARPS < v1) fetch(stage);
+        if (++stage == C::STAGES) stage = 0, parity ^= 1u;
+#pragma unroll
         for (int g = 0; g < NG; g++) {
             uint32_t w[4];
-            ldmatrix4(w, wt_addr + g * 16 * C::ROW_BYTES);
-            const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
-            const uint32_t y0 = __byte_perm(cur.v[0][g / 2], cur.v[1][g / 2], sel);
-            const uint32_t y1 = __byte_perm(cur.v[2][g / 2], cur.v[3][g / 2], sel);
+            ldmatrix4(w, wt_addr + g * C::ROWS * C::ROW_BYTES);
 #pragma unroll
-            for (int i = 0; i < 4; i++) mma_bf16(acc[g * 4 + i], w, codes_bf16(y0, i), codes_bf16(y1, i));
+            for (int i = 0; i < 4; i++) mma_bf16(acc[g * 4 + i], w, codes_bf16(vc[0][g], i), codes_bf16(vc[1][g], i));
         }
-        cur = nxt;
-        cur_ok = nxt_ok;
+    }
+    if (v < v1) {
+        // A wait ran out: let this warp's copies land before the block's memory goes away. (fetch at v
+        // has refilled the stages of the blocks before v: those of v .. v + STAGES - 1 may be in flight.)
+        volatile int never = 0;
+        for (int i = 0; i < C::STAGES && v + i * WARPS < v1; i++) {
+            sm100::mbar_wait_warp(full + 8 * stage, parity, &never, nullptr);
+            if (++stage == C::STAGES) stage = 0, parity ^= 1u;
+        }
     }
 
     // Join the warps.
@@ -519,16 +670,21 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention
         for (int o = 4; o < 32; o <<= 1) {
             l[n] += __shfl_xor_sync(ALL, l[n], o);
 #pragma unroll
-            for (int g = 0; g < NG; g++) low[n][g] += __shfl_xor_sync(ALL, low[n][g], o);
+            for (int g = 0; g < NS; g++) low[n][g] += __shfl_xor_sync(ALL, low[n][g], o);
         }
         if (r == 0) {
-            s_m[warp][n * 4 + t] = m[n];
-            s_l[warp][n * 4 + t] = l[n];
+            const int h = ONE ? 0 : n * 4 + t;
+            s_m[warp][h] = m[n];
+            s_l[warp][h] = l[n];
 #pragma unroll
-            for (int g = 0; g < NG; g++) s_low[warp][n * 4 + t][g] = low[n][g];
+            for (int g = 0; g < NS; g++) {
+                const int own = ONE ? t + 4 * g : g;
+                if (own < NG) s_low[warp][h][own] = low[n][g];
+            }
         }
     }
     __syncthreads();
+    if (*abort) return;  // the row is left unwritten; the device status tells
     float *sacc = reinterpret_cast<float *>(smem) + warp * C::ROWS * D;
 #pragma unroll
     for (int i = 0; i < 4 * NG; i++)
@@ -557,29 +713,30 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : 3) cache4_attention
     }
 }
 
-template <int D, int PARTS, int NT>
+template <int D, int PARTS, int HEADS>
 int launch_attention(const Cache4Args &a, const SplitRows &rows, cudaStream_t stream) {
-    using C = AttnCfg<D, PARTS, NT>;
-    auto kernel = cache4_attention_kernel<D, PARTS, NT>;
+    using C = AttnCfg<D, PARTS, HEADS>;
+    auto kernel = cache4_attention_kernel<D, PARTS, HEADS>;
     if (C::SMEM > 40 * 1024) {  // with the static arrays, past the 48 KB that need no attribute
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return cuda_fail(e, "cache4_attention smem attribute");
     }
-    const int64_t group = a.H / a.c.Hkv, chunks = (group + C::HC - 1) / C::HC;
+    const int64_t group = a.H / a.c.Hkv, chunks = (group + HEADS - 1) / HEADS;
     KernelTrace tr("cache4_attention", stream);
     kernel<<<dim3((unsigned)rows.splits, (unsigned)(a.c.Hkv * chunks), (unsigned)a.B), WARPS * 32, C::SMEM, stream>>>(a, rows);
     return check_launch("cache4_attention");
 }
 
-// Heads of one key/value head that a CTA takes: 4, or 8 where the parts of 8 heads' weights fit the
-// product's 16 rows.
-int heads_per_cta(int64_t group, int dtype) { return dtype != DC_F32 && group > 4 ? 8 : 4; }
+// Heads of one key/value head that a CTA takes: a single one has its own kernel; otherwise 4, or 8 where
+// the parts of 8 heads' weights fit the product's 16 rows (two parts: 16-bit queries).
+int heads_per_cta(int64_t group, int dtype) { return group == 1 ? 1 : (dtype != DC_F32 && group > 4 ? 8 : 4); }
 
 template <int D>
 int launch_dim(const Cache4Args &a, const SplitRows &rows, cudaStream_t stream) {
-    if (a.dtype == DC_F32) return launch_attention<D, 3, 1>(a, rows, stream);
-    return heads_per_cta(a.H / a.c.Hkv, a.dtype) == 8 ? launch_attention<D, 2, 2>(a, rows, stream)
-                                                      : launch_attention<D, 2, 1>(a, rows, stream);
+    const int heads = heads_per_cta(a.H / a.c.Hkv, a.dtype);
+    if (a.dtype == DC_F32) return heads == 1 ? launch_attention<D, 3, 1>(a, rows, stream) : launch_attention<D, 3, 4>(a, rows, stream);
+    if (heads == 1) return launch_attention<D, 2, 1>(a, rows, stream);
+    return heads == 8 ? launch_attention<D, 2, 8>(a, rows, stream) : launch_attention<D, 2, 4>(a, rows, stream);
 }
 
 // Whether runs of four channels of a (B, H, T, D) view start on 4-element boundaries.
@@ -612,13 +769,16 @@ int cache4_read(const Cache4Args &a, cudaStream_t stream) {
     return check_launch("cache4_read");
 }
 
-// Splits of each row: three CTAs of 4 warps on every SM twice over, at least one block a warp.
+// Splits of each row: enough CTAs to fill every SM's four places six times over, so that sequences of
+// different lengths even out, with at least 8 blocks a warp then; below that, down to one block a warp,
+// as many as fill the places once.
 int cache4_splits(int64_t B, int64_t H, int64_t Hkv, int64_t capacity, int64_t window, int64_t sinks, int dtype) {
     const int64_t group = H / Hkv, per = heads_per_cta(group, dtype), chunks = (group + per - 1) / per;
     const int64_t ctas = std::max<int64_t>(1, B * Hkv * chunks);
     const int64_t keys = window ? std::min(capacity, std::min(window, capacity) + std::min(sinks, capacity)) : capacity;
-    const int64_t fill = (int64_t)device_sm_count() * 6 / ctas, most = (keys + 16 * WARPS - 1) / (16 * WARPS);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(128, std::min(fill, most)));
+    const int64_t places = (int64_t)device_sm_count() * 4, most = (keys + 16 * WARPS - 1) / (16 * WARPS);
+    const int64_t once = std::min(places / ctas, most), even = std::min((6 * places + ctas - 1) / ctas, most / 8);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(once, even)));
 }
 
 int cache4_attention(const Cache4Args &a, const SplitRows &rows, cudaStream_t stream) {

@@ -84,16 +84,16 @@ int fill_weight(const char *what, const dc_tensor_t *w, int dtype, int64_t D) {
 
 // A cache's description.
 int fill_cache(const dc_cache4_t *cache, Cache4 &c) {
-    if (!cache || !cache->codes || !cache->scales) return fail(DC_ERR_VALUE, "cache: codes and scales are required");
-    if ((reinterpret_cast<uintptr_t>(cache->codes) & 15u) || (reinterpret_cast<uintptr_t>(cache->scales) & 15u))
-        return fail(DC_ERR_VALUE, "cache: codes and scales must be 16-byte aligned");
+    if (!cache || !cache->data) return fail(DC_ERR_VALUE, "cache: its memory is required");
+    if (reinterpret_cast<uintptr_t>(cache->data) & 15u) return fail(DC_ERR_VALUE, "cache: its memory must be 16-byte aligned");
     if (cache->num_pages < 1 || cache->num_pages > 0x7fffffff || cache->kv_heads < 1 || cache->kv_heads > 32767)
         return fail(DC_ERR_VALUE, "cache: pages and heads must be at least 1, pages below 2^31, heads below 2^15");
     if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
         return fail(DC_ERR_UNSUPPORTED, "cache: the head dim must be 64, 128 or 256");
     if (cache->page_size < 16 || cache->page_size % 16) return fail(DC_ERR_VALUE, "cache: the page size must be a multiple of 16");
-    c.codes = static_cast<uint8_t *>(cache->codes);
-    c.scales = static_cast<uint32_t *>(cache->scales);
+    if (cache->num_pages * cache->kv_heads >= (1ll << 31) / (cache->page_size / 16))
+        return fail(DC_ERR_UNSUPPORTED, "cache: 2^31 blocks of 16 tokens and more");
+    c.data = static_cast<uint8_t *>(cache->data);
     c.pages = cache->num_pages;
     c.Hkv = cache->kv_heads;
     c.D = cache->head_dim;

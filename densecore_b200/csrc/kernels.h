@@ -75,8 +75,7 @@ int rotary_launch(RotaryArgs &a, int dtype, bool interleaved, int mode, cudaStre
 
 // The 4-bit key/value cache (cache4.cu).
 struct Cache4 {
-    uint8_t *codes;    // (pages, 2, Hkv, page_size, D / 2)
-    uint32_t *scales;  // (pages, 2, Hkv, page_size, D / 32): scale | low << 16, bfloat16 each
+    uint8_t *data;  // (pages, Hkv, page_size / 16) blocks of 20 D bytes (cache4.cu)
     int64_t pages;
     int Hkv, D, page_size;
 };

@@ -232,15 +232,14 @@ DC_API int dc_qk_norm_rotary_bwd(const dc_tensor_t *q_grad, const dc_tensor_t *k
  * bfloat16, scale = (its largest - low) / 15 rounded up to bfloat16, and codes = (x - low) / scale
  * rounded to nearest even, in 32-bit arithmetic; it stands for low + scale * code. A group with an
  * infinity or a NaN stands for NaN.
- *  codes   num_pages * 2 * kv_heads * page_size * head_dim / 2 bytes, scales 4 bytes per group;
- *          16-byte aligned device memory of the caller's. All zero is a cache of zeros.
+ *  data: num_pages * kv_heads * (page_size / 16) * 20 * head_dim bytes of the caller's device memory,
+ *  16-byte aligned; a page is contiguous. All zero is a cache of zeros.
  *  Page tables (B, P), lengths, start and end positions (B) are int32 device tensors. A position
  *  outside the table, a length outside 0..P * page_size or a page id outside 0..num_pages - 1 sets
  *  dc_device_status() to 3; it is then not written, reads as zero, or is left out of the attention
  *  (lengths are clamped). Entries behind a sequence's length are not read. */
 typedef struct dc_cache4 {
-    void *codes;
-    void *scales;
+    void *data;
     int64_t num_pages;
     int32_t kv_heads, head_dim, page_size; /* head_dim 64, 128 or 256; page_size a multiple of 16 */
 } dc_cache4_t;

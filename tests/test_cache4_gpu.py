@@ -75,12 +75,12 @@ def test_append_and_read(dtype, dim, layout):
             want[i, :, start[i]:end[i]] = d[i, :, :n]
         assert torch.equal(y, want)
     # places from `end` on, and pages of no sequence, keep what they hold
-    before = cache.codes.clone(), cache.scales.clone()
+    before = cache.data.clone()
     cache.append(k * 0, v, table, start, start)
-    assert torch.equal(cache.codes, before[0]) and torch.equal(cache.scales, before[1])
+    assert torch.equal(cache.data, before)
     unused = torch.ones(pages, dtype=torch.bool, device="cuda")
     unused[table.flatten().long()] = False
-    assert (cache.codes[unused] == 0).all()
+    assert (cache.data[unused] == 0).all()
     # one token at a time
     one = dc.KVCache4(pages, kv, dim, page_size=page)
     for i in range(5):
@@ -214,10 +214,10 @@ def test_entries_out_of_range_are_reported_and_left_out():
     assert status() == 3 and torch.isfinite(got).all() and torch.equal(got[1], want[1])
     k, _ = cache.read(bad, lens, 64)
     assert status() == 3 and (k[0, :, 16:32] == 0).all() and (k[0, :, :16] != 0).any()
-    before = cache.codes.clone()
+    before = cache.data.clone()
     x = torch.randn(2, 1, 4, 64, device="cuda")
     cache.append(x, x, table, i32(-4, 64))  # before the start, behind the table
-    assert status() == 3 and torch.equal(cache.codes, before)
+    assert status() == 3 and torch.equal(cache.data, before)
     assert status() == 0
 
 
@@ -254,7 +254,7 @@ def test_cache_of_more_than_four_gigabytes():
     if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
         pytest.skip("needs memory")
     page, kv, dim = 256, 8, 256
-    pages = (5 << 30) // (2 * kv * page * dim // 2)
+    pages = (5 << 30) // (kv * page // 16 * 20 * dim)
     cache = dc.KVCache4(pages, kv, dim, page_size=page)
     table = i32(pages - 1, 0).view(1, 2)
     x = torch.randn(1, kv, 300, dim, device="cuda")

@@ -192,18 +192,18 @@ def test_c_entry_points_refuse_before_any_device_work():
     spread = fake((2, 4, 8, 64))
     spread.strides[1] = 0  # an output whose heads share memory
     assert rotary(out=spread) == _lib.DC_ERR_VALUE
-    cache = _lib.DcCache4(0x10000, 0x20000, 4, 2, 64, 16)
+    cache = _lib.DcCache4(0x10000, 4, 2, 64, 16)
     table, n, one = fake((2, 3), _lib.DC_I32), fake((2,), _lib.DC_I32), fake((2, 4, 1, 64))
 
     def attention(cache=cache, q=one, table=table, n=n, window=0, sinks=0, out=one, lse=fake((2, 4, 1))):
         return L.dc_cache4_attention(ctypes.byref(cache), r(q), r(table), r(n), window, sinks, 0, 0.0, r(out), r(lse), None, 0, None)
 
-    for kw in (dict(cache=_lib.DcCache4(0, 0x20000, 4, 2, 64, 16)), dict(cache=_lib.DcCache4(0x10004, 0x20000, 4, 2, 64, 16)),
-               dict(cache=_lib.DcCache4(0x10000, 0x20000, 4, 2, 64, 20)), dict(q=fake((2, 3, 1, 64))),
+    for kw in (dict(cache=_lib.DcCache4(0, 4, 2, 64, 16)), dict(cache=_lib.DcCache4(0x10004, 4, 2, 64, 16)),
+               dict(cache=_lib.DcCache4(0x10000, 4, 2, 64, 20)), dict(q=fake((2, 3, 1, 64))),
                dict(q=fake((2, 4, 2, 64))), dict(table=fake((2, 3), _lib.DC_I64)), dict(n=fake((3,), _lib.DC_I32)),
                dict(window=-1), dict(out=fake((2, 4, 1, 64), _lib.DC_BF16)), dict(lse=fake((2, 4)))):
         assert attention(**kw) == _lib.DC_ERR_VALUE, kw
-    assert attention(cache=_lib.DcCache4(0x10000, 0x20000, 4, 2, 96, 16)) == _lib.DC_ERR_UNSUPPORTED
+    assert attention(cache=_lib.DcCache4(0x10000, 4, 2, 96, 16)) == _lib.DC_ERR_UNSUPPORTED
     assert attention(table=fake((2, 1 << 28), _lib.DC_I32)) == _lib.DC_ERR_UNSUPPORTED
     if not torch.cuda.is_available():
         assert window() == rotary() == attention() == _lib.DC_ERR_CUDA
