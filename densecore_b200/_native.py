@@ -12,6 +12,7 @@ materialised (B, H, L, S) float mask is accepted as one case of it.
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -214,7 +215,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 def _on(dev):
     """The context in which ``dev`` is the current device."""
-    return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _device_of(first, *rest):
@@ -238,24 +239,53 @@ def _stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _sliding_window(q, k, v, window, sinks, offset, scale=None, mask=None, lengths=None, precision=None):
-    """Forward through a sliding window (dc_sdpa_window_fwd): (out, lse)."""
+# Scratch sizes depend on sizes (and the device's SM count) only; asking the library costs as much as a
+# launch, which shows in single-token calls. `index`: the device's.
+@functools.lru_cache(maxsize=1024)
+def _window_scratch(index, *sizes):
+    return _lib.load().dc_sdpa_window_fwd_workspace_size(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _cache4_scratch(index, *sizes):
+    return _lib.load().dc_cache4_attention_workspace_size(*sizes)
+
+
+def _decode_buffers(like, rows_shape, scratch, need_lse):
+    """(logsumexp or None, its packed view, scratch pointer, the tensor that holds the scratch): a
+    logsumexp that nobody asked for lies behind the scratch, in one allocation."""
+    b, h = rows_shape
+    if need_lse:
+        lse = torch.empty((b, h, 1), device=like.device, dtype=torch.float32)
+        hold = torch.empty(scratch, dtype=torch.uint8, device=like.device) if scratch else None
+        return lse, _lib.packed(lse), hold.data_ptr() if scratch else None, hold
+    at = (scratch + 15) // 16 * 16
+    hold = torch.empty(at + 4 * b * h, dtype=torch.uint8, device=like.device)
+    ptr = hold.data_ptr()
+    return None, _lib._PACK[3](ptr + at, _lib.DC_F32, 3, b, h, 1, h, 1, 1), ptr if scratch else None, hold
+
+
+def _sliding_window(q, k, v, window, sinks, offset, scale=None, mask=None, lengths=None, precision=None, need_lse=True):
+    """Forward through a sliding window (dc_sdpa_window_fwd): (out, lse); one query row without
+    ``need_lse``: (out, None)."""
     L = _lib.load()
     dev = _device_of(q, k, v, mask, lengths)
     B, H, Lq, E = q.shape
-    S, Ev = k.shape[2], v.shape[3]
-    out = torch.empty((B, H, Lq, Ev), device=dev, dtype=torch.float32)
-    lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32)
+    Hkv, S, Ev = k.shape[1], k.shape[2], v.shape[3]
+    out = torch.empty_like(q) if E == Ev else torch.empty((B, H, Lq, Ev), device=dev, dtype=torch.float32)
     prec = precision_code() if precision is None else precision
     has, sc = _scale_args(scale)
     with _on(dev):
-        need = 0
-        if Lq == 1 and k.shape[1] and H % k.shape[1] == 0:
-            need = L.dc_sdpa_window_fwd_workspace_size(B, H, k.shape[1], Lq, S, E, window, sinks)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        r = _refs(q, k, v, mask, lengths, out, lse)
-        st = L.dc_sdpa_window_fwd(*r[:4], window, sinks, offset, r[4], has, sc, prec, r[5], r[6],
-                                  ws.data_ptr() if need else None, need, _stream(dev))
+        if Lq == 1:
+            need = _window_scratch(dev.index, B, H, Hkv, Lq, S, E, window, sinks) if Hkv and H % Hkv == 0 else 0
+            lse, lse_ref, ptr, _hold = _decode_buffers(q, (B, H), need, need_lse)
+        else:
+            need, ptr = 0, None
+            lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32)
+            lse_ref = _lib.packed(lse)
+        r = _refs(q, k, v, mask, lengths, out)
+        st = L.dc_sdpa_window_fwd(*r[:4], window, sinks, offset, r[4], has, sc, prec, r[5], lse_ref, ptr, need,
+                                  _stream(dev))
     _lib.check(st, "sliding window attention failed")
     return out, lse
 
@@ -346,23 +376,21 @@ def _cache4_read(desc, page_table, lengths, max_length):
     return key, value
 
 
-def _cache4_attention(desc, q, page_table, lengths, window=0, sinks=0, scale=None):
-    """One token per sequence over a 4-bit cache (dc_cache4_attention): (out, lse)."""
+def _cache4_attention(desc, q, page_table, lengths, window=0, sinks=0, scale=None, need_lse=True):
+    """One token per sequence over a 4-bit cache (dc_cache4_attention): (out, lse), or (out, None)
+    without ``need_lse``."""
     L = _lib.load()
     dev = _device_of(q, page_table, lengths)
     B, H = q.shape[:2]
     out = torch.empty_like(q)
-    lse = torch.empty((B, H, 1), device=dev, dtype=torch.float32)
     has, sc = _scale_args(scale)
     with _on(dev):
-        r = _refs(q, page_table, lengths, out, lse)
-        need = 0
-        if H and H % desc.kv_heads == 0:
-            need = L.dc_cache4_attention_workspace_size(B, H, desc.kv_heads, desc.head_dim,
-                                                        page_table.shape[1] * desc.page_size, window, sinks,
-                                                        _lib._DTYPES[q.dtype])
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        st = L.dc_cache4_attention(_lib.ref(desc), *r[:3], window, sinks, has, sc, r[3], r[4],
-                                   ws.data_ptr() if need else None, need, _stream(dev))
+        kv = desc.kv_heads
+        need = _cache4_scratch(dev.index, B, H, kv, desc.head_dim, page_table.shape[1] * desc.page_size, window, sinks,
+                               _lib._DTYPES[q.dtype]) if H and H % kv == 0 else 0
+        lse, lse_ref, ptr, _hold = _decode_buffers(q, (B, H), need, need_lse)
+        q_, table_, lengths_, out_ = _refs(q, page_table, lengths, out)
+        st = L.dc_cache4_attention(_lib.ref(desc), q_, table_, lengths_, window, sinks, has, sc, out_, lse_ref, ptr, need,
+                                   _stream(dev))
     _lib.check(st, "cache attention failed")
     return out, lse

@@ -14,7 +14,7 @@ from . import _lib, _native
 
 
 def _whole(name, value, least):
-    if isinstance(value, bool) or not isinstance(value, numbers.Integral):
+    if type(value) is not int and (isinstance(value, bool) or not isinstance(value, numbers.Integral)):
         raise TypeError(f"{name} must be a whole number")
     if value < least:
         raise ValueError(f"{name} must be at least {least}")
@@ -118,5 +118,5 @@ class KVCache4:
             raise TypeError("scale must be real")
         window = 0 if window is None else _whole("window", window, 1)
         out, lse = _native._cache4_attention(self._desc, query, page_table, lengths, window,
-                                             _whole("sinks", sinks, 0), scale)
+                                             _whole("sinks", sinks, 0), scale, return_lse)
         return (out, lse) if return_lse else out

@@ -20,15 +20,18 @@
 // are applied to their results (keys) or to the weights before (values):
 //   s_j    = sum_g scale_jg (q_g . c_jg) + mid_jg sum(q_g)
 //   out_c  = sum_j (p_j scale_jg) c_jc + sum_j p_j mid_jg
-// with c = code - 8 and mid = low + 8 scale: centred, so that the two parts cancel little. c is exact
-// in 16 bits, and a normal number there: fed as fp16 subnormals (code * 2^-24, one instruction a pair
-// less) the same products came out 10 times less exact, the tensor core aligning its terms by the
-// exponents as written. q is scaled by a power of two and split into two fp16 parts (22
-// bits below the head's largest channel), p * scale into bfloat16 parts (three for float32 queries:
-// 24 bits; two for 16-bit queries), a part being a row or column of the product: one m16n8k16
-// product takes 16 keys, 4 heads and both parts. mma.sync, not tcgen05: at one query row per head the
-// products fill an eighth of even these tiles, their time is far from the bound, and their operands
-// come straight from registers (4-bit codes would have to be expanded into shared memory first).
+// with c = code - 8 and mid = low + 8 scale: centred, so that the two parts cancel little. The small
+// operand is scaled by a power of two and split into parts that a product takes as rows or columns:
+//   weights  p * scale into bfloat16 parts (three for float32 queries: 24 bits; two for 16-bit ones)
+//   q        one head per CTA: as a 28-bit integer in four signed digits to the base 128, multiplied
+//            with the codes as bytes (m16n8k32, exact sums; half the unpacking of 16-bit codes);
+//            several: two fp16 parts (22 bits below the head's largest channel), so that a group's
+//            product gives a lane both parts of one head (m16n8k16)
+// Codes are exact in every one of these types. (As fp16 subnormals, code * 2^-24, they come without a
+// subtraction, but the sums came out 10 times less exact: the tensor core aligns its terms by the
+// exponents as written.) mma.sync, not tcgen05: at one query row per head the products fill an eighth of
+// even these tiles, their time is far from the bound, and their operands come straight from registers
+// (4-bit codes would have to be expanded into shared memory first).
 // A warp works alone on blocks of 16 keys (never across a page), which bulk copies bring into a ring of
 // its own in shared memory a few blocks ahead; its own running maximum, which moves only when it grows
 // by more than 2^8 (sum, mids and accumulators share it), is joined with the other warps' at the end.
@@ -90,7 +93,7 @@ __host__ __device__ constexpr int block_bytes(int D) { return 20 * D; }
 
 // Where halfword (group g, r) of token `slot` (0..15) lies among a block's codes of keys or values.
 __device__ __forceinline__ int code_at(int which, int slot, int r, int g, int ng) {
-    return which ? 2 * (((slot % 8) * 8 + r) * ng + g) + slot / 8 : 2 * ((slot * 4 + r / 2) * ng + g) + r % 2;
+    return which ? 2 * (((slot / 4 % 2 * 8 + r) * 4 + slot % 4) * ng + g) + slot / 8 : 2 * ((slot * 4 + r / 2) * ng + g) + r % 2;
 }
 
 // The keys or values of the block of 16 tokens that holds position pos of sequence b, and its slot
@@ -220,25 +223,25 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bo
 
 // --------------------------------------------------------------------------- attention ----
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + c. (d may be c.)
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 // (a, b) rounded to bfloat16, a in the low half.
@@ -247,18 +250,24 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
+// (x & mask) | bits in one instruction (the compiler made two of it).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+    return r;
+}
 // The four pairs of codes of y, less 8, as fp16: pairs 0 and 2 as they are, 1 and 3 times 16 (their
 // bits lie four higher in the mantissa, which saves a shift; q is divided by 16 there).
 __device__ __forceinline__ void codes_f16(uint32_t y, uint32_t (&c)[4]) {
     const uint32_t z = y >> 8;
-    const uint32_t w[4] = {(y & 0x000F000Fu) | 0x64006400u, (y & 0x00F000F0u) | 0x64006400u,  // 1024 + code, 1024 + 16 code
-                           (z & 0x000F000Fu) | 0x64006400u, (z & 0x00F000F0u) | 0x64006400u};
+    const uint32_t w[4] = {and_or(y, 0x000F000Fu, 0x64006400u), and_or(y, 0x00F000F0u, 0x64006400u),  // 1024 + code, 1024 + 16 code
+                           and_or(z, 0x000F000Fu, 0x64006400u), and_or(z, 0x00F000F0u, 0x64006400u)};
 #pragma unroll
     for (int i = 0; i < 4; i++) asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(c[i]) : "r"(w[i]), "r"((i & 1) ? 0x64806480u : 0x64086408u));
 }
 // Pair i of codes, less 8, as bfloat16.
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t y, int i) {
-    const uint32_t z = ((y >> (4 * i)) & 0x000F000Fu) | 0x43004300u;  // 128 + code
+    const uint32_t z = and_or(y >> (4 * i), 0x000F000Fu, 0x43004300u);  // 128 + code
     uint32_t r;
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(z), "r"(0x43084308u));
     return r;
@@ -300,16 +309,23 @@ struct AttnCfg {
     static constexpr bool ONE = HEADS == 1;
     static constexpr int NT = ONE ? 1 : HEADS / 4;              // heads of a lane
     static constexpr int NS = ONE ? (NG + 3) / 4 : NG;          // groups of a lane
-    static constexpr int ROWS = HEADS * PARTS;                  // rows of the second product in use
-    static_assert(ROWS <= 16, "the parts of the weights fill one product's rows");
-    static constexpr int ROW_BYTES = 48;                        // 16 weights of a row, padded against bank conflicts
+    // The values' product: channels x keys times keys x columns, a column being a part of a head's weights.
+    // A lane's columns 2 t, 2 t + 1 of tile n are its own heads': parts 0, 1 of head 4 n + t (two parts), or
+    // parts 2 n, 2 n + 1 of head t (three); of one head simply parts 0, 1, ...
+    static constexpr int COLS = ONE ? 8 : (PARTS == 2 ? 2 * HEADS : 16), NC = COLS / 8;
+    static_assert(ONE || PARTS == 2 || HEADS == 4, "three parts: four heads");
+    __host__ __device__ static constexpr int column(int head, int part) {
+        return ONE ? part : (PARTS == 2 ? head / 4 * 8 + head % 4 * 2 + part : part / 2 * 8 + head * 2 + part % 2);
+    }
+    // A group's tile of weights: COLS rows of 16 keys in bfloat16, padded against bank conflicts.
+    static constexpr int W_GROUP = COLS * 32 + 32;
     static constexpr int STAGES = D == 64 ? 4 : (D == 128 ? 3 : 2);  // blocks of a warp's ring
     // Shared memory: the warps' rings | q fragments | the warps' weight tiles; after the loop the
     // accumulators.
     static constexpr int BLOCK = block_bytes(D), RING = STAGES * BLOCK;
-    static constexpr int Q_BYTES = NT * NG * 32 * 16, W_BYTES = NG * ROWS * ROW_BYTES;
+    static constexpr int Q_BYTES = NT * NG * 32 * 16, W_BYTES = NG * W_GROUP;
     static constexpr int OFF_Q = WARPS * RING, OFF_W = OFF_Q + Q_BYTES, LOOP_BYTES = OFF_W + WARPS * W_BYTES;
-    static constexpr int ACC_BYTES = WARPS * ROWS * D * 4;
+    static constexpr int ACC_COLS = ONE ? PARTS : COLS, ACC_BYTES = WARPS * ACC_COLS * D * 4;
     static constexpr int SMEM = LOOP_BYTES > ACC_BYTES ? LOOP_BYTES : ACC_BYTES;
 };
 
@@ -320,7 +336,7 @@ __device__ __forceinline__ float load_q(const Cache4Args &a, int64_t at) {
 }
 
 template <int D, int PARTS, int HEADS>
-__global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4))
+__global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : (HEADS == 1 ? 5 : 4)))
     cache4_attention_kernel(const Cache4Args a, const SplitRows rows) {
     using C = AttnCfg<D, PARTS, HEADS>;
     constexpr int NG = C::NG, NT = C::NT, NS = C::NS;
@@ -328,6 +344,7 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t s_full[WARPS][C::STAGES];
     __shared__ int s_abort;
+    __shared__ int s_digits[NG][4];  // one head: the sums of each group's digits
     __shared__ float s_qsum[HEADS][NG], s_exp[HEADS], s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_low[WARPS][HEADS][NG];
     griddep_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
@@ -414,31 +431,51 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(ALL, top, o));
         int e = 0;
         if (top > 0.0f && top <= 3.402823466e38f) frexpf(top, &e);
+        bool finite = true;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             float s = x[g];
+            finite = finite && fabsf(s) <= 3.402823466e38f;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(ALL, s, o);
             if (lane == 0) s_qsum[h][g] = s * (a.scale * LOG2E);
-            // Channel 32 g + lane = 4 r' + i of a group: k-pair member r' & 1 of lane t' = r' / 2, pair i.
-            const int rr = lane >> 2, i = lane & 3;
-            const float y = ldexpf(x[g], (i & 1) ? -e - 4 : -e);
-            const __half hi = __float2half_rn(y), lo16 = __float2half_rn(y - __half2float(hi));
+            if constexpr (ONE) {
+                // Channel 32 g + lane = 8 t' + 2 j + high: byte j of lane t', low or high nibbles.
+                int y = __float2int_rn(ldexpf(x[g], 27 - e));
 #pragma unroll
-            for (int part = 0; part < 2; part++) {
-                const int col = (ONE ? g & 3 : h & 3) * 2 + part, tile = ONE ? 0 : h >> 2;
-                __half *frag = reinterpret_cast<__half *>(smem + C::OFF_Q + ((tile * NG + g) * 32 + col * 4 + (rr >> 1)) * 16);
-                frag[i * 2 + (rr & 1)] = part ? lo16 : hi;
+                for (int digit = 0; digit < 4; digit++) {  // lowest first
+                    const int d = digit == 3 ? y : ((y + 64) & 127) - 64;
+                    y = (y - d) >> 7;
+                    // columns 2 (g & 3), + 1: of the high pair (digits 3, 2) or the low pair (1, 0)
+                    const int col = (g & 3) * 2 + 1 - (digit & 1), pair = digit >= 2 ? 0 : 1;
+                    int8_t *frag = reinterpret_cast<int8_t *>(smem + C::OFF_Q + (g * 32 + col * 4 + (lane >> 3)) * 16);
+                    frag[pair * 8 + (lane & 1) * 4 + ((lane >> 1) & 3)] = (int8_t)d;
+                    const int sum = __reduce_add_sync(ALL, d);
+                    if (lane == 0) s_digits[g][3 - digit] = sum;
+                }
+            } else {
+                // Channel 32 g + lane = 4 r' + i of a group: k-pair member r' & 1 of lane t' = r' / 2, pair i.
+                const int rr = lane >> 2, i = lane & 3;
+                const float y = ldexpf(x[g], (i & 1) ? 10 - e : 14 - e);  // far above the subnormals, low part too
+                const __half hi = __float2half_rn(y), lo16 = __float2half_rn(y - __half2float(hi));
+#pragma unroll
+                for (int part = 0; part < 2; part++) {
+                    const int col = (h & 3) * 2 + part;
+                    __half *frag = reinterpret_cast<__half *>(smem + C::OFF_Q + (((h >> 2) * NG + g) * 32 + col * 4 + (rr >> 1)) * 16);
+                    frag[i * 2 + (rr & 1)] = part ? lo16 : hi;
+                }
             }
         }
-        if (lane == 0) s_exp[h] = ldexpf(a.scale * LOG2E, e);
+        // (An infinity or a NaN does not survive the digits: it goes into the factor.)
+        finite = __all_sync(ALL, finite);
+        if (lane == 0) s_exp[h] = finite ? ldexpf(a.scale * LOG2E, ONE ? e - 27 : e - 14) : NAN;
     }
     __syncthreads();
 
     // Heads n * 4 + t (one head: head 0), groups g (one head: t + 4 g) of this lane.
     // m: the running maximum; base: what the weights are relative to (m, or 0 before there is one).
     float mul[NT], qsum[NT][NS], m[NT], base[NT], l[NT], low[NT][NS];
-    float acc[4 * NG][4];
+    float acc[2 * NG][C::NC][4];  // channels 32 g + 4 r + 2 j (and + 1) of tile 2 g + j
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         mul[n] = s_exp[ONE ? 0 : n * 4 + t];
@@ -451,19 +488,33 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
             low[n][g] = 0.0f;
         }
     }
+    // One head: -8 times the sums of digits 3, 2 (and 1, 0), which turns codes into code - 8.
+    int centre_hi[ONE ? NS : 1][4], centre_lo[ONE ? NS : 1][4];
+    if constexpr (ONE) {
 #pragma unroll
-    for (int i = 0; i < 4 * NG; i++)
+        for (int g = 0; g < NS; g++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) acc[i][c] = 0.0f;
+            for (int i = 0; i < 4; i++) {
+                centre_hi[g][i] = t + 4 * g < NG ? -8 * s_digits[t + 4 * g][i & 1] : 0;
+                centre_lo[g][i] = t + 4 * g < NG ? -8 * s_digits[t + 4 * g][2 + (i & 1)] : 0;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NG; i++)
+#pragma unroll
+        for (int n = 0; n < C::NC; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[i][n][c] = 0.0f;
+    // The warp's weight tiles. Keys r and r + 8 (slots 2 r, 2 r + 1 of the product) are stored at place
+    // r % 4, half r / 4, so that a lane's four slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9 are eight bytes.
     uint8_t *wt = smem + C::OFF_W + warp * C::W_BYTES;
-    // (Rows past the tile's are read as its last: what they give is never looked at.)
-    const uint32_t wt_addr = (uint32_t)__cvta_generic_to_shared(wt) + min(lane & 15, C::ROWS - 1) * C::ROW_BYTES + (lane >> 4) * 16;
+    const uint32_t wt_put = (r & 3) * 8 + (r >> 2) * 4, wt_get = r * 32 + t * 8;
 
     // This lane's places in a block: codes of keys r and r + 8 (its quarter of each group), of values
     // (t, t + 8) and (t + 4, t + 12) (its eighth of each group), and of both the scales of places r and
     // r + 8.
     const uint8_t *blk = smem + warp * C::RING;
-    const uint32_t koff = r * (D / 2) + t * 4 * NG, voff = 10 * D + (t * 8 + r) * 4 * NG;
+    const uint32_t koff = r * (D / 2) + t * 4 * NG, voff = 10 * D + lane * 4 * NG;
     const uint32_t soff = 8 * D + (r * NG + (ONE ? (NG < 4 ? t % NG : t) : 0)) * 4;
     int stage = 0;
     uint32_t parity = 0;
@@ -494,24 +545,23 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
         // Scores of keys r and r + 8.
         float s0[NT], s1[NT];
         if constexpr (ONE) {
-            float c[NS][4];
-#pragma unroll
-            for (int i = 0; i < NS; i++) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
+            int hi[NS][4], lw[NS][4];  // digits 3, 2 and 1, 0 of keys r, r + 8
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                uint32_t y0[4], y1[4];
-                codes_f16(kc[0][g], y0);
-                codes_f16(kc[1][g], y1);
+                const uint32_t y[4] = {kc[0][g] & 0x0F0F0F0Fu, kc[1][g] & 0x0F0F0F0Fu, (kc[0][g] >> 4) & 0x0F0F0F0Fu,
+                                       (kc[1][g] >> 4) & 0x0F0F0F0Fu};
                 const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + (g * 32 + lane) * 16);
-                const uint32_t a0[4] = {y0[0], y1[0], y0[1], y1[1]}, a1[4] = {y0[2], y1[2], y0[3], y1[3]};
-                mma_f16(c[g / 4], a0, q.x, q.y);
-                mma_f16(c[g / 4], a1, q.z, q.w);
+                mma_u8s8(hi[g / 4], y, q.x, q.y, g % 4 ? hi[g / 4] : centre_hi[g / 4]);
+                mma_u8s8(lw[g / 4], y, q.z, q.w, g % 4 ? lw[g / 4] : centre_lo[g / 4]);
             }
             float x0 = 0.0f, x1 = 0.0f;
 #pragma unroll
             for (int i = 0; i < NS; i++) {
-                x0 = fmaf(bf16_low(ks[0][i]) * mul[0], c[i][0] + c[i][1], fmaf(mid(ks[0][i]), qsum[0][i], x0));
-                x1 = fmaf(bf16_low(ks[1][i]) * mul[0], c[i][2] + c[i][3], fmaf(mid(ks[1][i]), qsum[0][i], x1));
+                // Each pair of digits is below 2^23: exact in 32 bits, their sum rounded once.
+                const float d0 = fmaf((float)(hi[i][0] * 128 + hi[i][1]), 16384.0f, (float)(lw[i][0] * 128 + lw[i][1]));
+                const float d1 = fmaf((float)(hi[i][2] * 128 + hi[i][3]), 16384.0f, (float)(lw[i][2] * 128 + lw[i][3]));
+                x0 = fmaf(bf16_low(ks[0][i]) * mul[0], d0, fmaf(mid(ks[0][i]), qsum[0][i], x0));
+                x1 = fmaf(bf16_low(ks[1][i]) * mul[0], d1, fmaf(mid(ks[1][i]), qsum[0][i], x1));
             }
             if (NG < 4 && t >= NG) x0 = x1 = 0.0f;  // head dim 64: two groups for four lanes
 #pragma unroll
@@ -535,9 +585,10 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + ((n * NG + g) * 32 + lane) * 16);
-                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_f16(c, a0, q.x, q.y);
-                    mma_f16(c, a1, q.z, q.w);
+                    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float c[4];
+                    mma_f16(c, a0, q.x, q.y, zero);
+                    mma_f16(c, a1, q.z, q.w, c);
                     s0[n] = fmaf(sc0, c[0] + c[1], s0[n]);
                     s1[n] = fmaf(sc1, c[2] + c[3], s1[n]);
                     b0[n] = fmaf(mid0, qsum[n][g], b0[n]);
@@ -575,30 +626,15 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
 #pragma unroll
                 for (int g = 0; g < NS; g++) low[n][g] *= corr[n];
             }
-            float f[2];  // the factors of accumulator rows r and r + 8
-            if constexpr (ONE) {
-                f[0] = f[1] = corr[0];
-            } else {
+            // (A lane's columns are its own heads'.)
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int h = min((r + 8 * i) / PARTS, HEADS - 1);
-                    f[i] = __shfl_sync(ALL, corr[0], h & 3);
-                    if constexpr (NT == 2) {
-                        const float other = __shfl_sync(ALL, corr[NT - 1], h & 3);
-                        if (h >= 4) f[i] = other;
-                    }
-                }
-            }
+            for (int i = 0; i < 2 * NG; i++)
 #pragma unroll
-            for (int i = 0; i < 4 * NG; i++) {
-                acc[i][0] *= f[0];
-                acc[i][1] *= f[0];
-                acc[i][2] *= f[1];
-                acc[i][3] *= f[1];
-            }
+                for (int n = 0; n < C::NC; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) acc[i][n][c] *= corr[NT == 2 ? n : 0];
         }
-        // Weights times the values' scales, in bfloat16 parts, to the warp's tile: row head * PARTS
-        // + part, slots 2 r and 2 r + 1 for keys r and r + 8.
+        // Weights times the values' scales, in bfloat16 parts, to the warp's tiles.
         uint32_t vs[2][NS];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -626,12 +662,12 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
                 const uint32_t z0 = vs[0][g], z1 = vs[1][g];
                 low[n][g] = fmaf(p0, mid(z0), fmaf(p1, mid(z1), low[n][g]));
                 float w0 = p0 * bf16_low(z0), w1 = p1 * bf16_low(z1);
-                const int own = ONE ? t + 4 * g : g, row = ONE ? 0 : (n * 4 + t) * PARTS;
+                const int own = ONE ? t + 4 * g : g;
                 if (own < NG) {
 #pragma unroll
                     for (int part = 0; part < PARTS; part++) {
                         const uint32_t w = pack_bf16(w0, w1);
-                        *reinterpret_cast<uint32_t *>(wt + (own * C::ROWS + row + part) * C::ROW_BYTES + 4 * r) = w;
+                        *reinterpret_cast<uint32_t *>(wt + own * C::W_GROUP + C::column(ONE ? 0 : n * 4 + t, part) * 32 + wt_put) = w;
                         w0 -= bf16_low(w);
                         w1 -= bf16_high(w);
                     }
@@ -640,17 +676,24 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
         }
         uint32_t vc[2][NG];
 #pragma unroll
-        for (int i = 0; i < 2; i++) read_words<NG>(cur + voff + i * 4 * 8 * 4 * NG, vc[i]);
+        for (int i = 0; i < 2; i++) read_words<NG>(cur + voff + i * 32 * 4 * NG, vc[i]);
         __syncwarp();
         // Every lane holds its part of the block: the stage takes the block STAGES further on.
         if (v + C::STAGES * WARPS < v1) fetch(stage);
         if (++stage == C::STAGES) stage = 0, parity ^= 1u;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            uint32_t w[4];
-            ldmatrix4(w, wt_addr + g * C::ROWS * C::ROW_BYTES);
+            // (Columns without a part are read as they come: what they give is never looked at.)
+            uint2 w[C::NC];
 #pragma unroll
-            for (int i = 0; i < 4; i++) mma_bf16(acc[g * 4 + i], w, codes_bf16(vc[0][g], i), codes_bf16(vc[1][g], i));
+            for (int n = 0; n < C::NC; n++) w[n] = *reinterpret_cast<const uint2 *>(wt + g * C::W_GROUP + n * 256 + wt_get);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const uint32_t y[4] = {codes_bf16(vc[0][g], 2 * j), codes_bf16(vc[0][g], 2 * j + 1), codes_bf16(vc[1][g], 2 * j),
+                                       codes_bf16(vc[1][g], 2 * j + 1)};
+#pragma unroll
+                for (int n = 0; n < C::NC; n++) mma_bf16(acc[2 * g + j][n], y, w[n].x, w[n].y);
+            }
         }
     }
     if (v < v1) {
@@ -685,14 +728,16 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
     }
     __syncthreads();
     if (*abort) return;  // the row is left unwritten; the device status tells
-    float *sacc = reinterpret_cast<float *>(smem) + warp * C::ROWS * D;
+    float *sacc = reinterpret_cast<float *>(smem) + warp * C::ACC_COLS * D;
 #pragma unroll
-    for (int i = 0; i < 4 * NG; i++)
+    for (int i = 0; i < 2 * NG; i++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int row = r + 8 * (c >> 1), ch = (i / 4) * 32 + (2 * t + (c & 1)) * 4 + (i & 3);
-            if (row < C::ROWS) sacc[row * D + ch] = acc[i][c];
-        }
+        for (int n = 0; n < C::NC; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int col = n * 8 + 2 * t + (c & 1), ch = (i / 2) * 32 + 4 * r + 2 * (i & 1) + (c >> 1);
+                if (col < C::ACC_COLS) sacc[col * D + ch] = acc[i][n][c];
+            }
     __syncthreads();
     for (int i = threadIdx.x; i < nh * D; i += WARPS * 32) {
         const int h = i / D, d = i % D;
@@ -705,7 +750,7 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4
             float x = s_low[w][h][d / 32];
 #pragma unroll
             for (int part = 0; part < PARTS; part++)
-                x += reinterpret_cast<const float *>(smem)[(w * C::ROWS + h * PARTS + part) * D + d];
+                x += reinterpret_cast<const float *>(smem)[(w * C::ACC_COLS + C::column(h, part)) * D + d];
             sum = fmaf(s_l[w][h], f, sum);
             o = fmaf(x, f, o);
         }
@@ -728,8 +773,10 @@ int launch_attention(const Cache4Args &a, const SplitRows &rows, cudaStream_t st
 }
 
 // Heads of one key/value head that a CTA takes: a single one has its own kernel; otherwise 4, or 8 where
-// the parts of 8 heads' weights fit the product's 16 rows (two parts: 16-bit queries).
-int heads_per_cta(int64_t group, int dtype) { return group == 1 ? 1 : (dtype != DC_F32 && group > 4 ? 8 : 4); }
+// the weights take two parts (16-bit queries: two tiles of columns, as three parts of four heads).
+int heads_per_cta(int64_t group, int dtype) {
+    return group == 1 ? 1 : (dtype != DC_F32 && group > 4 ? 8 : 4);
+}
 
 template <int D>
 int launch_dim(const Cache4Args &a, const SplitRows &rows, cudaStream_t stream) {

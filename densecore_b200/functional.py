@@ -181,7 +181,7 @@ def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.
 
 
 def _whole_number(name, value, least=None):
-    if isinstance(value, (bool, np.bool_)) or not isinstance(value, numbers.Integral):
+    if type(value) is not int and (isinstance(value, (bool, np.bool_)) or not isinstance(value, numbers.Integral)):
         raise TypeError(f"{name} must be a whole number")
     if least is not None and value < least:
         raise ValueError(f"{name} must be at least {least}")
@@ -258,7 +258,7 @@ def sliding_window_attention(query, key, value, window, sinks=0, attn_mask=None,
             raise NotImplementedError("sliding window attention with lengths has no gradient")
         out = _SlidingWindow.apply(q, k, v, window, sinks, offset, float(scale), mask)
     else:
-        out, _lse = _native._sliding_window(q, k, v, window, sinks, offset, float(scale), mask, lengths)
+        out, _lse = _native._sliding_window(q, k, v, window, sinks, offset, float(scale), mask, lengths, need_lse=False)
     return out.squeeze(1) if rank == 3 else out
 
 
@@ -319,7 +319,7 @@ def _rotary_args(what, query, key, positions, inv_freq, interleaved, amplitude):
         raise TypeError("inv_freq must be a float64 Tensor")
     if type(interleaved) is not bool:
         raise TypeError("interleaved must be a bool")
-    if isinstance(amplitude, (bool, np.bool_)) or not isinstance(amplitude, numbers.Real):
+    if type(amplitude) is not float and (isinstance(amplitude, (bool, np.bool_)) or not isinstance(amplitude, numbers.Real)):
         raise TypeError("amplitude must be real")
     if query.dim() == 3:
         return query.unsqueeze(1), None if key is None else key.unsqueeze(1)
@@ -392,7 +392,7 @@ def qk_norm_rotary(query, key, query_weight, key_weight, positions, inv_freq, *,
             raise ValueError(f"norm weights must be ({query.shape[-1]},), got {tuple(w.shape)}")
     if key is None and key_weight is not None:
         raise ValueError("a key weight needs a key")
-    if isinstance(eps, (bool, np.bool_)) or not isinstance(eps, numbers.Real):
+    if type(eps) is not float and (isinstance(eps, (bool, np.bool_)) or not isinstance(eps, numbers.Real)):
         raise TypeError("eps must be real")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
