@@ -114,32 +114,67 @@ __device__ __forceinline__ Place place_of(const Cache4Args &a, int64_t b, int64_
     return {nullptr, 0};
 }
 
-// Filling and reading back are bound by HBM. A block takes a run of tokens of one (sequence, head) of
-// the keys or the values (grid: token runs, 2 Hkv, B); a thread four channels of ROWS tokens, whose
-// loads are issued together; eight neighbours make a group of 32.
+// Filling and reading back are bound by HBM and, close behind, by the arithmetic on each value. A block
+// takes a run of tokens of one (sequence, head) of the keys or the values (grid: token runs, 2 Hkv, B); a
+// thread four channels of ROWS tokens, whose loads are issued together; eight neighbours make a group of
+// 32. The tokens' places (a division by the page size, a look into the table) are found once a block.
 constexpr int ROWS = 4;
 
-// rint(d / scale) of the correctly rounded quotient, by a product with the reciprocal where that
-// cannot round the other way (the product is off by less than 1e-5 for quotients up to 15).
-__device__ __forceinline__ float code_of(float d, float scale, float inv) {
+// The places of the block's tokens t0 .. (at most 64), those from `last` on null.
+__device__ __forceinline__ void block_places(const Cache4Args &a, int64_t b, int64_t pos0, int64_t t0, int64_t last, int run, int which,
+                                             int head, Place *places) {
+    if ((int)threadIdx.x < run) {
+        const int64_t t = t0 + threadIdx.x;
+        places[threadIdx.x] = t < last ? place_of(a, b, pos0 + t, which, head) : Place{nullptr, 0};
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// x / 15, correctly rounded, then up to bfloat16 (x >= 0), as bits. The product with 1/15 is off by less
+// than two units in the last place, which matters only where those cross a bfloat16: there, and where it
+// is not a normal number, the division is done.
+__device__ __forceinline__ uint32_t fifteenth_up(float x) {
+    uint32_t w = __float_as_uint(x * (1.0f / 15.0f));
+    if (((w + 4u) & 0xFFFFu) <= 8u || w < 0x01000000u || w > 0x7E000000u) w = __float_as_uint(__fdiv_rn(x, 15.0f));
+    return (w + 0xFFFFu) & 0xFFFF0000u;
+}
+
+// The code of x = d above low: the correctly rounded d / scale to the nearest whole number (ties to
+// even), by a product with the reciprocal (off by less than 1e-5 for quotients up to 15) where that
+// cannot round the other way. inv NaN: divide.
+__device__ __forceinline__ uint32_t code_of(float d, float scale, float inv) {
+    constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the rounded number
     const float q = d * inv;
-    float c = rintf(q);
-    if (!(fabsf(q - c) < 0.4999f)) c = rintf(__fdiv_rn(d, scale));
-    return fminf(fmaxf(c, 0.0f), 15.0f);
+    float m = q + MAGIC;
+    if (!(fabsf(q - (m - MAGIC)) < 0.4999f)) m = __fdiv_rn(d, scale) + MAGIC;
+    return __float_as_uint(m) & 15u;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Args a, bool vec) {
+    __shared__ Place places[256 / 16 * ROWS];
     const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
     const int64_t b = blockIdx.z;
-    const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes;
-    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS) + threadIdx.x / lanes, start = a.starts[b * a.starts_stride];
+    const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes, row0 = threadIdx.x / lanes;
+    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), start = a.starts[b * a.starts_stride];
     const int64_t last = min(a.T, a.ends ? a.ends[b * a.ends_stride] - start : a.T);  // tokens from here on stay out
+    if (t0 >= last) return;
     const T *src = static_cast<const T *>(a.x[which]) + b * a.xs[which][0] + head * a.xs[which][1] + (int64_t)(4 * quad) * a.xs[which][3];
     float x[ROWS][4];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int64_t t = t0 + i * pass;
+        const int64_t t = t0 + row0 + i * pass;
         if (t < last) {
             load4(src + t * a.xs[which][2], a.xs[which][3], vec, x[i]);
         } else {
@@ -147,39 +182,33 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Args a, 
             for (int e = 0; e < 4; e++) x[i][e] = 0.0f;
         }
     }
+    block_places(a, b, start, t0, last, pass * ROWS, which, head, places);
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int64_t t = t0 + i * pass;
         float mn = fminf(fminf(x[i][0], x[i][1]), fminf(x[i][2], x[i][3]));
-        float mx = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < 4; e++) finite = finite && fabsf(x[i][e]) <= 3.402823466e38f;
-        if (!finite) mx = INFINITY;
+        float mx = max_nan(max_nan(x[i][0], x[i][1]), max_nan(x[i][2], x[i][3]));
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) {
             mn = fminf(mn, __shfl_xor_sync(ALL, mn, o));
-            mx = fmaxf(mx, __shfl_xor_sync(ALL, mx, o));
+            mx = max_nan(mx, __shfl_xor_sync(ALL, mx, o));
         }
-        if (t >= last) continue;
+        const Place at = places[row0 + i * pass];
+        if (!at.half) continue;
         // low: bits below bfloat16 cut, one step further down for a negative value that had some.
         uint32_t lb = __float_as_uint(mn);
         if ((lb >> 31) && (lb & 0xFFFFu)) lb += 0x10000u;
         lb &= 0xFFFF0000u;
-        const float low = __uint_as_float(lb);
-        const float width = __fdiv_rn(__fsub_rn(mx, low), 15.0f);
-        uint32_t sb = (__float_as_uint(width) + 0xFFFFu) & 0xFFFF0000u;  // up to bfloat16 (width >= 0)
-        uint32_t codes = 0;
-        if (!(fabsf(low) <= 3.402823466e38f) || !(width <= 3.3e38f)) {
+        const float low = __uint_as_float(lb), width = __fsub_rn(mx, low);
+        uint32_t sb = 0, codes = 0;
+        if (!(width <= 3.402823466e38f)) {  // an infinity or a NaN among the values, or their range overflows
             lb = sb = 0x7FC00000u;  // NaN
-        } else if (sb) {
+        } else if (width > 0.0f) {
+            sb = fifteenth_up(width);
             const float scale = __uint_as_float(sb);
-            const float inv = scale > 1e-37f && scale < 1e37f ? __frcp_rn(scale) : NAN;  // NaN: divide
+            const float inv = scale > 1e-37f && scale < 1e37f ? rcp_fast(scale) : NAN;  // NaN: divide
 #pragma unroll
-            for (int e = 0; e < 4; e++) codes |= (uint32_t)code_of(__fsub_rn(x[i][e], low), scale, inv) << (4 * e);
+            for (int e = 0; e < 4; e++) codes |= code_of(__fsub_rn(x[i][e], low), scale, inv) << (4 * e);
         }
-        const Place at = place_of(a, b, start + t, which, head);
-        if (!at.half) continue;
         reinterpret_cast<uint16_t *>(at.half)[code_at(which, at.slot, r, g, ng)] = (uint16_t)codes;
         if (r == 0) reinterpret_cast<uint32_t *>(at.half + 8 * a.c.D)[at.slot * ng + g] = (sb >> 16) | lb;
     }
@@ -187,36 +216,39 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Args a, 
 
 // Token t of sequence b from the cache, in float32; zeros from the sequence's length on.
 __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bool vec) {
+    __shared__ Place places[256 / 16 * ROWS];
     const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
     const int64_t b = blockIdx.z;
-    const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes;
-    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS) + threadIdx.x / lanes, len = a.lens[b * a.lens_stride];
+    const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes, row0 = threadIdx.x / lanes;
+    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), len = a.lens[b * a.lens_stride];
+    block_places(a, b, 0, t0, min(a.T, len), pass * ROWS, which, head, places);
     uint32_t codes[ROWS], sl[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int64_t t = t0 + i * pass;
+        const Place at = places[row0 + i * pass];
         codes[i] = sl[i] = 0u;  // a zero
-        if (t < a.T && t < len) {
-            const Place at = place_of(a, b, t, which, head);
-            if (at.half) {
-                codes[i] = reinterpret_cast<const uint16_t *>(at.half)[code_at(which, at.slot, r, g, ng)];
-                sl[i] = reinterpret_cast<const uint32_t *>(at.half + 8 * a.c.D)[at.slot * ng + g];
-            }
+        if (at.half) {
+            codes[i] = reinterpret_cast<const uint16_t *>(at.half)[code_at(which, at.slot, r, g, ng)];
+            sl[i] = reinterpret_cast<const uint32_t *>(at.half + 8 * a.c.D)[at.slot * ng + g];
         }
     }
+    float *dst = a.y[which] + b * a.ys[which][0] + head * a.ys[which][1] + (int64_t)(4 * quad) * a.ys[which][3];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int64_t t = t0 + i * pass;
+        const int64_t t = t0 + row0 + i * pass;
         if (t >= a.T) continue;
         const float scale = bf16_low(sl[i]), low = bf16_high(sl[i]);
-        const float4 y = make_float4(fmaf(scale, (float)(codes[i] & 15u), low), fmaf(scale, (float)((codes[i] >> 4) & 15u), low),
-                                     fmaf(scale, (float)((codes[i] >> 8) & 15u), low), fmaf(scale, (float)(codes[i] >> 12), low));
-        float *dst = a.y[which] + b * a.ys[which][0] + head * a.ys[which][1] + t * a.ys[which][2] + (int64_t)(4 * quad) * a.ys[which][3];
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)  // 2^23 + code, less 2^23: the code, without the conversion unit
+            y[e] = fmaf(scale, __uint_as_float(((codes[i] >> (4 * e)) & 15u) | 0x4B000000u) - 8388608.0f, low);
+        float *row = dst + t * a.ys[which][2];
         if (vec) {
-            *reinterpret_cast<float4 *>(dst) = y;
+            *reinterpret_cast<float4 *>(row) = make_float4(y[0], y[1], y[2], y[3]);
         } else {
-            const int64_t s = a.ys[which][3];
-            dst[0] = y.x, dst[s] = y.y, dst[2 * s] = y.z, dst[3 * s] = y.w;
+            const int64_t st = a.ys[which][3];
+#pragma unroll
+            for (int e = 0; e < 4; e++) row[e * st] = y[e];
         }
     }
 }

@@ -79,10 +79,20 @@ struct Piece {
             w[0] = v.x, w[1] = v.y;
         }
     }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) w[i] = 0u;
+    }
     __device__ __forceinline__ float at(int i) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
         else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i & 1)))));
         else return __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+    }
+    // Values of a unit (this piece, then `next`) by twos.
+    __device__ __forceinline__ float2 two(const Piece &next, int i) const {
+        if constexpr (V == 1) return make_float2(at(0), next.at(0));
+        const Piece &p = i < 2 ? *this : next;
+        return make_float2(p.at(2 * (i & 1)), p.at(2 * (i & 1) + 1));
     }
 };
 
@@ -97,11 +107,24 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void store(T *row, int at, int64_t inner, const float *f) {
-    if constexpr (V == 1) row[at * inner] = from_f<T>(f[0]);
-    else if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(row + at) = make_float4(f[0], f[1], f[2], f[3]);
-    else *reinterpret_cast<uint2 *>(row + at) = make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]));
+template <typename T>
+__device__ __forceinline__ void store4(T *p, float2 a, float2 b) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(p) = make_float4(a.x, a.y, b.x, b.y);
+    else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y));
+}
+
+// Two products (and sums) in one instruction, each rounded as alone.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(r))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
+    return r;
 }
 
 __device__ __forceinline__ float weight_at(const RotaryOperand &o, int at) {
@@ -149,14 +172,14 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
             e1[u] = e0[u] + V;
         }
     }
-    float gw[2][NG][2 * V];
+    float2 gw[2][NG][V];
     if constexpr (MODE == NORM_BWD) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
 #pragma unroll
             for (int u = 0; u < UPL; u++)
 #pragma unroll
-                for (int i = 0; i < 2 * V; i++) gw[k][u][i] = 0.0f;
+                for (int i = 0; i < V; i++) gw[k][u][i] = make_float2(0.0f, 0.0f);
     }
     // The weights, in 32 bits, for every item of the block.
     __shared__ __align__(16) float s_w[2][MODE == ROTATE ? 4 : 2 * MAX_PAIRS];
@@ -201,28 +224,41 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
                 cs[u][i] = turns[u] ? s_cos[warp][pair] : 1.0f;
                 sn[u][i] = turns[u] ? s_sin[warp][pair] : 0.0f;
             }
-        // Rows h0 .. h1 - 1 of operand K.
+        // Rows h0 .. h1 - 1 of operand K. Values go in twos (P to a unit): (0, 1), (2, 3) of each piece, or, with
+        // single elements, the unit's two.
+        constexpr int P = V;
         auto rows = [&](auto operand, int h0, int h1) {
             constexpr int K = decltype(operand)::value;
             if (h0 >= h1) return;
             const RotaryOperand &o = a.op[K];
-            float w[NW][2 * V];
+            float2 w[NW][P];
             if constexpr (MODE != ROTATE) {
 #pragma unroll
                 for (int u = 0; u < UPL; u++)
 #pragma unroll
-                    for (int i = 0; i < 2 * V; i++) w[u][i] = has[u] ? s_w[K][(i < V ? e0[u] : e1[u]) + i % V] : 0.0f;
+                    for (int i = 0; i < P; i++) {
+                        w[u][i] = make_float2(0.0f, 0.0f);
+                        if (has[u]) w[u][i] = V == 1 ? make_float2(s_w[K][e0[u]], s_w[K][e1[u]])
+                                                     : *reinterpret_cast<const float2 *>(&s_w[K][(i < 2 ? e0[u] : e1[u]) + 2 * (i & 1)]);
+                    }
             }
             const T *xb = static_cast<const T *>(o.x) + b * o.xs[0] + l * o.xs[2];
             const T *gb = MODE == NORM_BWD ? static_cast<const T *>(o.g) + b * o.gs[0] + l * o.gs[2] : nullptr;
             T *yb = static_cast<T *>(o.y) + b * o.ys[0] + l * o.ys[2];
             for (int hb = h0; hb < h1; hb += rpw * R) {
+                // (Rows past the run and lanes past the row hold zeros.)
                 Piece<T, V> x[R][UPL][2], g[MODE == NORM_BWD ? R : 1][UPL][2];
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     const int h = hb + r * rpw + sub;
 #pragma unroll
-                    for (int u = 0; u < UPL; u++)
+                    for (int u = 0; u < UPL; u++) {
+                        x[r][u][0].zero();
+                        x[r][u][1].zero();
+                        if constexpr (MODE == NORM_BWD) {
+                            g[r][u][0].zero();
+                            g[r][u][1].zero();
+                        }
                         if (h < h1 && has[u]) {
                             const T *row = xb + h * o.xs[1];
                             x[r][u][0].load(row, e0[u], o.xs[3]);
@@ -233,75 +269,87 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
                                 g[r][u][1].load(gr, e1[u], o.gs[3]);
                             }
                         }
+                    }
                 }
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     const int h = hb + r * rpw + sub;
                     const bool live = h < h1;
-                    float f[UPL][2 * V], v[NG][2 * V];
-                    float ss = 0.0f;
+                    float2 f[UPL][P], v[NG][P];
+                    float2 ss = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int u = 0; u < UPL; u++)
 #pragma unroll
-                        for (int i = 0; i < 2 * V; i++) {
-                            const bool in = live && has[u];
-                            f[u][i] = in ? x[r][u][i / V].at(i % V) : 0.0f;
-                            if constexpr (MODE != ROTATE) ss = fmaf(f[u][i], f[u][i], ss);
-                            if constexpr (MODE == NORM_BWD) v[u][i] = in ? g[r][u][i / V].at(i % V) : 0.0f;
+                        for (int i = 0; i < P; i++) {
+                            f[u][i] = x[r][u][0].two(x[r][u][1], i);
+                            if constexpr (MODE != ROTATE) ss = fma2(f[u][i], f[u][i], ss);
+                            if constexpr (MODE == NORM_BWD) v[u][i] = g[r][u][0].two(g[r][u][1], i);
                         }
-                    float rinv = 1.0f;
+                    float2 rinv = make_float2(1.0f, 1.0f);
                     if constexpr (MODE != ROTATE) {
-                        for (int s = lpr >> 1; s > 0; s >>= 1) ss += __shfl_xor_sync(ALL, ss, s);
-                        rinv = 1.0f / sqrtf(ss * a.inv_D + a.eps);
+                        float sum = ss.x + ss.y;
+                        for (int m = lpr >> 1; m > 0; m >>= 1) sum += __shfl_xor_sync(ALL, sum, m);
+                        rinv.x = rinv.y = live ? rsqrtf(fmaf(sum, a.inv_D, a.eps)) : 0.0f;
                     }
                     if constexpr (MODE == NORM) {
 #pragma unroll
                         for (int u = 0; u < UPL; u++)
 #pragma unroll
-                            for (int i = 0; i < 2 * V; i++) f[u][i] = f[u][i] * rinv * w[u][i];
+                            for (int i = 0; i < P; i++) f[u][i] = mul2(mul2(f[u][i], rinv), w[u][i]);
                     }
                     // The rotation: of the row, or (backward) transposed, of the gradient. Channels that
                     // pass through are left alone, not multiplied by 1: an infinity beside them would
                     // come back as NaN.
 #pragma unroll
                     for (int u = 0; u < UPL; u++) {
-                        float *z = MODE == NORM_BWD ? v[MODE == NORM_BWD ? u : 0] : f[u];
+                        float2 *z = MODE == NORM_BWD ? v[MODE == NORM_BWD ? u : 0] : f[u];
                         if (turns[u]) {
+                            if constexpr (V == 1 || INTER) {  // a pair in each two
 #pragma unroll
-                            for (int i = 0; i < V; i++) {
-                                const int ia = INTER ? 2 * i : i, ib = INTER ? 2 * i + 1 : V + i;
-                                const float za = z[ia], zb = z[ib];
-                                z[ia] = fmaf(za, cs[u][i], -zb * sn[u][i]);
-                                z[ib] = fmaf(zb, cs[u][i], za * sn[u][i]);
+                                for (int i = 0; i < P; i++)
+                                    z[i] = make_float2(fmaf(z[i].x, cs[u][i], -z[i].y * sn[u][i]), fmaf(z[i].y, cs[u][i], z[i].x * sn[u][i]));
+                            } else {  // the first and second members of two pairs in z[i] and z[2 + i]
+#pragma unroll
+                                for (int i = 0; i < 2; i++) {
+                                    const float2 c = make_float2(cs[u][2 * i], cs[u][2 * i + 1]), s = make_float2(sn[u][2 * i], sn[u][2 * i + 1]);
+                                    const float2 ns = make_float2(-s.x, -s.y), za = z[i], zb = z[(2 + i) % P];
+                                    z[i] = fma2(za, c, mul2(zb, ns));
+                                    z[(2 + i) % P] = fma2(zb, c, mul2(za, s));
+                                }
                             }
                         }
                     }
                     if constexpr (MODE == NORM_BWD) {
-                        float dot = 0.0f;
+                        float2 dots = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int u = 0; u < UPL; u++)
 #pragma unroll
-                            for (int i = 0; i < 2 * V; i++) {
-                                const float n = f[u][i] * rinv;
-                                gw[K][u][i] = fmaf(v[u][i], n, gw[K][u][i]);
-                                f[u][i] = n;
-                                v[u][i] *= w[u][i];
-                                dot = fmaf(v[u][i], n, dot);
+                            for (int i = 0; i < P; i++) {
+                                f[u][i] = mul2(f[u][i], rinv);
+                                gw[K][u][i] = fma2(v[u][i], f[u][i], gw[K][u][i]);
+                                v[u][i] = mul2(v[u][i], w[u][i]);
+                                dots = fma2(v[u][i], f[u][i], dots);
                             }
-                        for (int s = lpr >> 1; s > 0; s >>= 1) dot += __shfl_xor_sync(ALL, dot, s);
-                        dot *= a.inv_D;
+                        float dot = dots.x + dots.y;
+                        for (int m = lpr >> 1; m > 0; m >>= 1) dot += __shfl_xor_sync(ALL, dot, m);
+                        dot *= -a.inv_D;
 #pragma unroll
                         for (int u = 0; u < UPL; u++)
 #pragma unroll
-                            for (int i = 0; i < 2 * V; i++) f[u][i] = rinv * fmaf(-f[u][i], dot, v[u][i]);
+                            for (int i = 0; i < P; i++) f[u][i] = mul2(rinv, fma2(f[u][i], make_float2(dot, dot), v[u][i]));
                     }
                     if (live) {
                         T *row = yb + h * o.ys[1];
 #pragma unroll
                         for (int u = 0; u < UPL; u++)
                             if (has[u]) {
-                                store<T, V>(row, e0[u], o.ys[3], f[u]);
-                                store<T, V>(row, e1[u], o.ys[3], f[u] + V);
+                                if constexpr (V == 1) {
+                                    row[e0[u] * o.ys[3]] = from_f<T>(f[u][0].x);
+                                    row[e1[u] * o.ys[3]] = from_f<T>(f[u][0].y);
+                                } else {
+                                    store4(row + e0[u], f[u][0], f[u][1 % P]);
+                                    store4(row + e1[u], f[u][2 % P], f[u][3 % P]);
+                                }
                             }
                     }
                 }
@@ -321,7 +369,7 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
             for (int u = 0; u < UPL; u++)
 #pragma unroll
                 for (int i = 0; i < 2 * V; i++) {
-                    float s = gw[k][u][i];
+                    float s = i & 1 ? gw[k][u][i / 2].y : gw[k][u][i / 2].x;
                     for (int m = lpr; m < 32; m <<= 1) s += __shfl_xor_sync(ALL, s, m);
                     if (has[u] && sub == 0) part[warp][(i < V ? e0[u] : e1[u]) + i % V] = s;
                 }
