@@ -66,22 +66,27 @@ struct Piece {
     static constexpr int WORDS = V == 1 ? 1 : V * (int)sizeof(T) / 4;
     uint32_t w[WORDS];
 
-    // V == 1 reads at any element stride; pieces of four elements lie on a boundary of their size.
-    __device__ __forceinline__ void load(const T *row, int at, int64_t inner) {
+    // The piece at p, zeros where it is not `there`. (Predicated: as branches the loads of a row cost more
+    // instructions than its arithmetic.)
+    __device__ __forceinline__ void load(const T *p, bool there) {
         if constexpr (V == 1) {
-            if constexpr (sizeof(T) == 4) w[0] = __float_as_uint(row[at * inner]);
-            else w[0] = reinterpret_cast<const uint16_t *>(row)[at * inner];
+            w[0] = 0u;
+            if (there) {
+                if constexpr (sizeof(T) == 4) w[0] = __float_as_uint(*p);
+                else w[0] = *reinterpret_cast<const uint16_t *>(p);
+            }
         } else if constexpr (WORDS == 4) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(row + at);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                         "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+                         : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3])
+                         : "l"(p), "r"((int)there)
+                         : "memory");
         } else {
-            const uint2 v = *reinterpret_cast<const uint2 *>(row + at);
-            w[0] = v.x, w[1] = v.y;
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@p ld.global.v2.b32 {%0, %1}, [%2];\n\t}"
+                         : "=&r"(w[0]), "=&r"(w[1])
+                         : "l"(p), "r"((int)there)
+                         : "memory");
         }
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < WORDS; i++) w[i] = 0u;
     }
     __device__ __forceinline__ float at(int i) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
@@ -108,9 +113,25 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T *p, float2 a, float2 b) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(p) = make_float4(a.x, a.y, b.x, b.y);
-    else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y));
+__device__ __forceinline__ void store4(T *p, float2 a, float2 b, bool there) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p st.global.v4.f32 [%0], {%1, %2, %3, %4};\n\t}" ::"l"(p), "f"(a.x), "f"(a.y),
+                     "f"(b.x), "f"(b.y), "r"((int)there)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p st.global.v2.b32 [%0], {%1, %2};\n\t}" ::"l"(p), "r"(pack2<T>(a.x, a.y)),
+                     "r"(pack2<T>(b.x, b.y)), "r"((int)there)
+                     : "memory");
+}
+
+// The sum over a row's lanes (1 << k of them; unrolled and predicated, not a loop over k).
+__device__ __forceinline__ float row_sum(float s, int lpr) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        const float other = __shfl_xor_sync(ALL, s, m);
+        if (m < lpr) s += other;
+    }
+    return s;
 }
 
 // Two products (and sums) in one instruction, each rounded as alone.
@@ -172,6 +193,7 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
             e1[u] = e0[u] + V;
         }
     }
+    const bool all_turn = a.rot == a.D;  // no channel passes through
     float2 gw[2][NG][V];
     if constexpr (MODE == NORM_BWD) {
 #pragma unroll
@@ -242,39 +264,33 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
                                                      : *reinterpret_cast<const float2 *>(&s_w[K][(i < 2 ? e0[u] : e1[u]) + 2 * (i & 1)]);
                     }
             }
-            const T *xb = static_cast<const T *>(o.x) + b * o.xs[0] + l * o.xs[2];
-            const T *gb = MODE == NORM_BWD ? static_cast<const T *>(o.g) + b * o.gs[0] + l * o.gs[2] : nullptr;
-            T *yb = static_cast<T *>(o.y) + b * o.ys[0] + l * o.ys[2];
+            // This lane's first row, and from one of its rows to the next; its pieces within a row.
+            const T *xr = static_cast<const T *>(o.x) + b * o.xs[0] + l * o.xs[2] + (h0 + sub) * o.xs[1];
+            const T *gr = MODE == NORM_BWD ? static_cast<const T *>(o.g) + b * o.gs[0] + l * o.gs[2] + (h0 + sub) * o.gs[1] : nullptr;
+            T *yr = static_cast<T *>(o.y) + b * o.ys[0] + l * o.ys[2] + (h0 + sub) * o.ys[1];
+            const int64_t x_step = rpw * o.xs[1], g_step = rpw * o.gs[1], y_step = rpw * o.ys[1];
+            const int64_t xi = V == 1 ? o.xs[3] : 1, gi = V == 1 ? o.gs[3] : 1, yi = V == 1 ? o.ys[3] : 1;
             for (int hb = h0; hb < h1; hb += rpw * R) {
                 // (Rows past the run and lanes past the row hold zeros.)
                 Piece<T, V> x[R][UPL][2], g[MODE == NORM_BWD ? R : 1][UPL][2];
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    const int h = hb + r * rpw + sub;
+                    const bool live = hb + r * rpw + sub < h1;
 #pragma unroll
                     for (int u = 0; u < UPL; u++) {
-                        x[r][u][0].zero();
-                        x[r][u][1].zero();
+                        x[r][u][0].load(xr + e0[u] * xi, live && has[u]);
+                        x[r][u][1].load(xr + e1[u] * xi, live && has[u]);
                         if constexpr (MODE == NORM_BWD) {
-                            g[r][u][0].zero();
-                            g[r][u][1].zero();
-                        }
-                        if (h < h1 && has[u]) {
-                            const T *row = xb + h * o.xs[1];
-                            x[r][u][0].load(row, e0[u], o.xs[3]);
-                            x[r][u][1].load(row, e1[u], o.xs[3]);
-                            if constexpr (MODE == NORM_BWD) {
-                                const T *gr = gb + h * o.gs[1];
-                                g[r][u][0].load(gr, e0[u], o.gs[3]);
-                                g[r][u][1].load(gr, e1[u], o.gs[3]);
-                            }
+                            g[r][u][0].load(gr + e0[u] * gi, live && has[u]);
+                            g[r][u][1].load(gr + e1[u] * gi, live && has[u]);
                         }
                     }
+                    xr += x_step;
+                    if (MODE == NORM_BWD) gr += g_step;
                 }
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    const int h = hb + r * rpw + sub;
-                    const bool live = h < h1;
+                    const bool live = hb + r * rpw + sub < h1;
                     float2 f[UPL][P], v[NG][P];
                     float2 ss = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -287,8 +303,7 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
                         }
                     float2 rinv = make_float2(1.0f, 1.0f);
                     if constexpr (MODE != ROTATE) {
-                        float sum = ss.x + ss.y;
-                        for (int m = lpr >> 1; m > 0; m >>= 1) sum += __shfl_xor_sync(ALL, sum, m);
+                        const float sum = row_sum(ss.x + ss.y, lpr);
                         rinv.x = rinv.y = live ? rsqrtf(fmaf(sum, a.inv_D, a.eps)) : 0.0f;
                     }
                     if constexpr (MODE == NORM) {
@@ -303,7 +318,7 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
 #pragma unroll
                     for (int u = 0; u < UPL; u++) {
                         float2 *z = MODE == NORM_BWD ? v[MODE == NORM_BWD ? u : 0] : f[u];
-                        if (turns[u]) {
+                        if (all_turn || turns[u]) {
                             if constexpr (V == 1 || INTER) {  // a pair in each two
 #pragma unroll
                                 for (int i = 0; i < P; i++)
@@ -330,28 +345,26 @@ __global__ void __launch_bounds__(WPB * 32, MODE == NORM_BWD ? 2 : 3) rotary_ker
                                 v[u][i] = mul2(v[u][i], w[u][i]);
                                 dots = fma2(v[u][i], f[u][i], dots);
                             }
-                        float dot = dots.x + dots.y;
-                        for (int m = lpr >> 1; m > 0; m >>= 1) dot += __shfl_xor_sync(ALL, dot, m);
-                        dot *= -a.inv_D;
+                        const float dot = row_sum(dots.x + dots.y, lpr) * -a.inv_D;
 #pragma unroll
                         for (int u = 0; u < UPL; u++)
 #pragma unroll
                             for (int i = 0; i < P; i++) f[u][i] = mul2(rinv, fma2(f[u][i], make_float2(dot, dot), v[u][i]));
                     }
-                    if (live) {
-                        T *row = yb + h * o.ys[1];
 #pragma unroll
-                        for (int u = 0; u < UPL; u++)
-                            if (has[u]) {
-                                if constexpr (V == 1) {
-                                    row[e0[u] * o.ys[3]] = from_f<T>(f[u][0].x);
-                                    row[e1[u] * o.ys[3]] = from_f<T>(f[u][0].y);
-                                } else {
-                                    store4(row + e0[u], f[u][0], f[u][1 % P]);
-                                    store4(row + e1[u], f[u][2 % P], f[u][3 % P]);
-                                }
+                    for (int u = 0; u < UPL; u++) {
+                        const bool there = live && has[u];
+                        if constexpr (V == 1) {
+                            if (there) {
+                                yr[e0[u] * yi] = from_f<T>(f[u][0].x);
+                                yr[e1[u] * yi] = from_f<T>(f[u][0].y);
                             }
+                        } else {
+                            store4(yr + e0[u], f[u][0], f[u][1 % P], there);
+                            store4(yr + e1[u], f[u][2 % P], f[u][3 % P], there);
+                        }
                     }
+                    yr += y_step;
                 }
             }
         };
