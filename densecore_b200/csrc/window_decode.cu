@@ -167,31 +167,49 @@ __global__ void __launch_bounds__(WARPS * 32) window_decode_kernel(const AttnPro
     }
 }
 
-// Joins a row's splits: one warp per row of D channels.
+// Joins a row's splits (at most MAX_SPLITS): a block per row, a thread per split for the factors, then
+// each warp every fourth split's D channels, and the warps' sums in order.
+constexpr int MAX_SPLITS = 128;
+
 __global__ void __launch_bounds__(128) split_combine_kernel(const SplitRows r) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-    const int lane = threadIdx.x & 31;
+    __shared__ float s_f[MAX_SPLITS], s_acc[4][256], s_top[4], s_sum[4];
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     griddep_wait();
-    if (row >= r.rows) return;
     const int64_t stride = r.D + 2;
     const float *src = r.part + row * r.splits * stride;
-    float top = -INFINITY, sum = 0.0f;
-    for (int s = lane; s < r.splits; s += 32) top = fmaxf(top, src[s * stride + r.D]);
+    const bool mine = (int)threadIdx.x < r.splits;
+    const float m = mine ? src[threadIdx.x * stride + r.D] : -INFINITY, l = mine ? src[threadIdx.x * stride + r.D + 1] : 0.0f;
+    float top = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(ALL, top, o));
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    // A split without a key adds its zeros (or the NaN of a NaN score).
+    const float f = m == -INFINITY ? 1.0f : exp2f(m - top);
+    s_f[threadIdx.x] = f;
+    float sum = l * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(ALL, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
     float acc[8] = {};
-    for (int s = 0; s < r.splits; s++) {
+#pragma unroll 4
+    for (int s = warp; s < r.splits; s += 4) {
         const float *part = src + s * stride;
-        const float ms = part[r.D];
-        const float c = ms == -INFINITY ? 1.0f : exp2f(ms - top);
-        sum = fmaf(part[r.D + 1], c, sum);
+        const float fs = s_f[s];
 #pragma unroll
         for (int x = 0; x < 8; x++)
-            if (lane + 32 * x < r.D) acc[x] = fmaf(part[lane + 32 * x], c, acc[x]);
+            if (lane + 32 * x < r.D) acc[x] = fmaf(part[lane + 32 * x], fs, acc[x]);
     }
 #pragma unroll
     for (int x = 0; x < 8; x++)
-        if (lane + 32 * x < r.D) split_finish(r, row, lane + 32 * x, top, sum, acc[x]);
+        if (lane + 32 * x < r.D) s_acc[warp][lane + 32 * x] = acc[x];
+    __syncthreads();
+    for (int d = threadIdx.x; d < r.D; d += 128)
+        split_finish(r, row, d, top, sum, (s_acc[0][d] + s_acc[1][d]) + (s_acc[2][d] + s_acc[3][d]));
 }
 
 bool aligned16(const void *ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
@@ -218,7 +236,7 @@ size_t split_rows_bytes(int64_t rows, int splits, int64_t D) { return splits > 1
 int split_combine(const SplitRows &r, cudaStream_t stream) {
     if (r.splits <= 1 || r.rows == 0) return DC_OK;
     KernelTrace tr("split_combine", stream);
-    const cudaError_t e = launch_dependent(split_combine_kernel, dim3((unsigned)((r.rows + 3) / 4)), dim3(128), 0, stream, r);
+    const cudaError_t e = launch_dependent(split_combine_kernel, dim3((unsigned)r.rows), dim3(128), 0, stream, r);
     return e == cudaSuccess ? DC_OK : cuda_fail(e, "split_combine");
 }
 
@@ -231,12 +249,15 @@ bool window_decode_supported(const AttnProblem &p) {
     return aligned16(p.k) && aligned16(p.v) && p.Hkv * chunks <= 65535;
 }
 
-// Splits of each row: three CTAs of 4 warps on every SM twice over, at least 128 keys each.
+// Splits of each row: three CTAs of 4 warps on every SM twice over, at least 128 keys each, or once over
+// with at least 32 keys each (two steps of the loop: one sequence's 1004 keys over 8 heads in 8 runs of
+// 128 took 14 us, eight steps one after another).
 int window_decode_splits(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t window, int64_t sinks) {
     const int64_t group = H / Hkv, chunks = group <= 2 ? 1 : (group + 3) / 4;
     const int64_t ctas = std::max<int64_t>(1, B * Hkv * chunks), keys = std::min(S, std::min(window, S) + std::min(sinks, S));
-    const int64_t fill = (int64_t)device_sm_count() * 6 / ctas, most = (keys + 127) / 128;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(128, std::min(fill, most)));
+    const int64_t sms = device_sm_count();
+    const int64_t twice = std::min(6 * sms / ctas, (keys + 127) / 128), once = std::min(3 * sms / ctas, (keys + 31) / 32);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS, std::max(twice, once)));
 }
 
 int window_decode(const AttnProblem &p, const SplitRows &rows, cudaStream_t stream) {
