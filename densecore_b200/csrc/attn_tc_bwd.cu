@@ -219,7 +219,18 @@ struct TcBwdArgs {
     const float *lse2;  // (B*H, L) lse * log2(e), written by the pre-pass
     float scale_log2;
     int *err;
+    // Sliding window: the first tokens' key tiles see every later row, 16,384 rows against the window and
+    // tile of their neighbours, and one CTA with all of them would outlast the rest. Their far rows (past
+    // the tile's window) are cut into sink_runs runs of at most sink_run query blocks for CTAs of their
+    // own, sink_ctas in all, which come first in the grid: number (run * sink_tiles + tile) * sink_units +
+    // unit (batch, key/value head and column half), each with 128 x 64 floats of dV and dK at sink_part.
+    uint32_t sink_ctas;
+    int sink_tiles, sink_units, sink_runs, sink_run;
+    float *sink_part;
 };
+
+// Floats of one such CTA's dV and dK.
+constexpr int64_t SINK_PART = 2 * TILE * 64;
 
 // ================================================================= pre-pass ==========
 struct PrepArgs {
@@ -391,22 +402,49 @@ __global__ void __maxnreg__(168)
     const AttnProblem &p = a.p;
     // Key tiles in ascending order: under causal masking tile 0 sees the most query rows.
     int64_t kt, bhd;
-    grouped_tile(blockIdx.x, (uint32_t)((p.S + TILE - 1) / TILE), (uint32_t)(p.B * p.Hkv * C::NH), kt, bhd);
+    const uint32_t sink_ctas = WIN ? a.sink_ctas : 0u;
+    const bool far = WIN && blockIdx.x < sink_ctas;  // a run of a first token's far rows
+    if (far) {
+        bhd = blockIdx.x % (uint32_t)a.sink_units;
+        kt = blockIdx.x / (uint32_t)a.sink_units % (uint32_t)a.sink_tiles;
+    } else {
+        grouped_tile(blockIdx.x - sink_ctas, (uint32_t)((p.S + TILE - 1) / TILE), (uint32_t)(p.B * p.Hkv * C::NH), kt, bhd);
+    }
     const int dh = (int)(bhd % C::NH);  // gradient column half
     const uint32_t bh = (uint32_t)(bhd / C::NH);
     const int64_t hk = bh % (uint32_t)p.Hkv, b = bh / (uint32_t)p.Hkv, k0 = kt * TILE;
     // Query blocks this CTA visits: for each query head of the group, rows [r_begin, L).
     // (through a window, those that see one of this CTA's keys).
     int64_t r_begin = p.causal ? min(k0, p.L) : 0, r_end = p.L;
-    if constexpr (WIN) window_rows(p, k0, min((int64_t)TILE, p.S - k0), r_begin, r_end);
-    const int qb_first = (int)(r_begin / QB);
-    const int qb_per_head = (int)((r_end + QB - 1) / QB) - qb_first;
-    const int nblk = qb_per_head * p.group;
+    int qb_first, qb_per_head, nblk, blk0 = 0;
+    if constexpr (WIN) {
+        const int64_t keys = min((int64_t)TILE, p.S - k0);
+        window_rows(p, k0, keys, r_begin, r_end);
+        qb_first = (int)(r_begin / QB);
+        if (sink_ctas && k0 < p.sinks) {
+            const int64_t near_end = max(r_begin, min(p.L, k0 + keys - 1 + p.window - p.offset));
+            const int near_blk = max(qb_first, (int)((near_end + QB - 1) / QB));
+            if (far) {
+                qb_first = near_blk;
+                blk0 = (int)(blockIdx.x / (uint32_t)a.sink_units / (uint32_t)a.sink_tiles) * a.sink_run;
+            } else {
+                r_end = (int64_t)near_blk * QB;
+            }
+        }
+        qb_per_head = max((int)((r_end + QB - 1) / QB) - qb_first, 0);
+        nblk = qb_per_head * p.group;
+        if (far) nblk = max(0, min(a.sink_run, nblk - blk0));
+    } else {
+        qb_first = (int)(r_begin / QB);
+        qb_per_head = (int)((p.L + QB - 1) / QB) - qb_first;
+        nblk = qb_per_head * p.group;
+    }
     auto bar = [&](int i) { return sb + C::OFF_BAR + 8u * (uint32_t)i; };
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sg + C::OFF_MISC);
     volatile int *abort = reinterpret_cast<volatile int *>(sg + C::OFF_MISC + 4);
     int *err = a.err;
     auto blk_coords = [&](int i, int64_t &h, int64_t &q0) {
+        if (WIN) i += blk0;
         h = hk * p.group + i / qb_per_head;
         q0 = (int64_t)(qb_first + i % qb_per_head) * QB;
     };
@@ -723,7 +761,10 @@ __global__ void __maxnreg__(168)
             }
         }
         const bool aborted = __any_sync(FULL, *abort != 0);
-        if (ok && !aborted && key_ok) {
+        if (far) {
+            if (ok && !aborted && key_ok && key < p.sinks)
+                store_row<64>(a.sink_part + (int64_t)blockIdx.x * SINK_PART + ((int64_t)half * TILE + row) * 64, 1, acc, half ? p.scale : 1.0f);
+        } else if (ok && !aborted && key_ok) {
             if (half) {
                 float *dkr = a.g.dk + b * a.g.dks[0] + hk * a.g.dks[1] + key * a.g.dks[2] + (int64_t)(64 * dh) * a.g.dks[3];
                 store_row<64>(dkr, a.g.dks[3], acc, p.scale);
@@ -1138,6 +1179,25 @@ __global__ void __maxnreg__(168)
     }
 }
 
+// Adds the far rows' runs to dV and dK of the first tokens' keys, in the order of the runs: a block per
+// (unit, tile), after the dK / dV kernel.
+template <int DD>
+__global__ void __launch_bounds__(256) bwd_sink_kernel(const TcBwdArgs a) {
+    const AttnProblem &p = a.p;
+    const int unit = blockIdx.x, tile = blockIdx.y, dh = unit % (DD / 64), bh = unit / (DD / 64);
+    const int64_t hk = bh % p.Hkv, b = bh / p.Hkv, k0 = (int64_t)tile * TILE;
+    const int keys = (int)min((int64_t)TILE, min(p.sinks, p.S) - k0);
+    for (int i = threadIdx.x; i < 2 * keys * 64; i += 256) {
+        const int col = i % 64, row = i / 64 % keys, half = i / 64 / keys;
+        float sum = 0.0f;
+        for (int run = 0; run < a.sink_runs; run++)
+            sum += a.sink_part[((int64_t)(run * a.sink_tiles + tile) * a.sink_units + unit) * SINK_PART + ((int64_t)half * TILE + row) * 64 + col];
+        const int64_t key = k0 + row, ch = 64 * dh + col;
+        if (half) a.g.dk[b * a.g.dks[0] + hk * a.g.dks[1] + key * a.g.dks[2] + ch * a.g.dks[3]] += sum;
+        else a.g.dv[b * a.g.dvs[0] + hk * a.g.dvs[1] + key * a.g.dvs[2] + ch * a.g.dvs[3]] += sum;
+    }
+}
+
 bool rows_vec(const void *ptr, const int64_t *st) {
     return st[3] == 1 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0 &&
            (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
@@ -1207,8 +1267,10 @@ int tc_backward_dd(const AttnProblem &p, const AttnGrads &g, int precision, cuda
     const int64_t rows_a = p.B * p.H * p.L, rows_b = p.B * p.Hkv * p.S;
     // Raw mode (3xTF32 with TMA-readable q, k, v and grad_out): the kernels read the hi
     // operands from the inputs and the pre-pass writes only the lo parts (half the scratch
-    // and the pre-pass's writes). Otherwise the pre-pass copies hi (rounded) and lo.
-    const bool raw = split && tma_readable(p.q, p.B, p.H, p.L, p.qs) && tma_readable(p.k, p.B, p.Hkv, p.S, p.ks) &&
+    // and the pre-pass's writes). Otherwise the pre-pass copies hi (rounded) and lo. Through a window it
+    // always does: rounded high parts leave 4.6e-7 of a gradient's norm wrong where truncated ones leave
+    // 1.3e-6 (8 x 12 heads of 1024 rows, window 256), for 15 us of 330.
+    const bool raw = !p.window && split && tma_readable(p.q, p.B, p.H, p.L, p.qs) && tma_readable(p.k, p.B, p.Hkv, p.S, p.ks) &&
                      tma_readable(p.v, p.B, p.Hkv, p.S, p.vs) && tma_readable(g.dout, p.B, p.H, p.L, g.dos);
     const int64_t NC = raw ? 1 : (split ? 2 : 1);  // copies per operand in the scratch
     const size_t bytes = sizeof(float) * (size_t)(NC * 2 * (rows_a + rows_b) * DD + rows_a);
@@ -1258,6 +1320,29 @@ int tc_backward_dd(const AttnProblem &p, const AttnGrads &g, int precision, cuda
     auto v_maps = [&](HiLoMaps &m, int box, CUtensorMapSwizzle sw) {
         return make_hilo(m, raw, p.v, p.vs, pa.vhl, DD, p.S, p.Hkv, p.B, box, sw);
     };
+    // The first tokens' far rows (TcBwdArgs): cut up where they are more than twice a regular tile's, into
+    // runs no shorter than that and no more of them than fill the GPU four times.
+    PoolScratch sink_ws;
+    sink_ws.stream = stream;
+    a.sink_ctas = 0;
+    a.sink_tiles = a.sink_units = a.sink_runs = a.sink_run = 0;
+    a.sink_part = nullptr;
+    if (p.window && p.sinks && p.S > 0 && p.L > 0) {
+        const int64_t qb = KC::QB, near_rows = max((int64_t)0, min(p.L, min((int64_t)TILE, p.S) - 1 + p.window - p.offset));
+        const int64_t far = p.group * ((p.L + qb - 1) / qb - (near_rows + qb - 1) / qb);
+        const int64_t regular = p.group * ((min(p.window, p.L) + TILE + qb - 1) / qb);
+        const int64_t tiles = (min(p.sinks, p.S) + TILE - 1) / TILE, units = p.B * p.Hkv * KC::NH;
+        const int64_t runs = min(min((int64_t)64, (far + regular - 1) / regular), 4 * (int64_t)device_sm_count() / (units * tiles));
+        if (far > 2 * regular && runs >= 2) {
+            a.sink_tiles = (int)tiles;
+            a.sink_units = (int)units;
+            a.sink_runs = (int)runs;
+            a.sink_run = (int)((far + runs - 1) / runs);
+            a.sink_ctas = (uint32_t)(runs * tiles * units);
+            if ((st = pool_alloc(&sink_ws.ptr, sizeof(float) * (size_t)a.sink_ctas * SINK_PART, stream))) return st;
+            a.sink_part = static_cast<float *>(sink_ws.ptr);
+        }
+    }
     // The two tensor-core kernels run concurrently; with tracing on, this record spans both
     // (from before the fork to after the join, on the caller's stream).
     KernelTrace pair("bwd_tc", stream);
@@ -1290,20 +1375,27 @@ int tc_backward_dd(const AttnProblem &p, const AttnGrads &g, int precision, cuda
                            : (masked ? attn_bwd_dkdv_tc_kernel<DD, false, true, false, true> : attn_bwd_dkdv_tc_kernel<DD, false, false, false, true>);
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)KC::SMEM);
         if (e != cudaSuccess) return cuda_fail(e, "attn_bwd_dkdv_tc smem attribute");
-        const unsigned grid = (unsigned)((p.S + TILE - 1) / TILE * p.Hkv * p.B * KC::NH);
-        KernelTrace tr("bwd_dkdv_tc", stream);
-        // Short rows (at most 512 queries): the CTAs are short and start-up bound, so the dK / dV
-        // CTAs become resident while the pre-pass drains (a programmatic dependent launch).
-        // Longer rows launch normally: there dK / dV taking every SM first delays the dQ kernel,
-        // the pair's longer part.
-        if (p.L <= 512) {
-            e = launch_dependent(kernel, dim3(grid), dim3(THREADS), KC::SMEM, stream, tk.hi, tv.hi, tqk.hi, tqmn.hi,
-                                 tdok.hi, tdomn.hi, tk.lo, tv.lo, tqk.lo, tqmn.lo, tdok.lo, tdomn.lo, a);
-            if (e != cudaSuccess) return cuda_fail(e, "attn_bwd_dkdv_tc");
-        } else {
-            kernel<<<grid, THREADS, KC::SMEM, stream>>>(tk.hi, tv.hi, tqk.hi, tqmn.hi, tdok.hi, tdomn.hi, tk.lo, tv.lo,
-                                                         tqk.lo, tqmn.lo, tdok.lo, tdomn.lo, a);
-            if ((st = check_launch("attn_bwd_dkdv_tc"))) return st;
+        const unsigned grid = (unsigned)((p.S + TILE - 1) / TILE * p.Hkv * p.B * KC::NH) + a.sink_ctas;
+        {
+            KernelTrace tr("bwd_dkdv_tc", stream);
+            // Short rows (at most 512 queries): the CTAs are short and start-up bound, so the dK / dV
+            // CTAs become resident while the pre-pass drains (a programmatic dependent launch).
+            // Longer rows launch normally: there dK / dV taking every SM first delays the dQ kernel,
+            // the pair's longer part.
+            if (p.L <= 512) {
+                e = launch_dependent(kernel, dim3(grid), dim3(THREADS), KC::SMEM, stream, tk.hi, tv.hi, tqk.hi, tqmn.hi,
+                                     tdok.hi, tdomn.hi, tk.lo, tv.lo, tqk.lo, tqmn.lo, tdok.lo, tdomn.lo, a);
+                if (e != cudaSuccess) return cuda_fail(e, "attn_bwd_dkdv_tc");
+            } else {
+                kernel<<<grid, THREADS, KC::SMEM, stream>>>(tk.hi, tv.hi, tqk.hi, tqmn.hi, tdok.hi, tdomn.hi, tk.lo, tv.lo,
+                                                             tqk.lo, tqmn.lo, tdok.lo, tdomn.lo, a);
+                if ((st = check_launch("attn_bwd_dkdv_tc"))) return st;
+            }
+        }
+        if (a.sink_ctas) {
+            KernelTrace tr("bwd_sink", stream);
+            bwd_sink_kernel<DD><<<dim3((unsigned)a.sink_units, (unsigned)a.sink_tiles), 256, 0, stream>>>(a);
+            if ((st = check_launch("bwd_sink"))) return st;
         }
     }
     if (p.L > 0) {

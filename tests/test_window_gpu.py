@@ -212,3 +212,21 @@ def test_repeats_bit_for_bit():
     first = check(q, k, v, 60, 4)[0]
     for _ in range(3):
         assert torch.equal(F.sliding_window_attention(q, k, v, 60, 4, enable_gqa=True), first)
+
+
+@pytest.mark.parametrize("layout", ["bshd", "odd"])
+@pytest.mark.parametrize("case", [  # b, h, kv, l, s, d, window, sinks, offset
+    (1, 1, 1, 1500, 1500, 64, 30, 4, None), (1, 4, 2, 1100, 1300, 64, 17, 200, None), (1, 2, 1, 1000, 1000, 128, 40, 130, None),
+    (2, 2, 2, 2000, 2000, 64, 1, 1, None), (1, 1, 1, 1500, 700, 64, 30, 4, -300), (1, 1, 1, 1300, 1300, 64, 30, 5000, None)])
+def test_first_tokens_seen_by_many_rows(case, layout):
+    # The first tokens' gradients are summed over runs of far rows by CTAs of their own.
+    b, h, kv, l, s, d, window, sinks, offset = case
+    q, k, v = make(b, h, kv, l, s, d, layout, 14)
+    check(q, k, v, window, sinks, offset)
+    mask = torch.arange(s, device="cuda") % 5 != 0
+    check(q, k, v, window, sinks, offset, mask=mask.view(1, 1, 1, s))
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    go = torch.ones(b, h, l, d, device="cuda")
+    runs = [torch.autograd.grad(F.sliding_window_attention(*leaves, window, sinks, offset=offset, enable_gqa=True), leaves, go)
+            for _ in range(2)]
+    assert all(torch.equal(x, y) for x, y in zip(*runs))
