@@ -351,11 +351,13 @@ struct AttnCfg {
     }
     // A group's tile of weights: COLS rows of 16 keys in bfloat16, padded against bank conflicts.
     static constexpr int W_GROUP = COLS * 32 + 32;
-    static constexpr int STAGES = D == 64 ? 4 : (D == 128 ? 3 : 2);  // blocks of a warp's ring
+    // Blocks a warp takes at a time (their chains overlap, and waiting, masks and maxima are paid once), and
+    // how many such sets its ring holds.
+    static constexpr int KB = D == 256 ? 1 : 2, STAGES = D == 64 ? 3 : 2;
     // Shared memory: the warps' rings | q fragments | the warps' weight tiles; after the loop the
     // accumulators.
-    static constexpr int BLOCK = block_bytes(D), RING = STAGES * BLOCK;
-    static constexpr int Q_BYTES = NT * NG * 32 * 16, W_BYTES = NG * W_GROUP;
+    static constexpr int BLOCK = block_bytes(D), STAGE = KB * BLOCK, RING = STAGES * STAGE;
+    static constexpr int Q_BYTES = NT * NG * 32 * 16, W_BYTES = KB * NG * W_GROUP;
     static constexpr int OFF_Q = WARPS * RING, OFF_W = OFF_Q + Q_BYTES, LOOP_BYTES = OFF_W + WARPS * W_BYTES;
     static constexpr int ACC_COLS = ONE ? PARTS : COLS, ACC_BYTES = WARPS * ACC_COLS * D * 4;
     static constexpr int SMEM = LOOP_BYTES > ACC_BYTES ? LOOP_BYTES : ACC_BYTES;
@@ -368,10 +370,10 @@ __device__ __forceinline__ float load_q(const Cache4Args &a, int64_t at) {
 }
 
 template <int D, int PARTS, int HEADS>
-__global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : (HEADS == 1 ? 5 : 4)))
+__global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : 4))
     cache4_attention_kernel(const Cache4Args a, const SplitRows rows) {
     using C = AttnCfg<D, PARTS, HEADS>;
-    constexpr int NG = C::NG, NT = C::NT, NS = C::NS;
+    constexpr int NG = C::NG, NT = C::NT, NS = C::NS, KB = C::KB;
     constexpr bool ONE = C::ONE;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t s_full[WARPS][C::STAGES];
@@ -400,39 +402,48 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : (
     const int per = (total + rows.splits - 1) / rows.splits, v0 = blockIdx.x * per, v1 = min(total, v0 + per);
     const uint32_t page16 = (uint32_t)a.c.page_size / 16;
     auto block_of = [&](int v) { return v < sink_blocks ? v : first + v - sink_blocks; };
-    // The pool's block numbers of this warp's next 32 blocks, one to a lane (-1: the table's entry is out
-    // of range), and of the 32 after those: the division by the page size and the table's latency are
-    // paid once in 32 blocks.
+    // The warp's sets of KB blocks: from v0 + warp * KB on, every WARPS-th. The pool's block numbers of its
+    // next 32 blocks, one to a lane, and of the 32 after those: the division by the page size and the
+    // table's latency are paid once in 32 blocks. BAD: the table's entry is out of range; ABSENT: no block.
+    constexpr int BAD = -1, ABSENT = -2;
     const int32_t *table = a.table + b * a.ts[0];
-    auto numbers = [&](int v) -> int {
-        v += lane * WARPS;
-        if (v >= v1) return -1;
+    auto numbers = [&](int set) -> int {  // of the 32 / KB sets from number `set` on
+        const int v = v0 + (warp + (set + lane / KB) * WARPS) * KB + lane % KB;
+        if (v >= v1) return ABSENT;
         const uint32_t at = (uint32_t)block_of(v), entry = at / page16;
         const int id = table[entry * a.ts[1]];
-        return (uint32_t)id < (uint32_t)a.c.pages ? (int)(((uint32_t)id * (uint32_t)a.c.Hkv + hk) * page16 + (at - entry * page16)) : -1;
+        return (uint32_t)id < (uint32_t)a.c.pages ? (int)(((uint32_t)id * (uint32_t)a.c.Hkv + hk) * page16 + (at - entry * page16)) : BAD;
     };
-    // This warp's ring. A block whose page id is out of range is not copied: its stage completes empty
-    // and its keys are left out (stage_ok).
+    // This warp's ring. A block whose page id is out of range is not copied: its keys are left out
+    // (stage_ok: KB bits a stage).
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * C::RING;
     const uint32_t full = (uint32_t)__cvta_generic_to_shared(&s_full[warp][0]);
     volatile int *abort = &s_abort;
     uint32_t stage_ok = 0;
-    int v = v0 + warp, fetched = 0;
-    int numbers_now = numbers(v), numbers_next = numbers(v + 32 * WARPS);
-    auto fetch = [&](int stage) {  // the warp's block number `fetched`
-        const int number = __shfl_sync(ALL, numbers_now, fetched & 31);
-        if ((++fetched & 31) == 0) {
-            numbers_now = numbers_next;
-            numbers_next = numbers(v0 + warp + (fetched + 32) * WARPS);
+    int v = v0 + warp * KB, fetched = 0;
+    int numbers_now = numbers(0), numbers_next = numbers(32 / KB);
+    auto fetch = [&](int stage) {  // the warp's set number `fetched`
+        int number[KB], there = 0;
+#pragma unroll
+        for (int e = 0; e < KB; e++) {
+            number[e] = __shfl_sync(ALL, numbers_now, (fetched * KB + e) & 31);
+            there += number[e] >= 0;
+            const int bit = stage * KB + e;
+            stage_ok = (stage_ok & ~(1u << bit)) | ((uint32_t)(number[e] >= 0) << bit);
         }
-        stage_ok = (stage_ok & ~(1u << stage)) | ((uint32_t)(number >= 0) << stage);
+        if ((++fetched * KB & 31) == 0) {
+            numbers_now = numbers_next;
+            numbers_next = numbers(fetched + 32 / KB);
+        }
         if (lane == 0) {
-            if (number >= 0) {
-                sm100::mbar_expect_tx(full + 8 * stage, C::BLOCK);
-                bulk_copy(ring + stage * C::BLOCK, a.c.data + (int64_t)number * C::BLOCK, C::BLOCK, full + 8 * stage);
-            } else {
-                atomicExch(a.err, BAD_TABLE);
-                sm100::mbar_arrive(full + 8 * stage);
+            if (there) sm100::mbar_expect_tx(full + 8 * stage, there * C::BLOCK);
+            else sm100::mbar_arrive(full + 8 * stage);
+#pragma unroll
+            for (int e = 0; e < KB; e++) {
+                if (number[e] >= 0)
+                    bulk_copy(ring + stage * C::STAGE + e * C::BLOCK, a.c.data + (int64_t)number[e] * C::BLOCK, C::BLOCK, full + 8 * stage);
+                else if (number[e] == BAD)
+                    atomicExch(a.err, BAD_TABLE);
             }
         }
     };
@@ -444,7 +455,7 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : (
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < C::STAGES; i++)
-        if (v + i * WARPS < v1) fetch(i);
+        if (v + i * WARPS * KB < v1) fetch(i);
 
     // q: per head a power of two that brings its largest channel below 1, the sums of its groups,
     // and the two fp16 parts in the order of the products' B fragments.
@@ -550,98 +561,115 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : (
     const uint32_t soff = 8 * D + (r * NG + (ONE ? (NG < 4 ? t % NG : t) : 0)) * 4;
     int stage = 0;
     uint32_t parity = 0;
-    for (; v < v1; v += WARPS) {
+    for (; v < v1; v += WARPS * KB) {
         if (!sm100::mbar_wait_warp(full + 8 * stage, parity, abort, a.err)) break;
-        const uint8_t *cur = blk + stage * C::BLOCK;
-        const bool cur_ok = (stage_ok >> stage) & 1u;
-        // Which of keys r and r + 8 are seen; all of them in most blocks.
-        const int k0 = block_of(v) * 16;
-        bool ok0 = true, ok1 = true;
-        const bool edge = !cur_ok || k0 + 16 > len || (k0 < lo && k0 + 16 > sinks);
-        if (edge) {
-            const int j0 = k0 + r, j1 = j0 + 8;
-            ok0 = cur_ok && j0 < len && (j0 >= lo || j0 < sinks);
-            ok1 = cur_ok && j1 < len && (j1 >= lo || j1 < sinks);
+        const uint8_t *cur = blk + stage * C::STAGE;
+        // Which of keys r and r + 8 of each block are seen; all of them in most sets.
+        bool ok0[KB], ok1[KB], edge = false;
+#pragma unroll
+        for (int e = 0; e < KB; e++) {
+            const int k0 = block_of(v + e) * 16;
+            ok0[e] = ok1[e] = true;
+            edge = edge || !((stage_ok >> (stage * KB + e)) & 1u) || k0 + 16 > len || (k0 < lo && k0 + 16 > sinks);
         }
-        uint32_t kc[2][NG], ks[2][NS];
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            read_words<NG>(cur + koff + 8 * i * (D / 2), kc[i]);
-            if constexpr (ONE) {
-#pragma unroll
-                for (int j = 0; j < NS; j++) read_words<1>(cur + soff + 8 * i * NG * 4 + 16 * j, &ks[i][j]);
-            } else {
-                read_words<NG>(cur + soff + 8 * i * NG * 4, ks[i]);
+            for (int e = 0; e < KB; e++) {
+                const bool there = (stage_ok >> (stage * KB + e)) & 1u;
+                const int j0 = block_of(v + e) * 16 + r, j1 = j0 + 8;
+                ok0[e] = there && j0 < len && (j0 >= lo || j0 < sinks);
+                ok1[e] = there && j1 < len && (j1 >= lo || j1 < sinks);
             }
         }
         // Scores of keys r and r + 8.
-        float s0[NT], s1[NT];
-        if constexpr (ONE) {
-            int hi[NS][4], lw[NS][4];  // digits 3, 2 and 1, 0 of keys r, r + 8
+        float s0[KB][NT], s1[KB][NT];
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t y[4] = {kc[0][g] & 0x0F0F0F0Fu, kc[1][g] & 0x0F0F0F0Fu, (kc[0][g] >> 4) & 0x0F0F0F0Fu,
-                                       (kc[1][g] >> 4) & 0x0F0F0F0Fu};
-                const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + (g * 32 + lane) * 16);
-                mma_u8s8(hi[g / 4], y, q.x, q.y, g % 4 ? hi[g / 4] : centre_hi[g / 4]);
-                mma_u8s8(lw[g / 4], y, q.z, q.w, g % 4 ? lw[g / 4] : centre_lo[g / 4]);
-            }
-            float x0 = 0.0f, x1 = 0.0f;
+        for (int e = 0; e < KB; e++) {
+            const uint8_t *at = cur + e * C::BLOCK;
+            uint32_t kc[2][NG], ks[2][NS];
 #pragma unroll
-            for (int i = 0; i < NS; i++) {
-                // Each pair of digits is below 2^23: exact in 32 bits, their sum rounded once.
-                const float d0 = fmaf((float)(hi[i][0] * 128 + hi[i][1]), 16384.0f, (float)(lw[i][0] * 128 + lw[i][1]));
-                const float d1 = fmaf((float)(hi[i][2] * 128 + hi[i][3]), 16384.0f, (float)(lw[i][2] * 128 + lw[i][3]));
-                x0 = fmaf(bf16_low(ks[0][i]) * mul[0], d0, fmaf(mid(ks[0][i]), qsum[0][i], x0));
-                x1 = fmaf(bf16_low(ks[1][i]) * mul[0], d1, fmaf(mid(ks[1][i]), qsum[0][i], x1));
-            }
-            if (NG < 4 && t >= NG) x0 = x1 = 0.0f;  // head dim 64: two groups for four lanes
+            for (int i = 0; i < 2; i++) {
+                read_words<NG>(at + koff + 8 * i * (D / 2), kc[i]);
+                if constexpr (ONE) {
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                x0 += __shfl_xor_sync(ALL, x0, o);
-                x1 += __shfl_xor_sync(ALL, x1, o);
-            }
-            s0[0] = x0;
-            s1[0] = x1;
-        } else {
-            float b0[NT], b1[NT];
-#pragma unroll
-            for (int n = 0; n < NT; n++) s0[n] = s1[n] = b0[n] = b1[n] = 0.0f;
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                uint32_t y0[4], y1[4];
-                codes_f16(kc[0][g], y0);
-                codes_f16(kc[1][g], y1);
-                const uint32_t a0[4] = {y0[0], y1[0], y0[1], y1[1]}, a1[4] = {y0[2], y1[2], y0[3], y1[3]};
-                const float sc0 = bf16_low(ks[0][g]), sc1 = bf16_low(ks[1][g]), mid0 = mid(ks[0][g]), mid1 = mid(ks[1][g]);
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + ((n * NG + g) * 32 + lane) * 16);
-                    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    float c[4];
-                    mma_f16(c, a0, q.x, q.y, zero);
-                    mma_f16(c, a1, q.z, q.w, c);
-                    s0[n] = fmaf(sc0, c[0] + c[1], s0[n]);
-                    s1[n] = fmaf(sc1, c[2] + c[3], s1[n]);
-                    b0[n] = fmaf(mid0, qsum[n][g], b0[n]);
-                    b1[n] = fmaf(mid1, qsum[n][g], b1[n]);
+                    for (int j = 0; j < NS; j++) read_words<1>(at + soff + 8 * i * NG * 4 + 16 * j, &ks[i][j]);
+                } else {
+                    read_words<NG>(at + soff + 8 * i * NG * 4, ks[i]);
                 }
             }
+            if constexpr (ONE) {
+                int hi[NS][4], lw[NS][4];  // digits 3, 2 and 1, 0 of keys r, r + 8
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                s0[n] = fmaf(s0[n], mul[n], b0[n]);
-                s1[n] = fmaf(s1[n], mul[n], b1[n]);
+                for (int g = 0; g < NG; g++) {
+                    const uint32_t y[4] = {kc[0][g] & 0x0F0F0F0Fu, kc[1][g] & 0x0F0F0F0Fu, (kc[0][g] >> 4) & 0x0F0F0F0Fu,
+                                           (kc[1][g] >> 4) & 0x0F0F0F0Fu};
+                    const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + (g * 32 + lane) * 16);
+                    mma_u8s8(hi[g / 4], y, q.x, q.y, g % 4 ? hi[g / 4] : centre_hi[g / 4]);
+                    mma_u8s8(lw[g / 4], y, q.z, q.w, g % 4 ? lw[g / 4] : centre_lo[g / 4]);
+                }
+                float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    // Each pair of digits is below 2^23: exact in 32 bits, their sum rounded once.
+                    const float d0 = fmaf((float)(hi[i][0] * 128 + hi[i][1]), 16384.0f, (float)(lw[i][0] * 128 + lw[i][1]));
+                    const float d1 = fmaf((float)(hi[i][2] * 128 + hi[i][3]), 16384.0f, (float)(lw[i][2] * 128 + lw[i][3]));
+                    x0 = fmaf(bf16_low(ks[0][i]) * mul[0], d0, fmaf(mid(ks[0][i]), qsum[0][i], x0));
+                    x1 = fmaf(bf16_low(ks[1][i]) * mul[0], d1, fmaf(mid(ks[1][i]), qsum[0][i], x1));
+                }
+                if (NG < 4 && t >= NG) x0 = x1 = 0.0f;  // head dim 64: two groups for four lanes
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    x0 += __shfl_xor_sync(ALL, x0, o);
+                    x1 += __shfl_xor_sync(ALL, x1, o);
+                }
+                s0[e][0] = x0;
+                s1[e][0] = x1;
+            } else {
+                float b0[NT], b1[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) s0[e][n] = s1[e][n] = b0[n] = b1[n] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    uint32_t y0[4], y1[4];
+                    codes_f16(kc[0][g], y0);
+                    codes_f16(kc[1][g], y1);
+                    const uint32_t a0[4] = {y0[0], y1[0], y0[1], y1[1]}, a1[4] = {y0[2], y1[2], y0[3], y1[3]};
+                    const float sc0 = bf16_low(ks[0][g]), sc1 = bf16_low(ks[1][g]), mid0 = mid(ks[0][g]), mid1 = mid(ks[1][g]);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint4 q = *reinterpret_cast<const uint4 *>(smem + C::OFF_Q + ((n * NG + g) * 32 + lane) * 16);
+                        const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float c[4];
+                        mma_f16(c, a0, q.x, q.y, zero);
+                        mma_f16(c, a1, q.z, q.w, c);
+                        s0[e][n] = fmaf(sc0, c[0] + c[1], s0[e][n]);
+                        s1[e][n] = fmaf(sc1, c[2] + c[3], s1[e][n]);
+                        b0[n] = fmaf(mid0, qsum[n][g], b0[n]);
+                        b1[n] = fmaf(mid1, qsum[n][g], b1[n]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    s0[e][n] = fmaf(s0[e][n], mul[n], b0[n]);
+                    s1[e][n] = fmaf(s1[e][n], mul[n], b1[n]);
+                }
             }
+        }
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < KB; e++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    s0[e][n] = ok0[e] ? s0[e][n] : -INFINITY;
+                    s1[e][n] = ok1[e] ? s1[e][n] : -INFINITY;
+                }
         }
         float corr[NT];
         bool moved = false;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            if (edge) {
-                s0[n] = ok0 ? s0[n] : -INFINITY;
-                s1[n] = ok1 ? s1[n] : -INFINITY;
-            }
-            float top = fmaxf(s0[n], s1[n]);
+            float top = fmaxf(s0[0][n], s1[0][n]);
+            if (KB == 2) top = fmaxf(top, fmaxf(s0[KB - 1][n], s1[KB - 1][n]));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(ALL, top, o));
             corr[n] = 1.0f;
@@ -667,64 +695,74 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : (
                     for (int c = 0; c < 4; c++) acc[i][n][c] *= corr[NT == 2 ? n : 0];
         }
         // Weights times the values' scales, in bfloat16 parts, to the warp's tiles.
-        uint32_t vs[2][NS];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if constexpr (ONE) {
-#pragma unroll
-                for (int j = 0; j < NS; j++) read_words<1>(cur + 10 * D + soff + 8 * i * NG * 4 + 16 * j, &vs[i][j]);
-            } else {
-                read_words<NG>(cur + 10 * D + soff + 8 * i * NG * 4, vs[i]);
-            }
-        }
-        if (edge) {  // a place behind the sequence's end may hold anything
-#pragma unroll
-            for (int g = 0; g < NS; g++) {
-                if (!ok0) vs[0][g] = 0u;
-                if (!ok1) vs[1][g] = 0u;
-            }
-        }
         __syncwarp();
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const float p0 = exp2_fast(s0[n] - base[n]), p1 = exp2_fast(s1[n] - base[n]);
-            l[n] += p0 + p1;
+        for (int e = 0; e < KB; e++) {
+            uint32_t vs[2][NS];
 #pragma unroll
-            for (int g = 0; g < NS; g++) {
-                const uint32_t z0 = vs[0][g], z1 = vs[1][g];
-                low[n][g] = fmaf(p0, mid(z0), fmaf(p1, mid(z1), low[n][g]));
-                float w0 = p0 * bf16_low(z0), w1 = p1 * bf16_low(z1);
-                const int own = ONE ? t + 4 * g : g;
-                if (own < NG) {
+            for (int i = 0; i < 2; i++) {
+                const uint8_t *at = cur + e * C::BLOCK + 10 * D + soff + 8 * i * NG * 4;
+                if constexpr (ONE) {
 #pragma unroll
-                    for (int part = 0; part < PARTS; part++) {
-                        const uint32_t w = pack_bf16(w0, w1);
-                        *reinterpret_cast<uint32_t *>(wt + own * C::W_GROUP + C::column(ONE ? 0 : n * 4 + t, part) * 32 + wt_put) = w;
-                        w0 -= bf16_low(w);
-                        w1 -= bf16_high(w);
+                    for (int j = 0; j < NS; j++) read_words<1>(at + 16 * j, &vs[i][j]);
+                } else {
+                    read_words<NG>(at, vs[i]);
+                }
+            }
+            if (edge) {  // a place behind the sequence's end may hold anything
+#pragma unroll
+                for (int g = 0; g < NS; g++) {
+                    if (!ok0[e]) vs[0][g] = 0u;
+                    if (!ok1[e]) vs[1][g] = 0u;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float p0 = exp2_fast(s0[e][n] - base[n]), p1 = exp2_fast(s1[e][n] - base[n]);
+                l[n] += p0 + p1;
+#pragma unroll
+                for (int g = 0; g < NS; g++) {
+                    const uint32_t z0 = vs[0][g], z1 = vs[1][g];
+                    low[n][g] = fmaf(p0, mid(z0), fmaf(p1, mid(z1), low[n][g]));
+                    float w0 = p0 * bf16_low(z0), w1 = p1 * bf16_low(z1);
+                    const int own = ONE ? t + 4 * g : g;
+                    if (own < NG) {
+#pragma unroll
+                        for (int part = 0; part < PARTS; part++) {
+                            const uint32_t w = pack_bf16(w0, w1);
+                            *reinterpret_cast<uint32_t *>(wt + (e * NG + own) * C::W_GROUP + C::column(ONE ? 0 : n * 4 + t, part) * 32 + wt_put) = w;
+                            w0 -= bf16_low(w);
+                            w1 -= bf16_high(w);
+                        }
                     }
                 }
             }
         }
-        uint32_t vc[2][NG];
-#pragma unroll
-        for (int i = 0; i < 2; i++) read_words<NG>(cur + voff + i * 32 * 4 * NG, vc[i]);
         __syncwarp();
-        // Every lane holds its part of the block: the stage takes the block STAGES further on.
-        if (v + C::STAGES * WARPS < v1) fetch(stage);
-        if (++stage == C::STAGES) stage = 0, parity ^= 1u;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            // (Columns without a part are read as they come: what they give is never looked at.)
-            uint2 w[C::NC];
+        for (int e = 0; e < KB; e++) {
+            uint32_t vc[2][NG];
 #pragma unroll
-            for (int n = 0; n < C::NC; n++) w[n] = *reinterpret_cast<const uint2 *>(wt + g * C::W_GROUP + n * 256 + wt_get);
+            for (int i = 0; i < 2; i++) read_words<NG>(cur + e * C::BLOCK + voff + i * 32 * 4 * NG, vc[i]);
+            if (e == KB - 1) {
+                // Every lane holds its part of the blocks: the stage takes the set STAGES further on.
+                __syncwarp();
+                if (v + C::STAGES * WARPS * KB < v1) fetch(stage);
+                if (++stage == C::STAGES) stage = 0, parity ^= 1u;
+            }
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint32_t y[4] = {codes_bf16(vc[0][g], 2 * j), codes_bf16(vc[0][g], 2 * j + 1), codes_bf16(vc[1][g], 2 * j),
-                                       codes_bf16(vc[1][g], 2 * j + 1)};
+            for (int g = 0; g < NG; g++) {
+                // (Columns without a part are read as they come: what they give is never looked at.)
+                uint2 w[C::NC];
 #pragma unroll
-                for (int n = 0; n < C::NC; n++) mma_bf16(acc[2 * g + j][n], y, w[n].x, w[n].y);
+                for (int n = 0; n < C::NC; n++) w[n] = *reinterpret_cast<const uint2 *>(wt + (e * NG + g) * C::W_GROUP + n * 256 + wt_get);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t y[4] = {codes_bf16(vc[0][g], 2 * j), codes_bf16(vc[0][g], 2 * j + 1), codes_bf16(vc[1][g], 2 * j),
+                                           codes_bf16(vc[1][g], 2 * j + 1)};
+#pragma unroll
+                    for (int n = 0; n < C::NC; n++) mma_bf16(acc[2 * g + j][n], y, w[n].x, w[n].y);
+                }
             }
         }
     }
@@ -732,7 +770,7 @@ __global__ void __launch_bounds__(WARPS * 32, D == 256 ? 2 : (HEADS == 8 ? 3 : (
         // A wait ran out: let this warp's copies land before the block's memory goes away. (fetch at v
         // has refilled the stages of the blocks before v: those of v .. v + STAGES - 1 may be in flight.)
         volatile int never = 0;
-        for (int i = 0; i < C::STAGES && v + i * WARPS < v1; i++) {
+        for (int i = 0; i < C::STAGES && v + i * WARPS * KB < v1; i++) {
             sm100::mbar_wait_warp(full + 8 * stage, parity, &never, nullptr);
             if (++stage == C::STAGES) stage = 0, parity ^= 1u;
         }
@@ -849,14 +887,14 @@ int cache4_read(const Cache4Args &a, cudaStream_t stream) {
 }
 
 // Splits of each row: enough CTAs to fill every SM's four places six times over, so that sequences of
-// different lengths even out, with at least 8 blocks a warp then; below that, down to one block a warp,
-// as many as fill the places once.
+// different lengths even out, with at least 8 blocks a warp then; below that, down to one set of two
+// blocks a warp, as many as fill the places once.
 int cache4_splits(int64_t B, int64_t H, int64_t Hkv, int64_t capacity, int64_t window, int64_t sinks, int dtype) {
     const int64_t group = H / Hkv, per = heads_per_cta(group, dtype), chunks = (group + per - 1) / per;
     const int64_t ctas = std::max<int64_t>(1, B * Hkv * chunks);
     const int64_t keys = window ? std::min(capacity, std::min(window, capacity) + std::min(sinks, capacity)) : capacity;
-    const int64_t places = (int64_t)device_sm_count() * 4, most = (keys + 16 * WARPS - 1) / (16 * WARPS);
-    const int64_t once = std::min(places / ctas, most), even = std::min((6 * places + ctas - 1) / ctas, most / 8);
+    const int64_t places = (int64_t)device_sm_count() * 4, most = (keys + 32 * WARPS - 1) / (32 * WARPS);
+    const int64_t once = std::min(places / ctas, most), even = std::min((6 * places + ctas - 1) / ctas, most / 4);
     return (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(once, even)));
 }
 
