@@ -551,14 +551,18 @@ __global__ void __maxnreg__(128)
             const float mnat = m == -INFINITY ? 0.0f : m * LN2;
             const float inv = 1.0f / lfin;
             float *orow = p.out + b * p.os[0] + h * p.os[1] + qrow * p.os[2] + (int64_t)half * C::HD * p.os[3];
-            if (p.os[3] == 1 && (reinterpret_cast<uintptr_t>(orow) & 15u) == 0) {
+            // (Through a window the head dim may be below D: its columns past Ev are zeros, not stored.)
+            const int cols = WIN ? (int)min((int64_t)C::HD, p.Ev - half * C::HD) : C::HD;
+            if (p.os[3] == 1 && (reinterpret_cast<uintptr_t>(orow) & 15u) == 0 && cols % 4 == 0) {
 #pragma unroll
                 for (int x = 0; x < C::HD; x += 4)
-                    *reinterpret_cast<float4 *>(orow + x) =
-                        make_float4(o[x] * inv, o[x + 1] * inv, o[x + 2] * inv, o[x + 3] * inv);
+                    if (!WIN || x < cols)
+                        *reinterpret_cast<float4 *>(orow + x) =
+                            make_float4(o[x] * inv, o[x + 1] * inv, o[x + 2] * inv, o[x + 3] * inv);
             } else {
 #pragma unroll
-                for (int x = 0; x < C::HD; x++) orow[x * p.os[3]] = o[x] * inv;
+                for (int x = 0; x < C::HD; x++)
+                    if (!WIN || x < cols) orow[x * p.os[3]] = o[x] * inv;
             }
             if (half == 0) p.lse[b * p.ls[0] + h * p.ls[1] + qrow * p.ls[2]] = mnat + logf(lfin);
         }
@@ -1038,14 +1042,18 @@ __global__ void __maxnreg__(128)
                 const float mnat = m == -INFINITY ? 0.0f : m * LN2;
                 const float inv = 1.0f / lfin;
                 float *orow = p.out + b * p.os[0] + h * p.os[1] + qrow * p.os[2] + (int64_t)half * C::HD * p.os[3];
-                if (p.os[3] == 1 && (reinterpret_cast<uintptr_t>(orow) & 15u) == 0) {
+                // (Through a window the head dim may be below D: its columns past Ev are zeros, not stored.)
+                const int cols = WIN ? (int)min((int64_t)C::HD, p.Ev - half * C::HD) : C::HD;
+                if (p.os[3] == 1 && (reinterpret_cast<uintptr_t>(orow) & 15u) == 0 && cols % 4 == 0) {
 #pragma unroll
                     for (int x = 0; x < C::HD; x += 4)
-                        *reinterpret_cast<float4 *>(orow + x) =
-                            make_float4(o[x] * inv, o[x + 1] * inv, o[x + 2] * inv, o[x + 3] * inv);
+                        if (!WIN || x < cols)
+                            *reinterpret_cast<float4 *>(orow + x) =
+                                make_float4(o[x] * inv, o[x + 1] * inv, o[x + 2] * inv, o[x + 3] * inv);
                 } else {
 #pragma unroll
-                    for (int x = 0; x < C::HD; x++) orow[x * p.os[3]] = o[x] * inv;
+                    for (int x = 0; x < C::HD; x++)
+                        if (!WIN || x < cols) orow[x * p.os[3]] = o[x] * inv;
                 }
                 if (half == 0) p.lse[b * p.ls[0] + h * p.ls[1] + qrow * p.ls[2]] = mnat + logf(lfin);
             }
@@ -1136,7 +1144,8 @@ int *device_error_word() {
 }
 
 bool tc_forward_supported(const AttnProblem &p) {
-    if (p.E != p.Ev || (p.E != 64 && p.E != 128)) return false;
+    // Through a window any head dims up to 128 (TMA fills the columns past them with zeros).
+    if (p.window ? (p.E > 128 || p.Ev > 128 || p.E == 0 || p.Ev == 0) : (p.E != p.Ev || (p.E != 64 && p.E != 128))) return false;
     if (p.qs[3] != 1 || p.ks[3] != 1 || p.vs[3] != 1) return false;
     if (!tma_stride_ok(p.L, p.qs[2]) || !tma_stride_ok(p.H, p.qs[1]) || !tma_stride_ok(p.B, p.qs[0])) return false;
     if (!tma_stride_ok(p.S, p.ks[2]) || !tma_stride_ok(p.Hkv, p.ks[1]) || !tma_stride_ok(p.B, p.ks[0])) return false;
@@ -1148,7 +1157,7 @@ bool tc_forward_supported(const AttnProblem &p) {
 
 int tc_forward(const AttnProblem &p, int precision, cudaStream_t stream) {
     const int split = precision == DC_PREC_TF32 ? 0 : 1;
-    return p.E == 64 ? launch_fwd<Fwd64>(p, split, stream) : launch_fwd<Fwd128>(p, split, stream);
+    return max(p.E, p.Ev) <= 64 ? launch_fwd<Fwd64>(p, split, stream) : launch_fwd<Fwd128>(p, split, stream);
 }
 
 int device_error(int reset) {

@@ -201,6 +201,15 @@ __device__ __forceinline__ void store_row(float *dst, int64_t inner, const float
     }
 }
 
+// store_row of the first n columns (n may be negative or above N).
+template <int N>
+__device__ __forceinline__ void store_row_below(float *dst, int64_t inner, const float *acc, float mul, int64_t n) {
+    if (n >= N) return store_row<N>(dst, inner, acc, mul);
+#pragma unroll
+    for (int c = 0; c < N; c++)
+        if (c < n) dst[c * inner] = acc[c] * mul;
+}
+
 // Tile `tile` and (batch, head) pair `bh` of CTA `idx` in the grouped order: idx runs over
 // groups of GROUP_HEADS pairs, inside a group over tiles (outer) and pairs (inner). The grids
 // are below 2^31 CTAs (tc_backward_supported), so the decode divides in 32 bits (every CTA
@@ -295,6 +304,15 @@ __device__ __forceinline__ void split_store(float *hl, int64_t at, int64_t lo_of
     }
 }
 
+// load4 of a row of n elements (through a window the head dim may be below DD): zeros from n on.
+__device__ __forceinline__ float4 load4_below(const float *row, int64_t inner, int j, int vec, int64_t n) {
+    if (4 * j + 4 <= n) return load4(row, inner, j, vec);
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = 4 * j + i < n ? row[(4 * j + i) * inner] : 0.0f;
+    return make_float4(x[0], x[1], x[2], x[3]);
+}
+
 // DD / 4 lanes per row of DD (a float4 each): rows of (q, grad_out, out) first, then rows of
 // (k, v).
 template <int DD>
@@ -311,9 +329,9 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(PrepArgs a) {
     if (r < rows_a) {
         int64_t b, h, l;
         row_bhl(r, p.L, p.H, a.rows32, b, h, l);
-        const float4 q4 = load4(p.q + b * p.qs[0] + h * p.qs[1] + l * p.qs[2], p.qs[3], j, a.vec);
-        const float4 d4 = load4(a.g.dout + b * a.g.dos[0] + h * a.g.dos[1] + l * a.g.dos[2], a.g.dos[3], j, a.vec);
-        const float4 o4 = load4(p.out + b * p.os[0] + h * p.os[1] + l * p.os[2], p.os[3], j, a.vec);
+        const float4 q4 = load4_below(p.q + b * p.qs[0] + h * p.qs[1] + l * p.qs[2], p.qs[3], j, a.vec, p.E);
+        const float4 d4 = load4_below(a.g.dout + b * a.g.dos[0] + h * a.g.dos[1] + l * a.g.dos[2], a.g.dos[3], j, a.vec, p.Ev);
+        const float4 o4 = load4_below(p.out + b * p.os[0] + h * p.os[1] + l * p.os[2], p.os[3], j, a.vec, p.Ev);
         float s = fmaf(d4.w, o4.w, fmaf(d4.z, o4.z, fmaf(d4.y, o4.y, d4.x * o4.x)));
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(group_mask, s, o);
@@ -327,8 +345,8 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(PrepArgs a) {
         const int64_t rr = r - rows_a;
         int64_t b, hk, sidx;
         row_bhl(rr, p.S, p.Hkv, a.rows32, b, hk, sidx);
-        const float4 k4 = load4(p.k + b * p.ks[0] + hk * p.ks[1] + sidx * p.ks[2], p.ks[3], j, a.vec);
-        const float4 v4 = load4(p.v + b * p.vs[0] + hk * p.vs[1] + sidx * p.vs[2], p.vs[3], j, a.vec);
+        const float4 k4 = load4_below(p.k + b * p.ks[0] + hk * p.ks[1] + sidx * p.ks[2], p.ks[3], j, a.vec, p.E);
+        const float4 v4 = load4_below(p.v + b * p.vs[0] + hk * p.vs[1] + sidx * p.vs[2], p.vs[3], j, a.vec, p.Ev);
         split_store(a.khl, rr * DD + 4 * j, rows_b * DD, k4, a.split, a.lo_only);
         split_store(a.vhl, rr * DD + 4 * j, rows_b * DD, v4, a.split, a.lo_only);
     }
@@ -767,10 +785,10 @@ __global__ void __maxnreg__(168)
         } else if (ok && !aborted && key_ok) {
             if (half) {
                 float *dkr = a.g.dk + b * a.g.dks[0] + hk * a.g.dks[1] + key * a.g.dks[2] + (int64_t)(64 * dh) * a.g.dks[3];
-                store_row<64>(dkr, a.g.dks[3], acc, p.scale);
+                store_row_below<64>(dkr, a.g.dks[3], acc, p.scale, WIN ? p.E - 64 * dh : 64);
             } else {
                 float *dvr = a.g.dv + b * a.g.dvs[0] + hk * a.g.dvs[1] + key * a.g.dvs[2] + (int64_t)(64 * dh) * a.g.dvs[3];
-                store_row<64>(dvr, a.g.dvs[3], acc, 1.0f);
+                store_row_below<64>(dvr, a.g.dvs[3], acc, 1.0f, WIN ? p.Ev - 64 * dh : 64);
             }
         }
     }
@@ -1167,7 +1185,7 @@ __global__ void __maxnreg__(168)
         if (ok && !aborted && row_ok) {
             float *dqr = a.g.dq + b * a.g.dqs[0] + h * a.g.dqs[1] + q * a.g.dqs[2] +
                          (int64_t)(64 * dh + 32 * half) * a.g.dqs[3];
-            store_row<32>(dqr, a.g.dqs[3], acc, p.scale);
+            store_row_below<32>(dqr, a.g.dqs[3], acc, p.scale, WIN ? p.E - (64 * dh + 32 * half) : 32);
         }
     }
 
@@ -1193,6 +1211,7 @@ __global__ void __launch_bounds__(256) bwd_sink_kernel(const TcBwdArgs a) {
         for (int run = 0; run < a.sink_runs; run++)
             sum += a.sink_part[((int64_t)(run * a.sink_tiles + tile) * a.sink_units + unit) * SINK_PART + ((int64_t)half * TILE + row) * 64 + col];
         const int64_t key = k0 + row, ch = 64 * dh + col;
+        if (ch >= (half ? p.E : p.Ev)) continue;
         if (half) a.g.dk[b * a.g.dks[0] + hk * a.g.dks[1] + key * a.g.dks[2] + ch * a.g.dks[3]] += sum;
         else a.g.dv[b * a.g.dvs[0] + hk * a.g.dvs[1] + key * a.g.dvs[2] + ch * a.g.dvs[3]] += sum;
     }
@@ -1220,11 +1239,12 @@ constexpr int kSideRoleDq = 0;
 
 bool tc_backward_supported(const AttnProblem &p, const AttnGrads &g) {
     (void)g;
-    if (p.E != p.Ev || (p.E != 64 && p.E != 128)) return false;
+    // Through a window any head dims up to 128 (the pre-pass's copies are padded with zeros).
+    if (p.window ? (p.E > 128 || p.Ev > 128 || p.E == 0 || p.Ev == 0) : (p.E != p.Ev || (p.E != 64 && p.E != 128))) return false;
     if (p.L >= (1ll << 31) - TILE || p.S >= (1ll << 31) - TILE) return false;
     // 1-D grids of tiles x heads x batch (x column halves at head dim 128).
     const int64_t tiles = (max(p.L, p.S) + TILE - 1) / TILE;
-    return 2 * p.B < (1ll << 31) && tiles * p.H * p.B * (p.E / 64) < (1ll << 31);
+    return 2 * p.B < (1ll << 31) && tiles * p.H * p.B * (max(p.E, p.Ev) <= 64 ? 1 : 2) < (1ll << 31);
 }
 
 namespace {
@@ -1435,7 +1455,7 @@ int tc_backward_dd(const AttnProblem &p, const AttnGrads &g, int precision, cuda
 }  // namespace
 
 int tc_backward(const AttnProblem &p, const AttnGrads &g, int precision, cudaStream_t stream) {
-    return p.E == 64 ? tc_backward_dd<64>(p, g, precision, stream) : tc_backward_dd<128>(p, g, precision, stream);
+    return max(p.E, p.Ev) <= 64 ? tc_backward_dd<64>(p, g, precision, stream) : tc_backward_dd<128>(p, g, precision, stream);
 }
 
 }  // namespace dc

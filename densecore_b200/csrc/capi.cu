@@ -476,7 +476,7 @@ static int fill_window(AttnProblem &p, int64_t window, int64_t sinks, int64_t of
 
 size_t dc_sdpa_window_fwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
                                          int64_t head_dim, int64_t window, int64_t sinks) {
-    if (q_len != 1 || batch <= 0 || kv_heads <= 0 || heads < kv_heads || kv_len <= 0 || (head_dim != 64 && head_dim != 128))
+    if (q_len != 1 || batch <= 0 || kv_heads <= 0 || heads < kv_heads || kv_len <= 0 || head_dim <= 0 || head_dim > 256)
         return 0;
     const int splits = window_decode_splits(batch, heads, kv_heads, kv_len, window, sinks);
     return split_rows_bytes(batch * heads, splits, head_dim);

@@ -42,7 +42,8 @@ struct SplitRows {
 size_t split_rows_bytes(int64_t rows, int splits, int64_t D);
 int split_combine(const SplitRows &r, cudaStream_t stream);
 
-// One query row per sequence through a sliding window (window_decode.cu): head dim 64 or 128.
+// One query row per sequence through a sliding window (window_decode.cu): head dims up to 256, rows on
+// 16-byte boundaries.
 bool window_decode_supported(const AttnProblem &p);
 int window_decode_splits(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t window, int64_t sinks);
 int window_decode(const AttnProblem &p, const SplitRows &rows, cudaStream_t stream);

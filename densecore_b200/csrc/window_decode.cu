@@ -41,12 +41,15 @@ __device__ __forceinline__ float4 ld_stream(const float *p) {
     return r;
 }
 
-__device__ __forceinline__ void ld8(const float *p, float (&f)[8]) {
-    const float4 a = ld_stream(p), b = ld_stream(p + 4);
+// Eight channels at p, of which the first n exist (a multiple of 4, perhaps none).
+__device__ __forceinline__ void ld8(const float *p, int n, float (&f)[8]) {
+    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 a = n > 0 ? ld_stream(p) : zero, b = n > 4 ? ld_stream(p + 4) : zero;
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
     f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
 }
 
+// D: the head dim rounded up to 64, 128 or 256; the lanes past it hold zeros.
 template <int D, int G>
 __global__ void __launch_bounds__(WARPS * 32) window_decode_kernel(const AttnProblem p, const SplitRows rows) {
     constexpr int LPK = D / VEC, KPW = 32 / LPK, SLOTS = WARPS * KPW;  // lanes per key, keys per warp, per CTA
@@ -56,6 +59,7 @@ __global__ void __launch_bounds__(WARPS * 32) window_decode_kernel(const AttnPro
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31, gl = lane % LPK;
     const int slot = (threadIdx.x >> 5) * KPW + lane / LPK;
+    const int have = (int)p.E - gl * VEC;  // channels of this lane that exist
     const int chunks = (p.group + G - 1) / G;
     const int64_t b = blockIdx.z, hk = blockIdx.y / chunks;
     const int64_t h0 = hk * p.group + (int64_t)(blockIdx.y % chunks) * G;
@@ -82,7 +86,7 @@ __global__ void __launch_bounds__(WARPS * 32) window_decode_kernel(const AttnPro
         const float *qr = p.q + b * p.qs[0] + (h0 + min(g, nh - 1)) * p.qs[1] + gl * VEC;
 #pragma unroll
         for (int x = 0; x < VEC; x++) {
-            q[g][x] = qr[x] * (p.scale * LOG2E);
+            q[g][x] = x < have ? qr[x] * (p.scale * LOG2E) : 0.0f;
             acc[g][x] = 0.0f;
         }
     }
@@ -98,8 +102,8 @@ __global__ void __launch_bounds__(WARPS * 32) window_decode_kernel(const AttnPro
             ok[a] = v < v1;
             key[a] = v < sinks ? v : v + skip;
             if (ok[a]) {
-                ld8(kb + key[a] * p.ks[2], kk[a]);
-                ld8(vb + key[a] * p.vs[2], vv[a]);
+                ld8(kb + key[a] * p.ks[2], have, kk[a]);
+                ld8(vb + key[a] * p.vs[2], have, vv[a]);
             } else {
 #pragma unroll
                 for (int x = 0; x < VEC; x++) kk[a][x] = vv[a][x] = 0.0f;
@@ -153,6 +157,7 @@ __global__ void __launch_bounds__(WARPS * 32) window_decode_kernel(const AttnPro
     __syncthreads();
     for (int i = threadIdx.x; i < nh * D; i += WARPS * 32) {
         const int g = i / D, d = i % D;
+        if (d >= p.E) continue;
         float top = -INFINITY, sum = 0.0f, a = 0.0f;
 #pragma unroll
         for (int s = 0; s < SLOTS; s++) top = fmaxf(top, s_m[s][g]);
@@ -241,7 +246,7 @@ int split_combine(const SplitRows &r, cudaStream_t stream) {
 }
 
 bool window_decode_supported(const AttnProblem &p) {
-    if (p.L != 1 || p.window == 0 || p.E != p.Ev || (p.E != 64 && p.E != 128)) return false;
+    if (p.L != 1 || p.window == 0 || p.E != p.Ev || p.E % 4 || p.E == 0 || p.E > 256) return false;
     if (p.qs[3] != 1 || p.ks[3] != 1 || p.vs[3] != 1) return false;
     for (int i = 0; i < 3; i++)
         if (p.ks[i] % 4 || p.vs[i] % 4) return false;
@@ -261,7 +266,7 @@ int window_decode_splits(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t w
 }
 
 int window_decode(const AttnProblem &p, const SplitRows &rows, cudaStream_t stream) {
-    const int st = p.E == 64 ? launch_group<64>(p, rows, stream) : launch_group<128>(p, rows, stream);
+    const int st = p.E <= 64 ? launch_group<64>(p, rows, stream) : (p.E <= 128 ? launch_group<128>(p, rows, stream) : launch_group<256>(p, rows, stream));
     return st ? st : split_combine(rows, stream);
 }
 

@@ -230,3 +230,30 @@ def test_first_tokens_seen_by_many_rows(case, layout):
     runs = [torch.autograd.grad(F.sliding_window_attention(*leaves, window, sinks, offset=offset, enable_gqa=True), leaves, go)
             for _ in range(2)]
     assert all(torch.equal(x, y) for x, y in zip(*runs))
+
+
+@pytest.mark.parametrize("layout", ["plain", "bshd"])
+@pytest.mark.parametrize("dims", [(4, 4), (20, 20), (32, 32), (48, 80), (80, 48), (96, 96), (128, 32), (30, 30), (33, 64), (124, 128), (160, 64), (200, 256)])
+def test_head_dims(dims, layout):
+    e, ev = dims
+    g = torch.Generator(device="cuda").manual_seed(15)
+    r = lambda *x: torch.randn(x, generator=g, device="cuda")
+    if layout == "bshd":
+        q, k, v = r(2, 170, 4, e).transpose(1, 2), r(2, 200, 2, e).transpose(1, 2), r(2, 200, 2, ev).transpose(1, 2)
+    else:
+        q, k, v = r(2, 4, 170, e), r(2, 2, 200, e), r(2, 2, 200, ev)
+    check(q, k, v, 50, 3)
+    check(q, k, v, 50, 3, mask=torch.rand(2, 1, 170, 200, device="cuda") < 0.7)
+    # many rows behind the first tokens
+    q, k, v = r(1, 2, 1200, e), r(1, 1, 1200, e), r(1, 1, 1200, ev)
+    check(q, k, v, 20, 3)
+
+
+@pytest.mark.parametrize("d", [4, 32, 36, 80, 96, 160, 256, 33])
+def test_single_token_head_dims(d):
+    lens = torch.tensor([300, 1, 0, 299], dtype=torch.int32, device="cuda")
+    q, k, v = make(4, 6, 2, 1, 300, d, "plain", 16)
+    for i, n in enumerate(lens.tolist()):
+        k[i, :, n:], v[i, :, n:] = math.nan, math.nan
+    got = F.sliding_window_attention(q, k, v, 100, 5, lengths=lens, enable_gqa=True)
+    assert rel(got, reference(q, torch.nan_to_num(k), torch.nan_to_num(v), 100, 5, 0, lens=lens)) <= 1e-5
