@@ -49,6 +49,18 @@ std::string shape_str(const dc_tensor_t *t) {
     return s + ")";
 }
 
+bool usable(const dc_tensor_t *t) {
+    if (!t || t->ndim < 0 || t->ndim > 4) return false;
+    int64_t n = 1;
+    for (int i = 0; i < t->ndim; i++) {
+        if (t->sizes[i] < 0) return false;
+        n = t->sizes[i] == 0 ? 0 : n;
+    }
+    const int dt = t->dtype;
+    const uintptr_t size = dt == DC_F64 || dt == DC_I64 ? 8 : (dt == DC_F16 || dt == DC_BF16 ? 2 : (dt == DC_BOOL ? 1 : 4));
+    return n == 0 || (t->data && (reinterpret_cast<uintptr_t>(t->data) & (size - 1)) == 0);
+}
+
 int device_ok() {
     int n = 0;
     cudaError_t e = cudaGetDeviceCount(&n);
@@ -462,11 +474,11 @@ static int fill_window(AttnProblem &p, int64_t window, int64_t sinks, int64_t of
     if (offset > far || offset < -far)
         return fail(DC_ERR_VALUE, "sliding window attention: the offset must lie within 2^32 of 0");
     p.causal = 0;
-    p.window = window < far ? window : far;
+    p.window = window < far ? window : far;  // (lengths are below 2^31)
     p.sinks = sinks < far ? sinks : far;
     p.offset = offset;
     if (!lengths) return DC_OK;
-    if (lengths->dtype != DC_I32 || lengths->ndim != 1 || lengths->sizes[0] != p.B)
+    if (!usable(lengths) || lengths->dtype != DC_I32 || lengths->ndim != 1 || lengths->sizes[0] != p.B)
         return fail(DC_ERR_VALUE, "sliding window attention: lengths must be int32 (B)");
     if (p.L != 1) return fail(DC_ERR_VALUE, "sliding window attention: lengths take a query length of 1");
     p.lens = static_cast<const int32_t *>(lengths->data);
@@ -490,6 +502,8 @@ int dc_sdpa_window_fwd(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tens
     int st = fill_problem(q, k, v, 0, has_scale, scale, p);
     if (!st) st = fill_mask(mask, p);
     if (!st) st = fill_window(p, window, sinks, offset, lengths);
+    if (!st && !(usable(q) && usable(k) && usable(v) && (!mask || usable(mask)) && usable(out) && usable(lse)))
+        st = fail(DC_ERR_VALUE, "sliding window attention: a tensor is null or not aligned to its type");
     if (!st) st = check_out(out, lse, p);
     if (!st) st = check_precision(precision);
     if (st) return st;

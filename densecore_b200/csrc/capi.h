@@ -12,6 +12,10 @@ namespace dc {
 // "(2, 3)" of a tensor, for messages.
 std::string shape_str(const dc_tensor_t *t);
 
+// Whether a view can be followed: sizes not negative, memory where there are elements, on a boundary of
+// their type (a kernel's access elsewhere would fault).
+bool usable(const dc_tensor_t *t);
+
 // DC_OK when there is a CUDA device.
 int device_ok();
 
@@ -31,6 +35,7 @@ struct ScopedWorkspace {
         stream = s;
         if (need == 0) return DC_OK;
         if (given) {
+            if (reinterpret_cast<uintptr_t>(given) & 3u) return fail(DC_ERR_VALUE, std::string(what) + ": must be 4-byte aligned");
             if (given_bytes < need)
                 return fail(DC_ERR_VALUE, std::string(what) + ": workspace of " +
                                               std::to_string(given_bytes) + " bytes, " +

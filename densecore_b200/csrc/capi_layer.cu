@@ -35,7 +35,8 @@ bool overlaps(const dc_tensor_t *t) {
 int fill_rotary(const char *what, const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *positions,
                 const dc_tensor_t *inv_freq, double amplitude, RotaryArgs &a) {
     const std::string name(what);
-    if (!q || !positions || !inv_freq) return fail(DC_ERR_VALUE, name + ": queries, positions and frequencies are required");
+    if (!usable(q) || (k && !usable(k)) || !usable(positions) || !usable(inv_freq))
+        return fail(DC_ERR_VALUE, name + ": queries, positions and frequencies are required, aligned to their types");
     if (q->ndim != 4 || !is_float(q->dtype)) return fail(DC_ERR_VALUE, name + " takes (B, H, L, D) float32, float16 or bfloat16 tensors");
     const int64_t B = q->sizes[0], L = q->sizes[2], D = q->sizes[3];
     if (k && (k->ndim != 4 || k->dtype != q->dtype || k->sizes[0] != B || k->sizes[2] != L || k->sizes[3] != D))
@@ -66,7 +67,7 @@ int fill_rotary(const char *what, const dc_tensor_t *q, const dc_tensor_t *k, co
 }
 
 int fill_operand(const char *what, RotaryOperand &o, const dc_tensor_t *x, dc_tensor_t *y) {
-    if (!y || y->dtype != x->dtype || !same_sizes(x, y) || overlaps(y))
+    if (!usable(y) || y->dtype != x->dtype || !same_sizes(x, y) || overlaps(y))
         return fail(DC_ERR_VALUE, std::string(what) + ": outputs must have the inputs' shape and type");
     o.x = x->data;
     o.y = y->data;
@@ -77,7 +78,7 @@ int fill_operand(const char *what, RotaryOperand &o, const dc_tensor_t *x, dc_te
 }
 
 int fill_weight(const char *what, const dc_tensor_t *w, int dtype, int64_t D) {
-    if (w && (w->ndim != 1 || w->sizes[0] != D || (w->dtype != DC_F32 && w->dtype != dtype)))
+    if (w && (!usable(w) || w->ndim != 1 || w->sizes[0] != D || (w->dtype != DC_F32 && w->dtype != dtype)))
         return fail(DC_ERR_VALUE, std::string(what) + ": weights must be (head dim), float32 or of the inputs' type");
     return DC_OK;
 }
@@ -102,11 +103,11 @@ int fill_cache(const dc_cache4_t *cache, Cache4 &c) {
 }
 
 int fill_table(const dc_tensor_t *table, Cache4Args &a) {
-    if (!table || table->dtype != DC_I32 || table->ndim != 2) return fail(DC_ERR_VALUE, "cache: the page table must be int32 (B, pages)");
+    if (!usable(table) || table->dtype != DC_I32 || table->ndim != 2) return fail(DC_ERR_VALUE, "cache: the page table must be int32 (B, pages)");
     a.B = table->sizes[0];
     a.P = table->sizes[1];
     if (a.B > 65535) return fail(DC_ERR_UNSUPPORTED, "cache: more than 65535 sequences in one call");
-    if (a.P * a.c.page_size >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "cache: page tables of 2^31 positions and more");
+    if (a.P >= (1ll << 31) || a.P * a.c.page_size >= (1ll << 31)) return fail(DC_ERR_UNSUPPORTED, "cache: page tables of 2^31 positions and more");
     a.table = static_cast<const int32_t *>(table->data);
     a.ts[0] = table->strides[0];
     a.ts[1] = table->strides[1];
@@ -114,7 +115,7 @@ int fill_table(const dc_tensor_t *table, Cache4Args &a) {
 }
 
 int fill_counts(const dc_tensor_t *t, int64_t B, const char *what, const int32_t *&ptr, int64_t &stride) {
-    if (!t || t->dtype != DC_I32 || t->ndim != 1 || t->sizes[0] != B)
+    if (!usable(t) || t->dtype != DC_I32 || t->ndim != 1 || t->sizes[0] != B)
         return fail(DC_ERR_VALUE, std::string("cache: ") + what + " must be int32 (B)");
     ptr = static_cast<const int32_t *>(t->data);
     stride = t->strides[0];
@@ -185,7 +186,7 @@ int dc_qk_norm_rotary_bwd(const dc_tensor_t *q_grad, const dc_tensor_t *k_grad, 
     dc_tensor_t *gws[2] = {q_weight_grad, k_weight_grad};
     for (int i = 0; i < 2 && !st && xs[i]; i++) {
         RotaryOperand &o = a.op[i];
-        if (!gs[i] || gs[i]->dtype != q->dtype || !same_sizes(gs[i], xs[i])) {
+        if (!usable(gs[i]) || gs[i]->dtype != q->dtype || !same_sizes(gs[i], xs[i])) {
             st = fail(DC_ERR_VALUE, "normed rotary backward: gradients must have the inputs' shape and type");
             break;
         }
@@ -223,7 +224,7 @@ int dc_cache4_append(const dc_cache4_t *cache, const dc_tensor_t *key, const dc_
     if (!st) st = fill_counts(start, a.B, "start positions", a.starts, a.starts_stride);
     if (!st && end) st = fill_counts(end, a.B, "end positions", a.ends, a.ends_stride);
     if (st) return st;
-    if (!key || !value || key->ndim != 4 || !is_float(key->dtype) || value->dtype != key->dtype || !same_sizes(key, value) ||
+    if (!usable(key) || !usable(value) || key->ndim != 4 || !is_float(key->dtype) || value->dtype != key->dtype || !same_sizes(key, value) ||
         key->sizes[0] != a.B || key->sizes[1] != a.c.Hkv || key->sizes[3] != a.c.D)
         return fail(DC_ERR_VALUE, "cache append: keys and values must be (B, kv heads, T, head dim) of one float type");
     a.T = key->sizes[2];
@@ -245,7 +246,7 @@ int dc_cache4_read(const dc_cache4_t *cache, const dc_tensor_t *page_table, cons
     if (!st) st = fill_table(page_table, a);
     if (!st) st = fill_counts(lengths, a.B, "lengths", a.lens, a.lens_stride);
     if (st) return st;
-    if (!key || !value || key->ndim != 4 || key->dtype != DC_F32 || value->dtype != DC_F32 || !same_sizes(key, value) ||
+    if (!usable(key) || !usable(value) || key->ndim != 4 || key->dtype != DC_F32 || value->dtype != DC_F32 || !same_sizes(key, value) ||
         key->sizes[0] != a.B || key->sizes[1] != a.c.Hkv || key->sizes[3] != a.c.D || overlaps(key) || overlaps(value))
         return fail(DC_ERR_VALUE, "cache read: keys and values must be float32 (B, kv heads, T, head dim)");
     a.T = key->sizes[2];
@@ -273,12 +274,12 @@ int dc_cache4_attention(const dc_cache4_t *cache, const dc_tensor_t *q, const dc
     if (!st) st = fill_table(page_table, a);
     if (!st) st = fill_counts(lengths, a.B, "lengths", a.lens, a.lens_stride);
     if (st) return st;
-    if (!q || q->ndim != 4 || !is_float(q->dtype) || q->sizes[0] != a.B || q->sizes[2] != 1 || q->sizes[3] != a.c.D ||
+    if (!usable(q) || q->ndim != 4 || !is_float(q->dtype) || q->sizes[0] != a.B || q->sizes[2] != 1 || q->sizes[3] != a.c.D ||
         q->sizes[1] % a.c.Hkv)
         return fail(DC_ERR_VALUE, "cache attention: queries must be (B, H, 1, head dim), H a multiple of the cache's heads");
-    if (!out || out->dtype != q->dtype || !same_sizes(out, q) || overlaps(out))
+    if (!usable(out) || out->dtype != q->dtype || !same_sizes(out, q) || overlaps(out))
         return fail(DC_ERR_VALUE, "cache attention: the output must have the queries' shape and type");
-    if (!lse || lse->dtype != DC_F32 || lse->ndim != 3 || lse->sizes[0] != a.B || lse->sizes[1] != q->sizes[1] || lse->sizes[2] != 1)
+    if (!usable(lse) || lse->dtype != DC_F32 || lse->ndim != 3 || lse->sizes[0] != a.B || lse->sizes[1] != q->sizes[1] || lse->sizes[2] != 1)
         return fail(DC_ERR_VALUE, "cache attention: the logsumexp must be float32 (B, H, 1)");
     if (window < 0 || sinks < 0) return fail(DC_ERR_VALUE, "cache attention: window and sinks must not be negative");
     a.H = q->sizes[1];

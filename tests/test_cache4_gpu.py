@@ -261,3 +261,42 @@ def test_cache_of_more_than_four_gigabytes():
     cache.append(x, x, table, i32(0))
     assert torch.equal(cache.read(table, i32(300), 300)[1], define(x))
     check(cache, table, torch.randn(1, 8, 1, dim, device="cuda"), i32(300))
+
+
+def test_empty_calls():
+    cache, table = fill(2, 2, 64, 64, 16)
+    none = torch.empty(2, 0, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 4, 1, 64, device="cuda")
+    out, lse = cache.attention(q, none, i32(0, 0), return_lse=True)
+    assert (out == 0).all() and (lse == 0).all() and status() == 0
+    assert (cache.attention(q, none, i32(3, 0)) == 0).all() and status() == 3
+    x = torch.randn(2, 2, 0, 64, device="cuda")
+    cache.append(x, x, table, i32(0, 0))
+    assert cache.read(table, i32(64, 64), 0)[0].shape == (2, 2, 0, 64)
+    empty = torch.empty(0, 4, dtype=torch.int32, device="cuda")
+    assert cache.attention(q[:0], empty, i32()).shape == (0, 4, 1, 64)
+    assert (cache.read(table, i32(0, 5), 200)[1][0] == 0).all() and status() == 0
+
+
+def test_two_threads_at_once():
+    # Host threads on streams of their own, each with its cache.
+    import threading
+    sets = [fill(2, 2, 500, 128, 16, seed=s) for s in (1, 2)]
+    q = torch.randn(2, 8, 1, 128, device="cuda")
+    lens = i32(500, 77)
+    want = [c.attention(q, t, lens) for c, t in sets]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got[i] = sets[i][0].attention(q, sets[i][1], lens)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert not errors and all(torch.equal(a, b) for a, b in zip(got, want))

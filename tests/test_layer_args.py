@@ -173,7 +173,8 @@ def test_c_entry_points_refuse_before_any_device_work():
         return L.dc_sdpa_window_fwd(r(q), r(k), r(k), r(mask), window, sinks, offset, r(lens), 0, 0.0, 0, r(out), r(lse),
                                     None, 0, None)
 
-    for kw in (dict(window=0), dict(sinks=-1), dict(offset=1 << 40), dict(lens=fake((2,), _lib.DC_I32)),
+    for kw in (dict(window=0), dict(sinks=-1), dict(offset=1 << 40), dict(q=fake((2, 4, 8, 64), ptr=0x10001)), dict(out=fake((2, 4, 8, 64), ptr=0)),
+               dict(lens=fake((2,), _lib.DC_I32, ptr=0), q=fake((2, 4, 1, 64)), out=fake((2, 4, 1, 64)), lse=fake((2, 4, 1))), dict(lens=fake((2,), _lib.DC_I32)),
                dict(mask=fake((3, 9), _lib.DC_BOOL)), dict(out=fake((2, 4, 8, 32))), dict(q=fake((2, 4, 8, 64), _lib.DC_BF16))):
         assert window(**kw) == _lib.DC_ERR_VALUE, kw
     pos, freq = fake((8,), _lib.DC_I64), fake((32,), _lib.DC_F64)
@@ -189,6 +190,10 @@ def test_c_entry_points_refuse_before_any_device_work():
     assert rotary(k=fake((2, 4, 7, 64)), kout=fake((2, 4, 7, 64))) == _lib.DC_ERR_VALUE
     odd = fake((2, 4, 8, 63))
     assert rotary(q=odd, out=odd, freq=fake((4,), _lib.DC_F64)) == _lib.DC_ERR_UNSUPPORTED
+    assert rotary(q=fake((2, 4, 8, 64), ptr=0)) == _lib.DC_ERR_VALUE  # no memory
+    assert rotary(q=fake((2, 4, 8, 64), ptr=0x10002)) == _lib.DC_ERR_VALUE  # off its type's boundary
+    negative = fake((-2, 4, -8, 64))
+    assert rotary(q=negative, out=negative, pos=fake((-8,), _lib.DC_I64)) == _lib.DC_ERR_VALUE
     spread = fake((2, 4, 8, 64))
     spread.strides[1] = 0  # an output whose heads share memory
     assert rotary(out=spread) == _lib.DC_ERR_VALUE
@@ -201,7 +206,7 @@ def test_c_entry_points_refuse_before_any_device_work():
     for kw in (dict(cache=_lib.DcCache4(0, 4, 2, 64, 16)), dict(cache=_lib.DcCache4(0x10004, 4, 2, 64, 16)),
                dict(cache=_lib.DcCache4(0x10000, 4, 2, 64, 20)), dict(q=fake((2, 3, 1, 64))),
                dict(q=fake((2, 4, 2, 64))), dict(table=fake((2, 3), _lib.DC_I64)), dict(n=fake((3,), _lib.DC_I32)),
-               dict(window=-1), dict(out=fake((2, 4, 1, 64), _lib.DC_BF16)), dict(lse=fake((2, 4)))):
+               dict(window=-1), dict(table=fake((2, 3), _lib.DC_I32, ptr=0)), dict(out=fake((2, 4, 1, 64), _lib.DC_BF16)), dict(lse=fake((2, 4)))):
         assert attention(**kw) == _lib.DC_ERR_VALUE, kw
     assert attention(cache=_lib.DcCache4(0x10000, 4, 2, 96, 16)) == _lib.DC_ERR_UNSUPPORTED
     assert attention(table=fake((2, 1 << 28), _lib.DC_I32)) == _lib.DC_ERR_UNSUPPORTED

@@ -226,3 +226,28 @@ def test_in_place_and_streams():
     assert torch.equal(q, ref)
     assert dc._lib.load().dc_device_status(0) == 0
     assert math.isfinite(float(q.sum()))
+
+
+def test_nothing_to_turn_and_infinities_that_pass_through():
+    q = torch.randn(1, 2, 3, 64, device="cuda")
+    q[0, 0, 0, 40] = math.inf
+    pos = torch.arange(3, device="cuda")
+    none = torch.empty(0, dtype=torch.float64, device="cuda")
+    assert torch.equal(F.rotary_embedding(q, None, pos, none, amplitude=2.0)[0], q)
+    freq, _ = F.rotary_frequencies(32, device="cuda")
+    y, _ = F.rotary_embedding(q, None, pos, freq)
+    assert torch.equal(y[..., 32:], q[..., 32:])
+
+
+def test_more_than_two_to_the_31_elements():
+    if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
+        pytest.skip("needs memory")
+    l, h, d = 560_000, 32, 128  # 2.3e9 elements
+    x = torch.empty(1, l, h, d, dtype=torch.bfloat16, device="cuda").normal_()
+    freq, _ = F.rotary_frequencies(d, device="cuda")
+    pos = torch.arange(l, device="cuda")
+    y, _ = F.rotary_embedding(x.transpose(1, 2), None, pos, freq)
+    tail, _ = F.rotary_embedding(x[:, -5:].transpose(1, 2).contiguous(), None, pos[-5:], freq)
+    assert torch.equal(y[:, :, -5:], tail)
+    head, _ = F.rotary_embedding(x[:, :5].transpose(1, 2).contiguous(), None, pos[:5], freq)
+    assert torch.equal(y[:, :, :5], head)

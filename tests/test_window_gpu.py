@@ -75,7 +75,8 @@ CASES = [  # b, h, kv, l, s, d, window, sinks, offset
     (1, 1, 1, 50, 50, 64, 10, 2, -200), (1, 1, 1, 50, 50, 64, 10, 2, 400), (1, 1, 1, 50, 50, 64, 10, 0, 400),
     (1, 2, 2, 130, 130, 64, 10 ** 12, 0, None), (1, 1, 1, 130, 130, 64, 7, 10 ** 12, None), (1, 8, 1, 70, 333, 64, 90, 64, None),
     (1, 2, 2, 40, 40, 32, 9, 3, None), (1, 2, 1, 75, 130, 20, 17, 40, None), (1, 1, 1, 33, 70, 256, 12, 3, None),
-    (1, 2, 2, 1, 500, 64, 100, 4, None), (2, 4, 2, 1, 500, 128, 100, 4, None)]
+    (1, 2, 2, 1, 500, 64, 100, 4, None), (2, 4, 2, 1, 500, 128, 100, 4, None), (1, 2, 2, 1, 500, 64, 100, 4, 700),
+    (1, 2, 2, 1, 500, 64, 100, 4, 520), (1, 2, 1, 1, 500, 64, 100, 4, -3), (1, 2, 1, 1, 500, 64, 100, 0, 499)]
 
 
 @pytest.mark.parametrize("layout", ["plain", "bshd", "odd"])
@@ -257,3 +258,42 @@ def test_single_token_head_dims(d):
         k[i, :, n:], v[i, :, n:] = math.nan, math.nan
     got = F.sliding_window_attention(q, k, v, 100, 5, lengths=lens, enable_gqa=True)
     assert rel(got, reference(q, torch.nan_to_num(k), torch.nan_to_num(v), 100, 5, 0, lens=lens)) <= 1e-5
+
+
+def test_ragged_single_tokens_with_masks():
+    lens = torch.tensor([300, 1, 0, 150], dtype=torch.int32, device="cuda")
+    q, k, v = make(4, 4, 2, 1, 300, 64, "plain", 17)
+    bias = torch.randn(4, 1, 1, 300, device="cuda")
+    hide = torch.rand(4, 4, 1, 300, device="cuda") < 0.5
+    for mask in (bias, hide):
+        got = F.sliding_window_attention(q, k, v, 100, 5, attn_mask=mask, lengths=lens, enable_gqa=True)
+        assert rel(got, reference(q, k, v, 100, 5, 0, mask, lens=lens)) <= 1e-5
+
+
+def test_broadcast_keys_get_summed_gradients():
+    # Keys and values shared by every sequence of the batch: views without a batch stride.
+    q = torch.randn(3, 2, 90, 64, device="cuda", requires_grad=True)
+    k = torch.randn(1, 2, 90, 64, device="cuda", requires_grad=True)
+    v = torch.randn(1, 2, 90, 64, device="cuda", requires_grad=True)
+    out = F.sliding_window_attention(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1), 20, 2)
+    go = torch.randn_like(out)
+    got = torch.autograd.grad(out, (q, k, v), go)
+    refs = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    ro = reference(refs[0], refs[1].expand(3, -1, -1, -1), refs[2].expand(3, -1, -1, -1), 20, 2, 0)
+    for a, r in zip((out, *got), (ro, *torch.autograd.grad(ro, refs, go.double()))):
+        assert rel(a.detach(), r.detach()) <= 1e-5
+
+
+def test_long_cache_past_two_to_the_32_bytes():
+    if torch.cuda.get_device_properties(0).total_memory < 60 << 30:
+        pytest.skip("needs memory")
+    s = 9_000_000  # 4.6 GB each
+    k = torch.zeros(1, 1, s, 128, device="cuda")
+    v = torch.zeros(1, 1, s, 128, device="cuda")
+    k[:, :, -200:].normal_(), v[:, :, -200:].normal_(), k[:, :, :4].normal_(), v[:, :, :4].normal_()
+    q = torch.randn(1, 2, 1, 128, device="cuda")
+    got = F.sliding_window_attention(q, k, v, 150, 4, enable_gqa=True)
+    kk, vv = (torch.cat((t[:, :, :4], t[:, :, -150:]), 2) for t in (k, v))
+    assert rel(got, reference(q, kk, vv, 1000, 0, 153)) <= 1e-5
+    two = F.sliding_window_attention(torch.cat((q, q), 2), k, v, 150, 4, enable_gqa=True)[:, :, 1:]
+    assert rel(two, reference(q, kk, vv, 1000, 0, 153)) <= 1e-5
