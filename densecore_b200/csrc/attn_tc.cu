@@ -111,6 +111,7 @@ struct TcFwdArgs {
     int64_t group_heads;  // (batch, head) pairs whose tiles are ordered together (their K / V fit in L2)
     float scale_log2;
     int *err;
+    const int *when;  // persistent windows: null, or zero for a kernel that has nothing to do
 };
 
 // tcgen05.ld / st of 16 or 32 consecutive columns of this thread's lane.
@@ -445,7 +446,7 @@ __global__ void __maxnreg__(128)
             // Interior blocks keep the raw scores and fold the scale into the exponent's FFMA
             // (the max commutes with a positive scale); edge blocks scale, mask and fill first.
             const bool raw = !edge && a.scale_log2 > 0.0f;
-            const float smul = raw ? a.scale_log2 : 1.0f;
+            float smul = raw ? a.scale_log2 : 1.0f;
             if (!raw) {
 #pragma unroll
                 for (int c = 0; c < C::HB; c++) {
@@ -470,6 +471,15 @@ __global__ void __maxnreg__(128)
             if (rescale) {
                 corr = ex2_approx(m - m_new);
                 m = m_new;
+            }
+            if constexpr (WIN) {
+                // The FFMA does not round s smul, the maximum is rounded: past 2^20 a difference of up to
+                // half an ulp counts (past 2^31 its power overflows), so the scores are rounded too.
+                if (smul != 1.0f && fabsf(m) > 0x1p20f) {
+#pragma unroll
+                    for (int c = 0; c < C::HB; c++) s[c] *= smul;
+                    smul = 1.0f;
+                }
             }
             const bool dead = (m == -INFINITY);
             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // four partial row sums: shorter chains
@@ -612,6 +622,9 @@ template <class C, bool SPLIT, bool MASKED, bool DROP, bool WIN>
 __global__ void __maxnreg__(128)
     attn_fwd_tc_persist_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                        const __grid_constant__ CUtensorMap tmv, const TcFwdArgs a) {
+    if constexpr (WIN) {
+        if (a.when && *a.when == 0) return;
+    }
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     const uint32_t sb = (raw + 1023u) & ~1023u;
@@ -932,7 +945,7 @@ __global__ void __maxnreg__(128)
                 // Interior blocks keep the raw scores and fold the scale into the exponent's FFMA
                 // (the max commutes with a positive scale); edge blocks scale, mask and fill first.
                 const bool rawp = !edge && a.scale_log2 > 0.0f;
-                const float smul = rawp ? a.scale_log2 : 1.0f;
+                float smul = rawp ? a.scale_log2 : 1.0f;
                 if (!rawp) {
 #pragma unroll
                     for (int c = 0; c < C::HB; c++) {
@@ -954,6 +967,15 @@ __global__ void __maxnreg__(128)
                 if (rescale) {
                     corr = ex2_approx(m - m_new);
                     m = m_new;
+                }
+                if constexpr (WIN) {
+                    // The FFMA does not round s smul, the maximum is rounded: past 2^20 a difference of up to
+                    // half an ulp counts (past 2^31 its power overflows), so the scores are rounded too.
+                    if (smul != 1.0f && fabsf(m) > 0x1p20f) {
+#pragma unroll
+                        for (int c = 0; c < C::HB; c++) s[c] *= smul;
+                        smul = 1.0f;
+                    }
                 }
                 const bool dead = (m == -INFINITY);
                 float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // four partial row sums: shorter chains
@@ -1089,7 +1111,7 @@ decltype(&attn_fwd_tc_kernel<C, true, true, true, false>) pick_fwd(bool split, b
 }
 
 template <class C>
-int launch_fwd(const AttnProblem &p, int split, cudaStream_t stream) {
+int launch_fwd(const AttnProblem &p, int split, cudaStream_t stream, const int *when = nullptr) {
     CUtensorMap tq, tk, tv;
     int st = make_tmap(&tq, p.q, p.E, p.L, p.H, p.B, p.qs, C::BM);
     if (!st) st = make_tmap(&tk, p.k, p.E, p.S, p.Hkv, p.B, p.ks, C::BN);
@@ -1104,6 +1126,7 @@ int launch_fwd(const AttnProblem &p, int split, cudaStream_t stream) {
     if (!a.err) return fail(DC_ERR_CUDA, "device error word is unavailable");
     const bool masked = p.mask_kind != MASK_NONE;
     const bool drop = p.keep != nullptr;
+    a.when = when;
     a.num_tiles = (int64_t)a.num_q_tiles * p.H * p.B;
     // Groups of heads whose K and V (S * (E + Ev) floats each) fit in about 48 MB, within one of
     // the L2's two 63 MB partitions (at 67 MB, two of config 4's heads, the forward measured
@@ -1118,7 +1141,7 @@ int launch_fwd(const AttnProblem &p, int split, cudaStream_t stream) {
     // (A window's tiles hold at most its keys, the tile's own and the sinks, each rounded up.)
     int64_t tile_keys = p.S;
     if (p.window) tile_keys = min(p.S, min(p.window, p.S) + C::BM + C::BN + min(p.sinks, p.S) + C::BN);
-    const bool persistent = (tile_keys + C::BN - 1) / C::BN <= 64 && a.num_tiles < (1ll << 31);
+    const bool persistent = when || ((tile_keys + C::BN - 1) / C::BN <= 64 && a.num_tiles < (1ll << 31));
     const int64_t ctas = persistent && a.num_tiles > sms ? sms : a.num_tiles;
     const bool win = p.window != 0;
     auto kernel = persistent ? pick_fwd<C, true>(split, masked, drop, win) : pick_fwd<C, false>(split, masked, drop, win);
@@ -1158,6 +1181,10 @@ bool tc_forward_supported(const AttnProblem &p) {
 int tc_forward(const AttnProblem &p, int precision, cudaStream_t stream) {
     const int split = precision == DC_PREC_TF32 ? 0 : 1;
     return max(p.E, p.Ev) <= 64 ? launch_fwd<Fwd64>(p, split, stream) : launch_fwd<Fwd128>(p, split, stream);
+}
+
+int tc_forward_if(const AttnProblem &p, const int *when, cudaStream_t stream) {
+    return launch_fwd<Fwd128>(p, 1, stream, when);
 }
 
 int device_error(int reset) {

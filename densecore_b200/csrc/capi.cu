@@ -514,7 +514,10 @@ int dc_sdpa_window_fwd(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tens
     if (p.B == 0 || p.H == 0 || p.L == 0) return DC_OK;
     if ((st = device_ok())) return st;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (precision != DC_PREC_FP32 && !p.lens && p.L > 1 && tc_forward_supported(p)) return tc_forward(p, precision, s);
+    if (!p.lens && p.L > 1) {
+        if (precision == DC_PREC_3XTF32 && window_forward_pick(p)) return window_forward(p, s);
+        if (precision != DC_PREC_FP32 && tc_forward_supported(p)) return tc_forward(p, precision, s);
+    }
     if (!window_decode_supported(p) || p.S == 0) return simt_forward(p, s);
     SplitRows rows{};
     rows.splits = window_decode_splits(p.B, p.H, p.Hkv, p.S, p.window, p.sinks);

@@ -27,6 +27,13 @@ int decode_pick_splits(const AttnProblem &p);
 size_t decode_workspace_bytes(int64_t B, int64_t H, int64_t Ev, int splits);
 int decode_forward(const AttnProblem &p, int splits, void *workspace, cudaStream_t stream);
 
+// Sliding-window forward on the 16-bit tensor cores (attn_win.cu): of what tc_forward takes, the calls with
+// a head dim above 64 that see enough keys to pay for the packing.
+bool window_forward_pick(const AttnProblem &p);
+int window_forward(const AttnProblem &p, cudaStream_t stream);
+// tc_forward (3xTF32, a window, a head dim above 64) if *when, in device memory, is not zero.
+int tc_forward_if(const AttnProblem &p, const int *when, cudaStream_t stream);
+
 // Rows whose keys are split over CTAs (window_decode.cu, cache4.cu): row (b, h) of out (B, H, 1, D)
 // and lse (B, H, 1). With one split the CTA writes its row; otherwise the partial results go to
 // `part` -- per row and split D accumulators, the maximum in base 2 and the sum, both relative to

@@ -16,4 +16,9 @@ bool tma_stride_ok(int64_t size, int64_t stride);
 int make_tmap(CUtensorMap *m, const float *base, int64_t D, int64_t rows, int64_t heads, int64_t batch,
               const int64_t *st, int box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
+// The same of 16-bit floats (contiguous copies of the library's own): the box is 64 of them (128 bytes)
+// by box_rows rows, with the 128-byte swizzle.
+int make_tmap_16bit(CUtensorMap *m, const void *base, int64_t D, int64_t rows, int64_t heads, int64_t batch, const int64_t *st,
+                    int box_rows);
+
 }  // namespace dc

@@ -297,3 +297,181 @@ def test_long_cache_past_two_to_the_32_bytes():
     assert rel(got, reference(q, kk, vv, 1000, 0, 153)) <= 1e-5
     two = F.sliding_window_attention(torch.cat((q, q), 2), k, v, 150, 4, enable_gqa=True)[:, :, 1:]
     assert rel(two, reference(q, kk, vv, 1000, 0, 153)) <= 1e-5
+
+
+# ---- long windows at head dims above 64: pairs of fp16 (22 bits, rounded to nearest, at most 2^-22 of an
+# operand, so a few 2^-22 of a score's absolute terms), tighter than the TF32 pairs of the bar above.
+def ran(f):
+    """The kernels that f() launched."""
+    dc._lib.kernel_timing(True)
+    dc._lib.kernel_timing_report(True)
+    f()
+    torch.cuda.synchronize()
+    names = set(dc._lib.kernel_timing_report(True))
+    dc._lib.kernel_timing(False)
+    return names
+
+
+LONG = [  # b, h, kv, l, s, e, ev, window, sinks, offset
+    (1, 2, 2, 1400, 1400, 128, 128, 10 ** 12, 0, None), (2, 2, 2, 2000, 2000, 128, 128, 700, 4, None),
+    (1, 4, 1, 700, 700, 128, 128, 333, 0, None), (1, 4, 2, 900, 900, 96, 128, 800, 70, None),
+    (1, 2, 2, 1283, 1283, 68, 100, 1283, 3, None), (1, 2, 2, 1301, 1301, 128, 4, 1200, 0, None),
+    (1, 8, 1, 129, 1999, 128, 128, 1500, 5, None), (1, 8, 1, 37, 640, 80, 80, 600, 0, None),
+    (1, 4, 1, 128, 704, 128, 128, 700, 1, 500), (1, 2, 2, 1500, 1500, 128, 128, 1400, 0, 300),
+    (1, 8, 1, 2, 65, 128, 128, 10 ** 12, 0, 4000), (1, 3, 1, 1100, 1100, 72, 124, 1000, 900, None),
+    (1, 4, 1, 900, 900, 128, 128, 633, 1, None), (1, 32, 1, 37, 640, 80, 80, 600, 0, None),
+    (1, 8, 1, 128, 704, 128, 128, 700, 1, 500), (1, 64, 1, 70, 300, 128, 128, 280, 2, None)]
+
+
+def pays(l, s, h, kv, window, offset):
+    """Whether a mean row sees 192 keys and 384 more per key row that is packed for it."""
+    first = (s - l if offset is None else offset) + 1
+    mean = sum(min(first + i, window, s) for i in range(l)) / l
+    return mean * l * h >= 192 * l * h + 384 * s * kv
+
+
+@pytest.mark.parametrize("layout", ["plain", "bshd"])
+@pytest.mark.parametrize("case", LONG)
+def test_long_windows_above_64_columns(case, layout):
+    b, h, kv, l, s, e, ev, window, sinks, offset = case
+    q, k, v = make(b, h, kv, l, s, 128, layout, 20)
+    q, k, v = q[..., :e], k[..., :e], v[..., :ev]
+    names = ran(lambda: F.sliding_window_attention(q, k, v, window, sinks, offset=offset, enable_gqa=True))
+    assert ("window_attend" in names) == pays(l, s, h, kv, window, offset)
+    check(q, k, v, window, sinks, offset)
+
+
+@pytest.mark.parametrize("kind", ["padding", "left", "rows", "bias", "lowest", "full", "strided"])
+def test_long_windows_masks(kind):
+    b, h, s = 2, 2, 1400
+    q, k, v = make(b, h, h, s, s, 128, "bshd", 21)
+    j = torch.arange(s, device="cuda")
+    mask = {
+        "padding": lambda: (j < torch.tensor([1300, 60], device="cuda")[:, None])[:, None, None],
+        "left": lambda: (j >= torch.tensor([700, 0], device="cuda")[:, None])[:, None, None],  # empty first rows
+        "rows": lambda: (j % 3 != 0)[:, None].expand(s, s),  # every third row empty
+        "bias": lambda: torch.randn(1, h, s, s, device="cuda"),
+        "lowest": lambda: torch.where(j % 2 == 0, torch.finfo(torch.float32).min, 0.5).expand(1, 1, s, s).clone(),
+        "full": lambda: torch.rand(b, h, s, s, device="cuda") < 0.5,
+        "strided": lambda: torch.randn(s, 2 * s + 1, device="cuda")[:, 1::2],
+    }[kind]()
+    call = lambda: F.sliding_window_attention(q, k, v, 1300, 2, attn_mask=mask)
+    assert "window_attend" in ran(call)
+    out, grads = check(q, k, v, 1300, 0 if kind == "left" else 2, mask=mask)
+    if kind == "rows":
+        assert (out[:, :, ::3] == 0).all() and (grads[0][:, :, ::3] == 0).all()
+    if kind == "lowest":
+        low = torch.full((s, s), torch.finfo(torch.float32).min, device="cuda")
+        assert (F.sliding_window_attention(q, k, v, 1300, attn_mask=low) == 0).all()
+
+
+def test_long_windows_hidden_keys_may_hold_anything():
+    s = 1400
+    q, k, v = make(1, 2, 2, s, s, 128, "plain", 22)
+    hide = torch.zeros(s, dtype=torch.bool, device="cuda")
+    hide[10:30] = True
+    hide[640:704] = True  # a whole tile of keys
+    bad = k.clone()
+    bad[:, :, 10:20], bad[:, :, 20:30], bad[:, :, 640:704] = math.nan, math.inf, math.nan
+    clean = F.sliding_window_attention(q, k, v, 1300, 4, attn_mask=~hide.expand(s, s))
+    assert rel(F.sliding_window_attention(q, bad, v, 1300, 4, attn_mask=~hide.expand(s, s)), clean.double()) <= 1e-6
+    minus = torch.where(hide, -math.inf, 0.0).expand(s, s).clone()
+    assert rel(F.sliding_window_attention(q, bad, v, 1300, 4, attn_mask=minus), clean.double()) <= 1e-6
+
+
+@pytest.mark.parametrize("big", [1e3, 1e6, 1e10, 1e30])
+@pytest.mark.parametrize("what", ["key", "value", "key column", "value column", "value tile", "small values"])
+def test_long_windows_outliers_leave_other_rows_exact(what, big):
+    # One key, value, column or tile far larger than the rest: rows that do not see it, or columns beside
+    # it, keep the tolerance relative to their own size. (The oracle's rows that see a huge key have one
+    # weight of 1; their scores' errors are relative to the huge one and are not compared.)
+    s, w = 2100, 800
+    q, k, v = make(1, 2, 2, s, s, 128, "plain", 23)
+    if what == "key":
+        k[:, :, 100] *= big
+    elif what == "value":
+        v[:, :, 100] *= big
+    elif what == "key column":  # seen by queries that have nothing in that column
+        k[..., 5] *= big
+        q[..., 5] = 0
+    elif what == "value column":
+        v[..., 5] *= big
+    elif what == "value tile":
+        v[:, :, 64:128] *= big
+    else:
+        v[:, :, 101:] /= big
+    out = F.sliding_window_attention(q, k, v, w)
+    ref = reference(q, k, v, w, 0, 0)
+    rows, cols = slice(100 + w, s), [c for c in range(128) if c != 5]
+    if what in ("key column", "value column"):
+        rows = slice(0, s)
+    assert rel(out[:, :, rows][..., cols], ref[:, :, rows][..., cols]) <= 1e-5
+    assert dc._lib.load().dc_device_status(1) == 0
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-18, 1e18, 1e30])
+def test_long_windows_of_any_magnitude(scale):
+    # Powers of ten that leave the scores where they were, and values of any size.
+    s = 1300
+    q, k, v = make(1, 2, 2, s, s, 128, "plain", 24)
+    assert rel(F.sliding_window_attention(q * scale, k / scale, v * scale, s), reference(q * scale, k / scale, v * scale, s, 0, 0)) <= 1e-5
+
+
+def test_long_windows_of_zeros():
+    s = 1300
+    q, k, v = make(1, 2, 2, s, s, 128, "plain", 25)
+    q[:, :, 5] = 0
+    k[:, :, 64:192] = 0
+    v[:, :, 128:300] = 0
+    v[..., 7] = 0
+    check(q, k, v, s, 0)
+    assert (F.sliding_window_attention(q, k, torch.zeros_like(v), s) == 0).all()
+
+
+def test_long_windows_captured_and_on_two_streams():
+    s = 1400
+    q, k, v = make(1, 2, 2, s, s, 128, "plain", 26)
+    f = lambda: F.sliding_window_attention(q, k, v, 1300, 2)
+    first = f()
+    f()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f()
+    graph.replay()
+    assert torch.equal(out, first)
+    k[:, :, 30] *= 1e10  # now a tile is wide
+    graph.replay()
+    assert torch.equal(out, f())
+    assert rel(out[:, :, 1340:], reference(q, k, v, 1300, 2, 0)[:, :, 1340:]) <= 1e-5
+    k[:, :, 30] /= 1e10
+    graph.replay()
+    assert torch.equal(out, f())
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    want = f()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for stream in (a, b):
+            with torch.cuda.stream(stream):
+                got.append(f())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("s,w", [(300, 100), (1400, 1300), (5000, 4500)])
+@pytest.mark.parametrize("big", [1e4, 1e8, 1e12, 1e18])
+def test_huge_scores_pick_one_key(d, s, w, big):
+    # One key's score is far above the others of every row (its gap passes 100): the row is that key's
+    # value, up to the tolerance. Rows that do not see it keep theirs.
+    q, k, v = make(1, 1, 1, s, s, d, "plain", 27)
+    q[..., 0] = q[..., 0].abs() + 1.0
+    k[:, :, 40] = 0
+    k[:, :, 40, 0] = big
+    out = F.sliding_window_attention(q, k, v, w)
+    seen = slice(40, 40 + w)
+    assert rel(out[:, :, seen], v[:, :, 40:41].expand_as(out[:, :, seen]).double()) <= 1e-5
+    ref = reference(q, k, v, w, 0, 0)
+    rest = torch.cat([out[:, :, :40], out[:, :, 40 + w:]], 2)
+    assert rel(rest, torch.cat([ref[:, :, :40], ref[:, :, 40 + w:]], 2)) <= 1e-5
+    assert dc._lib.load().dc_device_status(1) == 0
