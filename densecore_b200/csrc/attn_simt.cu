@@ -163,6 +163,7 @@ __global__ void bwd_delta_kernel(AttnProblem p, AttnGrads g) {
     float s = 0.0f;
     for (int64_t x = lane; x < p.Ev; x += WARP) s = fmaf(d[x * g.dos[3]], o[x * p.os[3]], s);
     s = warp_sum(s);
+    if (p.window && sees_one_key(p, b, h, i, lane, WARP, 0xffffffffu)) s = __uint_as_float(ONE_KEY);
     if (lane == 0) g.delta[row] = s;
 }
 
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(BK_WARPS *WARP) bwd_dkdv_simt_kernel(AttnProbl
                     float dp = 0.0f;
                     for (int d = 0; d < Ev; d++) dp = fmaf(dr[d], vr[d], dp);
                     const float z = keep_factor(p, b, h, i, kj);
-                    ds = pr * (dp * z - srow[2 * warp + 1]);
+                    ds = p.window && one_key(srow[2 * warp + 1]) ? 0.0f : pr * (dp * z - srow[2 * warp + 1]);
                     pr *= z;
                 }
                 sP[warp * BK_KEYS + lane] = pr;
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(BK_WARPS *WARP) bwd_dq_simt_kernel(AttnProblem
             const float *dr = sdo + warp * Ev, *vr = sv + lane * VP;
             float dp = 0.0f;
             for (int d = 0; d < Ev; d++) dp = fmaf(dr[d], vr[d], dp);
-            ds = pr * (dp * keep_factor(p, b, h, i, kj) - delta_i);
+            ds = p.window && one_key(delta_i) ? 0.0f : pr * (dp * keep_factor(p, b, h, i, kj) - delta_i);
         }
         sDS[warp * BK_KEYS + lane] = ds;
         __syncwarp();

@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(PrepArgs a) {
         for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(group_mask, s, o);
         split_store(a.qhl, r * DD + 4 * j, rows_a * DD, q4, a.split, a.lo_only);
         split_store(a.dohl, r * DD + 4 * j, rows_a * DD, d4, a.split, a.lo_only);
+        if (p.window && sees_one_key(p, b, h, l, j, LPR, group_mask)) s = __uint_as_float(ONE_KEY);
         if (j == 0) {
             a.g.delta[r] = s;
             a.lse2[r] = p.lse[b * p.ls[0] + h * p.ls[1] + l * p.ls[2]] * LOG2E;
@@ -662,24 +663,28 @@ __global__ void __maxnreg__(168)
             return true;
         };
         // Lane c holds the lse (base 2) and the delta of this half's query column c of block i.
-        auto colvals = [&](int i, float &lse2, float &del) {
+        auto colvals = [&](int i, float &lse2, float &del, bool &one) {
             int64_t h, q0;
             blk_coords(i, h, q0);
             const int64_t q = q0 + cb + (lane % CPT);
             lse2 = del = 0.0f;
+            one = false;
             if (q < p.L) {
                 const int64_t idx = (b * p.H + h) * p.L + q;
                 lse2 = a.lse2[idx];
                 del = a.g.delta[idx];
+                if (WIN && one_key(del)) del = 0.0f, one = true;
             }
         };
         float cur_l = 0.0f, cur_d = 0.0f;
-        if (ok && nblk > 0) colvals(0, cur_l, cur_d);
+        bool cur_one = false;
+        if (ok && nblk > 0) colvals(0, cur_l, cur_d, cur_one);
         for (int i = 0; ok && i < nblk; i++) {
             int64_t h, q0;
             blk_coords(i, h, q0);
             float nxt_l = 0.0f, nxt_d = 0.0f;
-            if (i + 1 < nblk) colvals(i + 1, nxt_l, nxt_d);
+            bool nxt_one = false;
+            if (i + 1 < nblk) colvals(i + 1, nxt_l, nxt_d, nxt_one);
             // Column c is query base + c: valid below L and, under causal masking, from `key` on.
             const int64_t base = q0 + cb;
             uint32_t vbits = 0xFFFFFFFFu;
@@ -742,6 +747,14 @@ __global__ void __maxnreg__(168)
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(bar(C::P_READY));
+            if constexpr (WIN) {
+                const unsigned ones = __ballot_sync(FULL, cur_one);
+                if (ones) {
+#pragma unroll
+                    for (int c = 0; c < CPT; c++)
+                        if ((ones >> c) & 1u) pv[c] = 0.0f;
+                }
+            }
             if (!warp_wait(bar(C::DP_FULL), i & 1, abort, err)) {
                 ok = false;
                 break;
@@ -772,6 +785,7 @@ __global__ void __maxnreg__(168)
             tc_fence_before();
             mbar_arrive(bar(C::DS_READY));
             cur_l = nxt_l;
+            cur_one = nxt_one;
             cur_d = nxt_d;
             if (!fold(i)) {
                 ok = false;
@@ -1100,7 +1114,9 @@ __global__ void __maxnreg__(168)
         }
         const int64_t ridx = (b * p.H + h) * p.L + q;
         const float lse2 = row_ok ? a.lse2[ridx] : 0.0f;
-        const float del = row_ok ? a.g.delta[ridx] : 0.0f;
+        float del = row_ok ? a.g.delta[ridx] : 0.0f;
+        const bool one = WIN && one_key(del);
+        if (one) del = 0.0f;
         float pv[CPT];      // P of the block in flight, this thread's columns
         uint32_t zcur = 0;  // its dropout keep bits
         // Reads S_j, releases its columns, and leaves P_j in pv.
@@ -1111,7 +1127,7 @@ __global__ void __maxnreg__(168)
             const bool edge = WIN ? !window_interior(p, q0, TILE, key0(j), NB)
                                   : MASKED || !row_ok || (int64_t)(j + 1) * NB > p.S || (p.causal && (int64_t)(j + 1) * NB - 1 > q0);
             if (WIN) {
-                vbits = !row_ok ? 0u : (edge ? window_key_bits(p, q, base) : vbits);
+                vbits = !row_ok || one ? 0u : (edge ? window_key_bits(p, q, base) : vbits);
             } else if (edge) vbits = row_ok ? col_bits32(0, (p.causal ? min(p.S, q + 1) : p.S) - base) : 0u;
             // The user mask along this query's row, loaded before the wait for S.
             float mk[MASKED ? CPT : 1];

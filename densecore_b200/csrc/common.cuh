@@ -228,6 +228,26 @@ __device__ __forceinline__ void window_rows(const AttnProblem &p, int64_t k0, in
     end = k0 < p.sinks ? p.L : max(begin, min(p.L, k0 + keys - 1 + p.window - p.offset));
 }
 
+// A row that sees one key gives it the weight 1 whatever its score: dS is 0, which dP - delta, the same
+// sum taken twice in different orders, is not. Through a window such a row's delta holds these bits (a NaN
+// that no sum gives) instead.
+constexpr uint32_t ONE_KEY = 0x7fc0beadu;
+__device__ __forceinline__ bool one_key(float delta) { return __float_as_uint(delta) == ONE_KEY; }
+
+// Whether query row i sees one key through the window and the mask, by `lanes` converged lanes (`group`).
+__device__ __forceinline__ bool sees_one_key(const AttnProblem &p, int64_t b, int64_t h, int64_t i, int lane, int lanes, unsigned group) {
+    const int64_t t = i + p.offset, hi = max((int64_t)0, min(t + 1, p.S)), lo = max((int64_t)0, min(t - p.window + 1, hi));
+    const int64_t first = min(p.sinks, lo), n = first + hi - lo;  // keys [0, first) and [lo, hi)
+    if (p.mask_kind == MASK_NONE || n == 0) return n == 1;
+    int seen = 0;  // the newest first: mostly two are seen at once
+    for (int64_t left = n; left > 0 && seen < 2; left -= lanes) {
+        const int64_t x = left - 1 - lane;
+        const bool visible = x >= 0 && !(mask_value(p, b, h, i, x < first ? x : lo + x - first) <= MASK_HIDES);
+        seen += __popc(__ballot_sync(group, visible) & group);
+    }
+    return seen == 1;
+}
+
 // Host side: the thread's last error message and a setter that returns the status.
 void set_error(const std::string &msg);
 std::string last_error();

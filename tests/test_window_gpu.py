@@ -475,3 +475,41 @@ def test_huge_scores_pick_one_key(d, s, w, big):
     rest = torch.cat([out[:, :, :40], out[:, :, 40 + w:]], 2)
     assert rel(rest, torch.cat([ref[:, :, :40], ref[:, :, 40 + w:]], 2)) <= 1e-5
     assert dc._lib.load().dc_device_status(1) == 0
+
+
+@pytest.mark.parametrize("layout", ["plain", "odd"])
+@pytest.mark.parametrize("d", [32, 64, 128, 200])
+@pytest.mark.parametrize("case", [  # l, s, window, sinks, offset, valid keys per sequence
+    (1, 1, 1, 0, None, None), (1, 1, 9, 4, None, None), (300, 300, 1, 0, None, None), (70, 300, 1, 0, None, None),
+    (200, 100, 50, 0, 149, None), (150, 150, 40, 0, 0, (1, 1)), (150, 150, 150, 3, 0, (1, 0)), (300, 300, 1, 0, 0, (200, 60)),
+    (129, 2, 1, 1, 0, (1, 1))])
+def test_rows_of_one_key_have_no_score_gradient(case, d, layout):
+    # A row's only key has the weight 1 whatever its score: dq and dk are exactly 0, dv is grad_out's sum.
+    l, s, window, sinks, offset, valid = case
+    q, k, v = (t.detach().requires_grad_() for t in make(2, 4, 2, l, s, d, layout, 28))
+    mask = None
+    if valid:
+        mask = (torch.arange(s, device="cuda") < torch.tensor(valid, device="cuda")[:, None])[:, None, None]
+    out = F.sliding_window_attention(q, k, v, window, sinks, attn_mask=mask, offset=offset, enable_gqa=True)
+    go = torch.randn(out.shape, device="cuda")
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), go)
+    refs = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    ref = reference(*refs, window, sinks, s - l if offset is None else offset, mask)
+    rq, rk, rv = torch.autograd.grad(ref, refs, go.double())
+    one = [(x == 0).all().item() for x in (rq, rk)]
+    if case != (200, 100, 50, 0, 149, None):
+        assert one == [True, True]
+        assert (dq == 0).all() and (dk == 0).all()
+    for a, r in ((out, ref), (dv, rv), (dq, rq), (dk, rk)):
+        assert rel(a.detach(), r.detach()) <= 1e-5
+
+
+def test_rows_of_one_key_beside_others():
+    # Every third row sees one key, the others all; float and bool masks, both tensor-core head dims.
+    for d in (64, 128):
+        q, k, v = make(1, 2, 2, 260, 260, d, "bshd", 29)
+        i, j = torch.arange(260, device="cuda")[:, None], torch.arange(260, device="cuda")
+        mask = (i % 3 != 0) | (j == i)
+        for m in (mask, torch.where(mask, 0.25, -math.inf)):
+            _, grads = check(q, k, v, 100, 2, mask=m)
+            assert (grads[0][:, :, ::3] == 0).all()
