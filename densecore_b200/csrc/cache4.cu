@@ -65,62 +65,97 @@ __device__ __forceinline__ float mid(uint32_t w) { return fmaf(8.0f, bf16_low(w)
 
 // ------------------------------------------------------------------ fill and read back ----
 
+// Two sums (fused products) in one instruction, each rounded as alone.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(r))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
+    return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// (x & mask) | bits in one instruction (the compiler made two of it).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+    return r;
+}
+
+// Eight channels as the pairs (x_e, x_{e + 4}).
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, int64_t inner, bool vec, float (&f)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        if (vec) {
-            const float4 v = *reinterpret_cast<const float4 *>(p);
-            f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-            return;
-        }
+__device__ __forceinline__ void load8(const T *p, int64_t inner, bool vec, float2 (&f)[4]) {
+    T e[8];
+    if (vec) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = p[i * inner];
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(e)[i] = reinterpret_cast<const uint4 *>(p)[i];
     } else {
-        T e[4];
-        if (vec) {
-            *reinterpret_cast<uint2 *>(e) = *reinterpret_cast<const uint2 *>(p);
-        } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) e[i] = p[i * inner];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) f[i] = (float)e[i];
+        for (int i = 0; i < 8; i++) e[i] = p[i * inner];
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = make_float2((float)e[i], (float)e[i + 4]);
 }
 
 // Bytes of a block of 16 tokens of a head, keys and values.
 __host__ __device__ constexpr int block_bytes(int D) { return 20 * D; }
 
-// Where halfword (group g, r) of token `slot` (0..15) lies among a block's codes of keys or values.
-__device__ __forceinline__ int code_at(int which, int slot, int r, int g, int ng) {
-    return which ? 2 * (((slot / 4 % 2 * 8 + r) * 4 + slot % 4) * ng + g) + slot / 8 : 2 * ((slot * 4 + r / 2) * ng + g) + r % 2;
+// Where halfword (group g, r) of token `slot` (0..15) lies among a block's codes of keys or values: the
+// token's part and the halfword's, in bytes.
+__device__ __forceinline__ int slot_at(int which, int slot, int ng) {
+    return which ? (slot / 4 % 2 * 32 + slot % 4) * 4 * ng + slot / 8 * 2 : slot * 16 * ng;
+}
+__device__ __forceinline__ int code_at(int which, int r, int g, int ng) {
+    return which ? 4 * (4 * r * ng + g) : 4 * (r / 2 * ng + g) + r % 2 * 2;
 }
 
-// The keys or values of the block of 16 tokens that holds position pos of sequence b, and its slot
-// there; null (and the device status) where the table has no page for it.
+// Position pos of sequence b, keys or values: the token's part of the codes, and from there the way to its
+// scales in bytes; null (and the device status) where the table has no page for it.
 struct Place {
-    uint8_t *half;
-    int slot;
+    uint8_t *codes;
+    int scales;
 };
 __device__ __forceinline__ Place place_of(const Cache4Args &a, int64_t b, int64_t pos, int which, int head) {
     if (pos >= 0 && pos < a.P * a.c.page_size) {
         const uint32_t entry = (uint32_t)pos / (uint32_t)a.c.page_size, slot = (uint32_t)pos - entry * (uint32_t)a.c.page_size;
         const int64_t page = a.table[b * a.ts[0] + entry * a.ts[1]];
-        if (page >= 0 && page < a.c.pages)
-            return {a.c.data + ((page * a.c.Hkv + head) * (a.c.page_size / 16) + slot / 16) * block_bytes(a.c.D) + which * 10 * a.c.D,
-                    (int)(slot % 16)};
+        if (page >= 0 && page < a.c.pages) {
+            const int ng = a.c.D / GROUP, at = slot_at(which, (int)(slot % 16), ng);
+            uint8_t *half = a.c.data + ((page * a.c.Hkv + head) * (a.c.page_size / 16) + slot / 16) * block_bytes(a.c.D) + which * 10 * a.c.D;
+            return {half + at, 8 * a.c.D + (int)(slot % 16) * 4 * ng - at};
+        }
     }
     atomicExch(a.err, BAD_TABLE);
     return {nullptr, 0};
 }
 
-// Filling and reading back are bound by HBM and, close behind, by the arithmetic on each value. A block
-// takes a run of tokens of one (sequence, head) of the keys or the values (grid: token runs, 2 Hkv, B); a
-// thread four channels of ROWS tokens, whose loads are issued together; eight neighbours make a group of
-// 32. The tokens' places (a division by the page size, a look into the table) are found once a block.
-constexpr int ROWS = 4;
+// Filling and reading back are bound by instructions (issue slots 70 and 77 % busy, HBM below 30 %). Grid:
+// token runs, 2 Hkv (keys or values of a head), B. Appending, a thread takes eight channels of APPEND_ROWS
+// tokens, whose loads are issued together, four neighbours make a group of 32, and a warp finds its tokens'
+// places (a division by the page size, a look into the table) by itself. Reading, a thread takes four
+// channels, so that a warp's stores are contiguous (eight: 24 -> 28 us), and the block finds the places.
+// 8 sequences of 700 to 1500 tokens, 8 heads of 128: append 28.5 us, read 22.5 us. (Appending with four
+// channels a thread: 37; two rows 32, eight 41.)
+constexpr int FILL_WARPS = 8, APPEND_ROWS = 4, READ_ROWS = 4;
 
-// The places of the block's tokens t0 .. (at most 64), those from `last` on null.
+// Appending: the places of a warp's tokens, those from `last` on null.
+__device__ __forceinline__ void warp_places(const Cache4Args &a, int64_t b, int64_t pos0, int64_t t0, int64_t last, int run, int which, int head,
+                                            Place *places) {
+    const int lane = threadIdx.x & 31;
+    if (lane < run) places[lane] = t0 + lane < last ? place_of(a, b, pos0 + t0 + lane, which, head) : Place{nullptr, 0};
+    __syncwarp();
+}
+
+// Reading: the places of the block's tokens t0 .. (at most 64), those from `last` on null.
 __device__ __forceinline__ void block_places(const Cache4Args &a, int64_t b, int64_t pos0, int64_t t0, int64_t last, int run, int which,
                                              int head, Place *places) {
     if ((int)threadIdx.x < run) {
@@ -150,50 +185,78 @@ __device__ __forceinline__ uint32_t fifteenth_up(float x) {
     return (w + 0xFFFFu) & 0xFFFF0000u;
 }
 
-// The code of x = d above low: the correctly rounded d / scale to the nearest whole number (ties to
-// even), by a product with the reciprocal (off by less than 1e-5 for quotients up to 15) where that
-// cannot round the other way. inv NaN: divide.
-__device__ __forceinline__ uint32_t code_of(float d, float scale, float inv) {
-    constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the rounded number
-    const float q = d * inv;
-    float m = q + MAGIC;
-    if (!(fabsf(q - (m - MAGIC)) < 0.4999f)) m = __fdiv_rn(d, scale) + MAGIC;
-    return __float_as_uint(m) & 15u;
+// The codes of eight values d = x - low (pairs e, e + 4), as a word: the correctly rounded d / scale to the
+// nearest whole number (ties to even), by a product with the reciprocal (off by less than 3e-6 for
+// quotients up to 15) where that cannot round the other way.
+__device__ __forceinline__ uint32_t codes_of(const float2 (&d)[4], float scale) {
+    constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: sums with it are rounded to whole numbers
+    const bool fast = scale > 1e-37f && scale < 1e37f;
+    const float2 inv = both(fast ? rcp_fast(scale) : 0.0f);
+    float2 n[4];
+    float2 r[4];
+    float off = fast ? 0.0f : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float2 q = mul2(d[e], inv);
+        n[e] = add2(add2(q, both(MAGIC)), both(-MAGIC));
+        r[e] = fma2(n[e], both(-1.0f), q);
+        off = fmaxf(off, fmaxf(fabsf(r[e].x), fabsf(r[e].y)));
+    }
+    if (off >= 0.49999f) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (!fast || fabsf(r[e].x) >= 0.49999f) n[e].x = __fdiv_rn(d[e].x, scale) + MAGIC - MAGIC;
+            if (!fast || fabsf(r[e].y) >= 0.49999f) n[e].y = __fdiv_rn(d[e].y, scale) + MAGIC - MAGIC;
+        }
+    }
+    // n_0 + 16 n_1 + 256 n_2 + 4096 n_3, exactly, then 2^23 more: the sum's low 16 bits.
+    const float2 w = add2(fma2(n[3], both(4096.0f), fma2(n[2], both(256.0f), fma2(n[1], both(16.0f), n[0]))), both(8388608.0f));
+    return __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x5410);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Args a, bool vec) {
-    __shared__ Place places[256 / 16 * ROWS];
-    const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
-    const int64_t b = blockIdx.z;
-    const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes, row0 = threadIdx.x / lanes;
-    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), start = a.starts[b * a.starts_stride];
+__global__ void __launch_bounds__(FILL_WARPS * 32, 4) cache4_append_kernel(const Cache4Args a, bool vec) {
+    constexpr int ROWS = APPEND_ROWS;
+    __shared__ Place places_of[FILL_WARPS][32 / (64 / 8) * ROWS];
+    const int which = blockIdx.y & 1, head = blockIdx.y >> 1, ng = a.c.D / GROUP;
+    const int64_t b = blockIdx.z, start = a.starts[b * a.starts_stride];
     const int64_t last = min(a.T, a.ends ? a.ends[b * a.ends_stride] - start : a.T);  // tokens from here on stay out
+    // Lanes of a row, rows a pass of the warp; this lane's row and first quad of channels.
+    const int lane = threadIdx.x & 31, lanes = a.c.D / 8, per = 32 / lanes, sub = lane / lanes, quad = 2 * (lane & (lanes - 1)), g = quad / 8, r = quad % 8;
+    const int64_t t0 = ((int64_t)blockIdx.x * FILL_WARPS + threadIdx.x / 32) * (per * ROWS);
     if (t0 >= last) return;
+    const int code = code_at(which, r, g, ng);
+    Place *places = places_of[threadIdx.x / 32];
     const T *src = static_cast<const T *>(a.x[which]) + b * a.xs[which][0] + head * a.xs[which][1] + (int64_t)(4 * quad) * a.xs[which][3];
-    float x[ROWS][4];
+    src += (t0 + sub) * a.xs[which][2];
+    const int64_t step = per * a.xs[which][2];
+    const int here = (int)min(last - t0, (int64_t)(per * ROWS));  // the warp's tokens
+    float2 x[ROWS][4];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int64_t t = t0 + row0 + i * pass;
-        if (t < last) {
-            load4(src + t * a.xs[which][2], a.xs[which][3], vec, x[i]);
+        if (sub + i * per < here) {
+            load8(src + i * step, a.xs[which][3], vec, x[i]);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[i][e] = 0.0f;
+            for (int e = 0; e < 4; e++) x[i][e] = both(0.0f);
         }
     }
-    block_places(a, b, start, t0, last, pass * ROWS, which, head, places);
+    warp_places(a, b, start, t0, last, per * ROWS, which, head, places);
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        float mn = fminf(fminf(x[i][0], x[i][1]), fminf(x[i][2], x[i][3]));
-        float mx = max_nan(max_nan(x[i][0], x[i][1]), max_nan(x[i][2], x[i][3]));
+        float mn = fminf(x[i][0].x, x[i][0].y), mx = max_nan(x[i][0].x, x[i][0].y);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
+        for (int e = 1; e < 4; e++) {
+            mn = fminf(mn, fminf(x[i][e].x, x[i][e].y));
+            mx = max_nan(mx, max_nan(x[i][e].x, x[i][e].y));
+        }
+#pragma unroll
+        for (int o = 2; o > 0; o >>= 1) {
             mn = fminf(mn, __shfl_xor_sync(ALL, mn, o));
             mx = max_nan(mx, __shfl_xor_sync(ALL, mx, o));
         }
-        const Place at = places[row0 + i * pass];
-        if (!at.half) continue;
+        const Place at = places[sub + i * per];
+        if (!at.codes) continue;
         // low: bits below bfloat16 cut, one step further down for a negative value that had some.
         uint32_t lb = __float_as_uint(mn);
         if ((lb >> 31) && (lb & 0xFFFFu)) lb += 0x10000u;
@@ -204,51 +267,64 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4Args a, 
             lb = sb = 0x7FC00000u;  // NaN
         } else if (width > 0.0f) {
             sb = fifteenth_up(width);
-            const float scale = __uint_as_float(sb);
-            const float inv = scale > 1e-37f && scale < 1e37f ? rcp_fast(scale) : NAN;  // NaN: divide
+            float2 d[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) codes |= code_of(__fsub_rn(x[i][e], low), scale, inv) << (4 * e);
+            for (int e = 0; e < 4; e++) d[e] = add2(x[i][e], both(-low));
+            codes = codes_of(d, __uint_as_float(sb));
         }
-        reinterpret_cast<uint16_t *>(at.half)[code_at(which, at.slot, r, g, ng)] = (uint16_t)codes;
-        if (r == 0) reinterpret_cast<uint32_t *>(at.half + 8 * a.c.D)[at.slot * ng + g] = (sb >> 16) | lb;
+        uint8_t *to = at.codes + code;
+        if (which) {
+            *reinterpret_cast<uint16_t *>(to) = (uint16_t)codes;
+            *reinterpret_cast<uint16_t *>(to + 16 * ng) = (uint16_t)(codes >> 16);
+        } else {  // halfwords r and r + 1 side by side
+            *reinterpret_cast<uint32_t *>(to) = codes;
+        }
+        if (r == 0) *reinterpret_cast<uint32_t *>(at.codes + at.scales + 4 * g) = (sb >> 16) | lb;
     }
 }
 
 // Token t of sequence b from the cache, in float32; zeros from the sequence's length on.
 __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bool vec) {
+    constexpr int ROWS = READ_ROWS;
     __shared__ Place places[256 / 16 * ROWS];
     const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
     const int64_t b = blockIdx.z;
     const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes, row0 = threadIdx.x / lanes;
     const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), len = a.lens[b * a.lens_stride];
     block_places(a, b, 0, t0, min(a.T, len), pass * ROWS, which, head, places);
+    const int code = code_at(which, r, g, ng);
     uint32_t codes[ROWS], sl[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
         const Place at = places[row0 + i * pass];
         codes[i] = sl[i] = 0u;  // a zero
-        if (at.half) {
-            codes[i] = reinterpret_cast<const uint16_t *>(at.half)[code_at(which, at.slot, r, g, ng)];
-            sl[i] = reinterpret_cast<const uint32_t *>(at.half + 8 * a.c.D)[at.slot * ng + g];
+        if (at.codes) {
+            codes[i] = *reinterpret_cast<const uint16_t *>(at.codes + code);
+            sl[i] = *reinterpret_cast<const uint32_t *>(at.codes + at.scales + 4 * g);
         }
     }
-    float *dst = a.y[which] + b * a.ys[which][0] + head * a.ys[which][1] + (int64_t)(4 * quad) * a.ys[which][3];
+    float *dst = a.y[which] + b * a.ys[which][0] + head * a.ys[which][1] + (t0 + row0) * a.ys[which][2] + (int64_t)(4 * quad) * a.ys[which][3];
+    const int64_t step = pass * a.ys[which][2];
+    const int here = (int)min(a.T - t0, (int64_t)(pass * ROWS));  // the block's tokens
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int64_t t = t0 + row0 + i * pass;
-        if (t >= a.T) continue;
-        const float scale = bf16_low(sl[i]), low = bf16_high(sl[i]);
-        float y[4];
+        if (row0 + i * pass >= here) continue;
+        const float2 scale = both(bf16_low(sl[i])), low = both(bf16_high(sl[i]));
+        float2 y[2];
 #pragma unroll
-        for (int e = 0; e < 4; e++)  // 2^23 + code, less 2^23: the code, without the conversion unit
-            y[e] = fmaf(scale, __uint_as_float(((codes[i] >> (4 * e)) & 15u) | 0x4B000000u) - 8388608.0f, low);
-        float *row = dst + t * a.ys[which][2];
+        for (int e = 0; e < 2; e++) {
+            // 2^23 + 16^n code, less 2^23, over 16^n: the code, exactly, without shifts or the conversion unit.
+            const float2 n = e ? make_float2(0x1p-8f, 0x1p-12f) : make_float2(1.0f, 0x1p-4f);
+            const float2 c = make_float2(__uint_as_float(and_or(codes[i], 15u << (8 * e), 0x4B000000u)),
+                                         __uint_as_float(and_or(codes[i], 15u << (8 * e + 4), 0x4B000000u)));
+            y[e] = fma2(scale, fma2(c, n, make_float2(-8388608.0f * n.x, -8388608.0f * n.y)), low);
+        }
+        float *row = dst + i * step;
         if (vec) {
-            *reinterpret_cast<float4 *>(row) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4 *>(row) = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
         } else {
             const int64_t st = a.ys[which][3];
-#pragma unroll
-            for (int e = 0; e < 4; e++) row[e * st] = y[e];
+            row[0] = y[0].x, row[st] = y[0].y, row[2 * st] = y[1].x, row[3 * st] = y[1].y;
         }
     }
 }
@@ -280,12 +356,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-// (x & mask) | bits in one instruction (the compiler made two of it).
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
     return r;
 }
 // The four pairs of codes of y, less 8, as fp16: pairs 0 and 2 as they are, 1 and 3 times 16 (their
@@ -856,33 +926,31 @@ int launch_dim(const Cache4Args &a, const SplitRows &rows, cudaStream_t stream) 
     return heads == 8 ? launch_attention<D, 2, 8>(a, rows, stream) : launch_attention<D, 2, 4>(a, rows, stream);
 }
 
-// Whether runs of four channels of a (B, H, T, D) view start on 4-element boundaries.
-bool vec4(const void *ptr, const int64_t *st, int size) {
-    return st[3] == 1 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0 && (reinterpret_cast<uintptr_t>(ptr) & (4 * size - 1)) == 0;
+// Whether the rows of a (B, H, T, D) view start on 16-byte boundaries.
+bool rows16(const void *ptr, const int64_t *st, int size) {
+    return st[3] == 1 && st[0] * size % 16 == 0 && st[1] * size % 16 == 0 && st[2] * size % 16 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
 }
 
 }  // namespace
 
-// Grid of the fill and read kernels.
-dim3 token_grid(const Cache4Args &a) {
-    const int64_t run = 256 / (a.c.D / 4) * ROWS;
-    return dim3((unsigned)((a.T + run - 1) / run), (unsigned)(2 * a.c.Hkv), (unsigned)a.B);
-}
+// Grid of the fill and read kernels, whose blocks take `run` tokens of a row of keys or values.
+dim3 token_grid(const Cache4Args &a, int64_t run) { return dim3((unsigned)((a.T + run - 1) / run), (unsigned)(2 * a.c.Hkv), (unsigned)a.B); }
 
 int cache4_append(const Cache4Args &a, cudaStream_t stream) {
     const int size = a.dtype == DC_F32 ? 4 : 2;
-    const bool vec = vec4(a.x[0], a.xs[0], size) && vec4(a.x[1], a.xs[1], size);
+    const bool vec = rows16(a.x[0], a.xs[0], size) && rows16(a.x[1], a.xs[1], size);
+    const dim3 grid = token_grid(a, FILL_WARPS * 32 / (a.c.D / 8) * APPEND_ROWS);
     KernelTrace tr("cache4_append", stream);
-    if (a.dtype == DC_F32) cache4_append_kernel<float><<<token_grid(a), 256, 0, stream>>>(a, vec);
-    else if (a.dtype == DC_F16) cache4_append_kernel<__half><<<token_grid(a), 256, 0, stream>>>(a, vec);
-    else cache4_append_kernel<__nv_bfloat16><<<token_grid(a), 256, 0, stream>>>(a, vec);
+    if (a.dtype == DC_F32) cache4_append_kernel<float><<<grid, FILL_WARPS * 32, 0, stream>>>(a, vec);
+    else if (a.dtype == DC_F16) cache4_append_kernel<__half><<<grid, FILL_WARPS * 32, 0, stream>>>(a, vec);
+    else cache4_append_kernel<__nv_bfloat16><<<grid, FILL_WARPS * 32, 0, stream>>>(a, vec);
     return check_launch("cache4_append");
 }
 
 int cache4_read(const Cache4Args &a, cudaStream_t stream) {
-    const bool vec = vec4(a.y[0], a.ys[0], 4) && vec4(a.y[1], a.ys[1], 4);
+    const bool vec = rows16(a.y[0], a.ys[0], 4) && rows16(a.y[1], a.ys[1], 4);
     KernelTrace tr("cache4_read", stream);
-    cache4_read_kernel<<<token_grid(a), 256, 0, stream>>>(a, vec);
+    cache4_read_kernel<<<token_grid(a, 256 / (a.c.D / 4) * READ_ROWS), 256, 0, stream>>>(a, vec);
     return check_launch("cache4_read");
 }
 
