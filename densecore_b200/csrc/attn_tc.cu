@@ -126,18 +126,27 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[N]) 
     else tmem_st16(taddr, r);
 }
 
+// The low part of x, which the tensor core reads cut to TF32: with NEAR half a step is added first, so that
+// it is rounded instead (a carry into the exponent included). At head dim 128 through a window the cut's
+// bias put the forward 1.0e-6 of its norm from 64 bits, 5.8e-7 with it (4 x 16 heads of 2048 tokens, a window
+// of 256: 175 -> 182 us).
+template <bool NEAR>
+__device__ __forceinline__ uint32_t low_part(float x) {
+    return tf32_lo_trunc(x) + (NEAR ? 0x1000u : 0u);
+}
+
 // 3xTF32 (SPLIT): the landed tile x stays in place as the hi operand (the tensor core reads
 // x truncated to TF32) and lo = x - trunc(x), exact, goes `lo_off` bytes further. Single-pass
 // TF32 rounds x to nearest in place instead of letting the tensor core drop the low mantissa
 // bits (which would bias every operand toward zero).
-template <bool SPLIT>
+template <bool SPLIT, bool NEAR>
 __device__ __forceinline__ void split_tile(uint8_t *hi, uint32_t lo_off, uint32_t bytes, int t) {
     for (uint32_t i = t; i < bytes / 16; i += 128) {
         float4 *ph = reinterpret_cast<float4 *>(hi) + i;
         const float4 x = *ph;
         if (SPLIT) {
             *(reinterpret_cast<uint4 *>(hi + lo_off) + i) =
-                make_uint4(tf32_lo_trunc(x.x), tf32_lo_trunc(x.y), tf32_lo_trunc(x.z), tf32_lo_trunc(x.w));
+                make_uint4(low_part<NEAR>(x.x), low_part<NEAR>(x.y), low_part<NEAR>(x.z), low_part<NEAR>(x.w));
         } else {
             float4 hv;
             hv.x = __uint_as_float(tf32_rna(x.x));
@@ -165,7 +174,7 @@ __device__ __forceinline__ float max_tree(const float (&v)[N]) {
 // Row `row` of a raw 128-byte-swizzled tile (rows of 128-byte chunks, chunk stride
 // `chunk_bytes`) into TMEM: with SPLIT the raw values as hi at col_hi and the exact remainder of
 // their TF32 truncation as lo at col_lo; without, the rounded TF32 values at col_hi.
-template <int CHUNKS, bool SPLIT>
+template <int CHUNKS, bool SPLIT, bool NEAR>
 __device__ __forceinline__ void row_to_tmem(const uint8_t *raw, uint32_t chunk_bytes, int row, uint32_t tlane,
                                             uint32_t col_hi, uint32_t col_lo) {
 #pragma unroll
@@ -180,7 +189,7 @@ __device__ __forceinline__ void row_to_tmem(const uint8_t *raw, uint32_t chunk_b
             for (int e = 0; e < 4; e++) {
                 if (SPLIT) {
                     hi[4 * g + e] = __float_as_uint(v[e]);
-                    lo[4 * g + e] = tf32_lo_trunc(v[e]);
+                    lo[4 * g + e] = low_part<NEAR>(v[e]);
                 } else {
                     hi[4 * g + e] = tf32_rna(v[e]);
                 }
@@ -375,7 +384,7 @@ __global__ void __maxnreg__(128)
         const int ct = threadIdx.x - 32 * C::W_CVT;
         const int quad = warp & 3;
         if (mbar_wait(bar(C::Q_FULL), 0, abort, err)) {
-            row_to_tmem<C::CHUNKS, SPLIT>(sg + C::OFF_V, C::Q_CHUNK, quad * 32 + lane,
+            row_to_tmem<C::CHUNKS, SPLIT, WIN && C::D == 128>(sg + C::OFF_V, C::Q_CHUNK, quad * 32 + lane,
                                           tmem + ((uint32_t)(quad * 32) << 16), C::COL_QHI, C::COL_QLO);
             tmem_wait_st();
             tc_fence_before();
@@ -383,11 +392,11 @@ __global__ void __maxnreg__(128)
             for (int j = 0; j < nblk; j++) {
                 const int ks = j % C::KST, vs = j % C::VST;
                 if (!mbar_wait(bar(C::K_FULL + ks), (j / C::KST) & 1, abort, err)) break;
-                split_tile<SPLIT>(sg + C::OFF_K + ks * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
+                split_tile<SPLIT, WIN && C::D == 128>(sg + C::OFF_K + ks * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
                 fence_proxy_async_smem();
                 mbar_arrive(bar(C::K_READY + ks));
                 if (!mbar_wait(bar(C::V_FULL + vs), (j / C::VST) & 1, abort, err)) break;
-                split_tile<SPLIT>(sg + C::OFF_V + vs * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
+                split_tile<SPLIT, WIN && C::D == 128>(sg + C::OFF_V + vs * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
                 fence_proxy_async_smem();
                 mbar_arrive(bar(C::V_READY + vs));
             }
@@ -494,7 +503,7 @@ __global__ void __maxnreg__(128)
                     if constexpr (DROP) pw = ((kbits >> (r0 + c)) & 1u) ? pc * p.keep_scale : 0.0f;
                     if (SPLIT) {
                         phi[c] = __float_as_uint(pw);
-                        plo[c] = tf32_lo_trunc(pw);
+                        plo[c] = low_part<WIN && C::D == 128>(pw);
                     } else {
                         phi[c] = tf32_rna(pw);
                     }
@@ -864,7 +873,7 @@ __global__ void __maxnreg__(128)
             for (int s = 0; s < QS; s++, x++) {
                 const int vs = vslot(x);
                 if (!(ok = mbar_wait(bar(C::V_FULL + vs), vpar(x), abort, err))) break;
-                row_to_tmem<CPS, SPLIT>(sg + C::OFF_V + vs * C::KV_STAGE, C::Q_CHUNK, quad * 32 + lane, tl,
+                row_to_tmem<CPS, SPLIT, WIN && C::D == 128>(sg + C::OFF_V + vs * C::KV_STAGE, C::Q_CHUNK, quad * 32 + lane, tl,
                                         C::COL_QHI + 32 * CPS * s, C::COL_QLO + 32 * CPS * s);
             }
             if (!ok) break;
@@ -874,11 +883,11 @@ __global__ void __maxnreg__(128)
             for (int j = 0; j < nblk; j++, kk++, x++) {
                 const int ks = kk % C::KST, vs = vslot(x);
                 if (!(ok = mbar_wait(bar(C::K_FULL + ks), (uint32_t)((kk / C::KST) & 1), abort, err))) break;
-                split_tile<SPLIT>(sg + C::OFF_K + ks * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
+                split_tile<SPLIT, WIN && C::D == 128>(sg + C::OFF_K + ks * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
                 fence_proxy_async_smem();
                 mbar_arrive(bar(C::K_READY + ks));
                 if (!(ok = mbar_wait(bar(C::V_FULL + vs), vpar(x), abort, err))) break;
-                split_tile<SPLIT>(sg + C::OFF_V + vs * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
+                split_tile<SPLIT, WIN && C::D == 128>(sg + C::OFF_V + vs * C::KV_STAGE, C::KV_BYTES, C::KV_BYTES, ct);
                 fence_proxy_async_smem();
                 mbar_arrive(bar(C::V_READY + vs));
             }
@@ -990,7 +999,7 @@ __global__ void __maxnreg__(128)
                         if constexpr (DROP) pw = ((kbits >> (r0 + c)) & 1u) ? pc * p.keep_scale : 0.0f;
                         if (SPLIT) {
                             phi[c] = __float_as_uint(pw);
-                            plo[c] = tf32_lo_trunc(pw);
+                            plo[c] = low_part<WIN && C::D == 128>(pw);
                         } else {
                             phi[c] = tf32_rna(pw);
                         }

@@ -3,11 +3,10 @@
 // No counterpart in DenseCore. Row i at t = i + offset sees the keys j <= t with t - j < window or
 // j < sinks (common.cuh); the online softmax and its rules are those of attn_tc.cu.
 //
-// attn_tc.cu multiplies float32 operands as TF32 pairs, three products each;
-// here they are pairs of fp16 instead, x = hi + lo to 22 bits, three products each (hi lo + lo hi +
-// hi hi), at twice the rate: a block of 64 keys costs 24 products of 128 x 64 x 16 and 12 of 128 x 128 x
-// 16 at head dim 128, 1560 cycles against 3260. And 22 bits rounded to nearest are nearer float32 than
-// TF32 pairs read with truncated high parts.
+// attn_tc.cu multiplies float32 operands as TF32 pairs, three products each; here they are pairs of fp16,
+// x = hi + lo to 22 bits rounded to nearest, three products each (hi lo + lo hi + hi hi), at twice the
+// rate: a block of 64 keys costs 24 products of 128 x 64 x 16 and 12 of 128 x 128 x 16 at head dim 128,
+// 1540 cycles at the nominal rate against 3070.
 //
 // fp16's range is met by powers of two, one for every row of q and every 64 rows of a head of k and v,
 // which bring the largest value to [2^14, 2^15); what they stand for is a factor of the row's and block's
@@ -22,9 +21,9 @@
 //
 // Three launches:
 //   pack   one pass over k and v (HBM-bound): a block takes 64 rows of a head, finds their power of two
-//          and whether it is wide, and writes hi and lo to contiguous scratch, padded to D columns. Keys are split once, not by
-//          every query tile that reads them, so the attention kernel has no converting warps, and the
-//          inputs may have any strides.
+//          and whether it is wide, and writes hi and lo to contiguous scratch, padded to D columns. Keys
+//          are split once, not by every query tile that reads them, so the attention kernel has no
+//          converting warps.
 //   attend one CTA per 128 query rows of a head. Warp 8 loads K and V blocks (hi and lo) into rings of
 //          three; warp 9 issues S_j = Q K_j^T into one of two TMEM buffers, Q in TMEM; warp 10 O_j = P_j
 //          V_j with P from TMEM into one of two buffers; warps 0-7 split their rows of Q into TMEM, run
@@ -32,7 +31,7 @@
 //          float32).
 //   tc     attn_tc.cu's kernel, one CTA per SM, which returns at once unless the call is left to it.
 // Measured with 16 heads of 16383 tokens, head dim 128, a window of 2048 (us): pack 119, attend 752, tc 7,
-// 868 in all against attn_tc.cu's 1427; its error against 64 bits is 4e-7 of the norm against 1.0e-6. What
+// 868 in all against attn_tc.cu's 1427; its error against 64 bits is 4e-7 of the norm against 5.8e-7. What
 // bounds attend now is no pipe: the tensor pipe is active 56 % of the cycles, issue slots are 38 % busy; the
 // chain S, softmax, P of a block is longer than its products. Four threads a row took 825, and two groups of
 // warps on alternate blocks, a thread a row, 869.
