@@ -57,10 +57,24 @@ class KVCache4:
         if page_size % 16:
             raise ValueError("page_size must be a multiple of 16")
         self.num_pages, self.kv_heads, self.head_dim, self.page_size = num_pages, kv_heads, int(head_dim), page_size
-        # A page is contiguous: copying one is copying data[page].
-        self.data = torch.zeros((num_pages, kv_heads, page_size // 16, 20 * self.head_dim), dtype=torch.uint8, device=device)
-        self.device = self.data.device
-        self._desc = _lib.DcCache4(self.data.data_ptr(), num_pages, kv_heads, self.head_dim, page_size)
+        self._hold(torch.zeros((num_pages, kv_heads, page_size // 16, 20 * self.head_dim), dtype=torch.uint8, device=device))
+
+    def _hold(self, data):
+        self._data, self.device = data, data.device
+        self._desc = _lib.DcCache4(data.data_ptr(), self.num_pages, self.kv_heads, self.head_dim, self.page_size)
+
+    @property
+    def data(self):
+        """The pages, uint8 (num_pages, kv_heads, page_size / 16, 20 head_dim). A page is contiguous: copying
+        one is copying ``data[page]``; a whole cache is restored with ``data.copy_()``."""
+        return self._data
+
+    def __getstate__(self):
+        return {name: value for name, value in self.__dict__.items() if name != "_desc"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._hold(self._data)
 
     def _table(self, page_table):
         _counts("page_table", page_table)

@@ -212,3 +212,23 @@ def test_c_entry_points_refuse_before_any_device_work():
     assert attention(table=fake((2, 1 << 28), _lib.DC_I32)) == _lib.DC_ERR_UNSUPPORTED
     if not torch.cuda.is_available():
         assert window() == rotary() == attention() == _lib.DC_ERR_CUDA
+
+
+def test_a_cache_keeps_to_its_own_memory():
+    # The pages cannot be replaced under the description that the kernels get; copies get their own.
+    import copy
+    import io
+    cache = dc.KVCache4(2, 1, 64, device="cpu")
+    cache.data[1] = 7
+    with pytest.raises(AttributeError):
+        cache.data = torch.zeros_like(cache.data)
+    twin = copy.deepcopy(cache)
+    file = io.BytesIO()
+    torch.save(cache, file)
+    file.seek(0)
+    loaded = torch.load(file, weights_only=False)
+    for other in (twin, loaded):
+        assert other.data.data_ptr() != cache.data.data_ptr() and torch.equal(other.data, cache.data)
+        assert other._desc.data == other.data.data_ptr() and other.device == cache.device
+        assert (other._desc.num_pages, other._desc.kv_heads, other._desc.head_dim, other._desc.page_size) == (2, 1, 64, 64)
+    assert cache._desc.data == cache.data.data_ptr()
