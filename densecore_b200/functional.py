@@ -219,8 +219,9 @@ def sliding_window_attention(query, key, value, window, sinks=0, attn_mask=None,
     tokens) and sees the keys j <= t with t - j < window or j < sinks, where ``attn_mask`` (bool, True
     may attend, or float32, added to the scores; a value of -1e30 or less hides its key as -inf does)
     lets it. ``lengths`` (int32 (B), L == 1, no gradient) are the keys that each sequence of a padded cache holds:
-    its row stands at the last of them. A row that sees no key gives 0 and zero gradients. scale
-    defaults to 1/sqrt(E). Not in DenseCore; the rules are those of its SDPA (functional.py:276-340).
+    its row stands at the last of them. A row that sees no key gives 0 and zero gradients, one that sees
+    a single key no gradient of query and key. Hidden keys may hold anything in the forward; hidden values,
+    and for the gradients hidden keys, must be finite. scale defaults to 1/sqrt(E). Not in DenseCore; the rules are those of its SDPA (functional.py:276-340).
     """
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not isinstance(t, torch.Tensor):

@@ -167,8 +167,10 @@ DC_API int dc_attn_merge(dc_tensor_t *out_acc, dc_tensor_t *lse_acc, const dc_te
  * sequence b are its first lengths[b] (clamped to 0..S) and its row stands at the last of them;
  * offset is then not used. mask, scale, precision, out, lse and rows that see no key are as in
  * dc_sdpa_fwd, with one difference: a float mask value of -1e30 or less hides its key as -inf does.
- * Keys that no row of a 128-row query tile sees are not read; key and value are taken as finite
- * where a tile sees them. Shapes the tensor-core kernels do not cover run the CUDA-core kernels. */
+ * Keys that no row of a 128-row query tile sees do not touch its results; where a tile sees them, values
+ * (and for the gradients keys) are taken as finite, hidden ones too. Shapes the tensor-core kernels do not
+ * cover run the CUDA-core kernels. Long windows at head dims above 64 take scratch of the size of key and
+ * value, padded to 128 channels, from the library's pool, or do without where there is no room. */
 
 /* Bytes of scratch dc_sdpa_window_fwd needs (0 unless q_len is 1 and the keys are split). */
 DC_API size_t dc_sdpa_window_fwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,
