@@ -300,3 +300,50 @@ def test_two_threads_at_once():
     threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
     [t.start() for t in threads], [t.join() for t in threads]
     assert not errors and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("scale", [1.0, 1.5, 1.0078125, 3e-38, 1.1e-37, 9e36, 2e37])
+def test_codes_at_and_beside_ties(scale):
+    # Halves of a step, and a few units in the last place beside them: to the even code, or to the near one.
+    s = torch.tensor(scale).bfloat16().float().item()
+    half = torch.arange(15, device="cuda") + 0.5
+    x = torch.zeros(15, 9, 32, device="cuda")
+    x[..., 31] = 15 * s
+    tie = (half * s)[:, None]
+    for step in range(9):
+        y = tie.clone()
+        for _ in range(abs(step - 4)):
+            y = torch.nextafter(y, torch.full_like(y, math.inf if step > 4 else -math.inf))
+        x[:, step, 1:31] = y
+    x = torch.cat([x, -x], 0).reshape(1, 1, 270, 32).repeat(1, 1, 1, 2)  # 270 tokens of 64 channels
+    pages, table = table_for(1, 270, 16)
+    cache = dc.KVCache4(pages, 1, 64, page_size=16)
+    cache.append(x, x, table, i32(0))
+    want = define(x)
+    for got in cache.read(table, i32(270), 270):
+        assert torch.equal(got, want)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("start,tokens", [(0, 1), (15, 2), (5, 31), (16, 33), (3, 127), (1, 130), (0, 517)])
+def test_append_across_blocks(dtype, dim, start, tokens):
+    # Runs that begin and end inside blocks of 16, pages and a kernel's run of tokens; rows 8 bytes off a
+    # 16-byte boundary; neighbours on both sides keep what they hold.
+    g = torch.Generator(device="cuda").manual_seed(7)
+    total, kv = start + tokens + 20, 3
+    pages, table = table_for(2, total, 16, seed=2)
+    cache = dc.KVCache4(pages, kv, dim, page_size=16)
+    old = torch.randn(2, kv, total, dim, generator=g, device="cuda").to(dtype)
+    cache.append(old, -old, table, i32(0, 0))
+    pad = 8 // old.element_size()
+    new = torch.randn(2, tokens, kv, dim + pad, generator=g, device="cuda").to(dtype)[..., pad:].transpose(1, 2)
+    cache.append(new, -new, table, i32(start, start), i32(start + tokens, start + (tokens + 1) // 2))
+    for sign, got in zip((1, -1), cache.read(table, i32(total, total), total)):
+        want = define(sign * old)
+        d = define(sign * new)
+        want[0, :, start:start + tokens] = d[0]
+        want[1, :, start:start + (tokens + 1) // 2] = d[1, :, :(tokens + 1) // 2]
+        assert torch.equal(got, want)
+    assert status() == 0
