@@ -1256,7 +1256,8 @@ constexpr int kSideRoleDq = 0;
 bool tc_backward_supported(const AttnProblem &p, const AttnGrads &g) {
     (void)g;
     // Through a window any head dims up to 128 (the pre-pass's copies are padded with zeros).
-    if (p.window ? (p.E > 128 || p.Ev > 128 || p.E == 0 || p.Ev == 0) : (p.E != p.Ev || (p.E != 64 && p.E != 128))) return false;
+    // Without a key its tiles would still walk one block (window_span), whose copies nobody wrote.
+    if (p.window ? (p.E > 128 || p.Ev > 128 || p.E == 0 || p.Ev == 0 || p.S == 0) : (p.E != p.Ev || (p.E != 64 && p.E != 128))) return false;
     if (p.L >= (1ll << 31) - TILE || p.S >= (1ll << 31) - TILE) return false;
     // 1-D grids of tiles x heads x batch (x column halves at head dim 128).
     const int64_t tiles = (max(p.L, p.S) + TILE - 1) / TILE;

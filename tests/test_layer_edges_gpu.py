@@ -1,0 +1,34 @@
+"""The ends of what the operators around attention accept: no keys, bad lengths, traced calls."""
+import pytest
+import torch
+
+from densecore_b200 import _native
+from densecore_b200 import functional as F
+
+pytestmark = pytest.mark.gpu
+
+
+def leave_nans_behind(d):
+    # The backward's scratch comes from the library's pool, which hands the next call what the last left.
+    q = torch.full((1, 4, 64, d), float("nan"), device="cuda", requires_grad=True)
+    F.sliding_window_attention(q, q, q, 16).sum().backward()
+
+
+@pytest.mark.parametrize("precision", ["3xtf32", "tf32", "fp32"])
+@pytest.mark.parametrize("d,ev", [(64, 64), (128, 128), (96, 20), (8, 72), (160, 160)])
+@pytest.mark.parametrize("rows", [1, 2, 4, 127, 129])
+def test_gradients_without_keys(rows, d, ev, precision):
+    # No row sees a key: outputs and gradients are exactly 0, whatever lies in the scratch.
+    codes = {"3xtf32": 0, "tf32": 1, "fp32": 2}
+    leave_nans_behind(128 if max(d, ev) > 64 else 64)
+    q, k, v = torch.randn(1, 2, rows, d, device="cuda"), torch.randn(1, 1, 0, d, device="cuda"), torch.randn(1, 1, 0, ev, device="cuda")
+    out, lse = _native._sliding_window(q, k, v, 3, 1, -rows, precision=codes[precision])
+    go = torch.randn_like(out)
+    gq, gk, gv = _native._sliding_window_backward(go, q, k, v, out, lse, 3, 1, -rows, precision=codes[precision])
+    assert (out == 0).all() and (lse == 0).all() and (gq == 0).all()
+    assert gk.shape == k.shape and gv.shape == v.shape
+    for mask in (torch.ones(rows, 0, dtype=torch.bool, device="cuda"), torch.zeros(1, 1, 1, 0, device="cuda")):
+        leaf = q.clone().requires_grad_()
+        y = F.sliding_window_attention(leaf, k, v, 3, 1, attn_mask=mask, enable_gqa=True)
+        y.backward(go)
+        assert (y == 0).all() and (leaf.grad == 0).all()
