@@ -304,6 +304,9 @@ struct WindowArgs {
     int64_t window, sinks, offset;
 };
 static int fill_window(AttnProblem &p, int64_t window, int64_t sinks, int64_t offset, const dc_tensor_t *lengths);
+static int window_memory_error() {
+    return fail(DC_ERR_VALUE, "sliding window attention: a tensor is null or not aligned to its type");
+}
 
 static int sdpa_bwd_impl(const dc_tensor_t *grad_out, const dc_tensor_t *q, const dc_tensor_t *k,
                          const dc_tensor_t *v, const dc_tensor_t *out, const dc_tensor_t *lse,
@@ -315,6 +318,12 @@ static int sdpa_bwd_impl(const dc_tensor_t *grad_out, const dc_tensor_t *q, cons
     int st = fill_problem(q, k, v, causal, has_scale, scale, p);
     if (!st) st = fill_mask(mask, p);
     if (!st && win) st = fill_window(p, win->window, win->sinks, win->offset, nullptr);
+    if (!st && win) {
+        const dc_tensor_t *const all[] = {grad_out, q, k, v, out, lse, grad_q, grad_k, grad_v};
+        for (const dc_tensor_t *t : all)
+            if (!st && !usable(t)) st = window_memory_error();
+        if (!st && mask && !usable(mask)) st = window_memory_error();
+    }
     if (!st) st = check_precision(precision);
     if (!st && dropout) st = set_keep(p, keep_bits, keep_scale);
     if (st) return st;
@@ -503,7 +512,7 @@ int dc_sdpa_window_fwd(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tens
     if (!st) st = fill_mask(mask, p);
     if (!st) st = fill_window(p, window, sinks, offset, lengths);
     if (!st && !(usable(q) && usable(k) && usable(v) && (!mask || usable(mask)) && usable(out) && usable(lse)))
-        st = fail(DC_ERR_VALUE, "sliding window attention: a tensor is null or not aligned to its type");
+        st = window_memory_error();
     if (!st) st = check_out(out, lse, p);
     if (!st) st = check_precision(precision);
     if (st) return st;

@@ -232,3 +232,32 @@ def test_a_cache_keeps_to_its_own_memory():
         assert other._desc.data == other.data.data_ptr() and other.device == cache.device
         assert (other._desc.num_pages, other._desc.kv_heads, other._desc.head_dim, other._desc.page_size) == (2, 1, 64, 64)
     assert cache._desc.data == cache.data.data_ptr()
+
+
+def window_backward(**kw):
+    """dc_sdpa_window_bwd on made-up memory, with the tensors in ``kw`` in place of good ones."""
+    L = _lib.load()
+    big, small = (2, 4, 8, 64), (2, 2, 9, 64)
+    ts = dict(go=fake(big), q=fake(big), k=fake(small), v=fake(small), out=fake(big), lse=fake((2, 4, 8)), mask=None,
+              gq=fake(big), gk=fake(small), gv=fake(small))
+    ts.update(kw)
+    r = {name: None if x is None else ctypes.byref(x) for name, x in ts.items()}
+    return L.dc_sdpa_window_bwd(r["go"], r["q"], r["k"], r["v"], r["out"], r["lse"], r["mask"], 4, 0, 1, 0, 0.0, 0, r["gq"], r["gk"],
+                                r["gv"], None, 0, None)
+
+
+# Made-up memory: these run only where there is no device that a call let through could touch.
+without_a_device = pytest.mark.skipif(torch.cuda.is_available(), reason="passes made-up addresses")
+
+
+@without_a_device
+@pytest.mark.parametrize("name", ["go", "q", "k", "v", "out", "lse", "gq", "gk", "gv", "mask"])
+def test_window_backward_refuses_memory_it_cannot_follow(name):
+    shape = {"k": (2, 2, 9, 64), "v": (2, 2, 9, 64), "gk": (2, 2, 9, 64), "gv": (2, 2, 9, 64), "lse": (2, 4, 8),
+             "mask": (8, 9)}.get(name, (2, 4, 8, 64))
+    for ptr in (0, 0x10002):
+        assert window_backward(**{name: fake(shape, ptr=ptr)}) == _lib.DC_ERR_VALUE
+        assert "aligned" in _lib.load().dc_last_error().decode()
+    if name != "mask":
+        assert window_backward(**{name: None}) == _lib.DC_ERR_VALUE
+    assert window_backward() == _lib.DC_ERR_CUDA
