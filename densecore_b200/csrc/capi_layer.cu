@@ -24,11 +24,14 @@ bool same_sizes(const dc_tensor_t *a, const dc_tensor_t *b) {
 }
 
 // Two writes to one place, or reads of another row's, would depend on order: outputs whose elements
-// share memory (an expanded dim) are refused.
+// share memory (an expanded dim) are refused. (Without an element nothing is shared.)
 bool overlaps(const dc_tensor_t *t) {
-    for (int i = 0; i < t->ndim; i++)
-        if (t->sizes[i] > 1 && t->strides[i] == 0) return true;
-    return false;
+    bool expanded = false;
+    for (int i = 0; i < t->ndim; i++) {
+        if (t->sizes[i] == 0) return false;
+        expanded = expanded || (t->sizes[i] > 1 && t->strides[i] == 0);
+    }
+    return expanded;
 }
 
 // Queries and keys (k null: none), positions and frequencies.

@@ -261,3 +261,15 @@ def test_window_backward_refuses_memory_it_cannot_follow(name):
     if name != "mask":
         assert window_backward(**{name: None}) == _lib.DC_ERR_VALUE
     assert window_backward() == _lib.DC_ERR_CUDA
+
+
+@without_a_device
+def test_expanded_outputs_without_elements_are_taken():
+    # torch.empty_like of an expanded tensor without elements is expanded too.
+    L = _lib.load()
+    r = ctypes.byref
+    for shape, dim in (((3, 2, 0, 64), 0), ((0, 5, 3, 64), 1)):
+        q, out = fake(shape, ptr=0), fake(shape, ptr=0)
+        q.strides[dim] = out.strides[dim] = 0
+        pos = fake(shape[2:3], _lib.DC_I64)
+        assert L.dc_rotary(r(q), None, r(pos), r(fake((32,), _lib.DC_F64)), 0, 1.0, 0, r(out), None, None) == _lib.DC_OK
