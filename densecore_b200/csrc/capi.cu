@@ -61,6 +61,15 @@ bool usable(const dc_tensor_t *t) {
     return n == 0 || (t->data && (reinterpret_cast<uintptr_t>(t->data) & (size - 1)) == 0);
 }
 
+bool overlaps(const dc_tensor_t *t) {
+    bool expanded = false;
+    for (int i = 0; i < t->ndim; i++) {
+        if (t->sizes[i] == 0) return false;
+        expanded = expanded || (t->sizes[i] > 1 && t->strides[i] == 0);
+    }
+    return expanded;
+}
+
 int device_ok() {
     int n = 0;
     cudaError_t e = cudaGetDeviceCount(&n);
@@ -304,6 +313,9 @@ struct WindowArgs {
     int64_t window, sinks, offset;
 };
 static int fill_window(AttnProblem &p, int64_t window, int64_t sinks, int64_t offset, const dc_tensor_t *lengths);
+static int window_overlap_error() {
+    return fail(DC_ERR_VALUE, "sliding window attention: an output's elements share memory");
+}
 static int window_memory_error() {
     return fail(DC_ERR_VALUE, "sliding window attention: a tensor is null or not aligned to its type");
 }
@@ -323,6 +335,7 @@ static int sdpa_bwd_impl(const dc_tensor_t *grad_out, const dc_tensor_t *q, cons
         for (const dc_tensor_t *t : all)
             if (!st && !usable(t)) st = window_memory_error();
         if (!st && mask && !usable(mask)) st = window_memory_error();
+        if (!st && (overlaps(grad_q) || overlaps(grad_k) || overlaps(grad_v))) st = window_overlap_error();
     }
     if (!st) st = check_precision(precision);
     if (!st && dropout) st = set_keep(p, keep_bits, keep_scale);
@@ -513,6 +526,7 @@ int dc_sdpa_window_fwd(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tens
     if (!st) st = fill_window(p, window, sinks, offset, lengths);
     if (!st && !(usable(q) && usable(k) && usable(v) && (!mask || usable(mask)) && usable(out) && usable(lse)))
         st = window_memory_error();
+    if (!st && (overlaps(out) || overlaps(lse))) st = window_overlap_error();
     if (!st) st = check_out(out, lse, p);
     if (!st) st = check_precision(precision);
     if (st) return st;

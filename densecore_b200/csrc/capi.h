@@ -16,6 +16,10 @@ std::string shape_str(const dc_tensor_t *t);
 // their type (a kernel's access elsewhere would fault).
 bool usable(const dc_tensor_t *t);
 
+// Two writes to one place, or reads of another row's, would depend on order: outputs whose elements
+// share memory (an expanded dim) are refused. (Without an element nothing is shared.)
+bool overlaps(const dc_tensor_t *t);
+
 // DC_OK when there is a CUDA device.
 int device_ok();
 

@@ -23,17 +23,6 @@ bool same_sizes(const dc_tensor_t *a, const dc_tensor_t *b) {
     return true;
 }
 
-// Two writes to one place, or reads of another row's, would depend on order: outputs whose elements
-// share memory (an expanded dim) are refused. (Without an element nothing is shared.)
-bool overlaps(const dc_tensor_t *t) {
-    bool expanded = false;
-    for (int i = 0; i < t->ndim; i++) {
-        if (t->sizes[i] == 0) return false;
-        expanded = expanded || (t->sizes[i] > 1 && t->strides[i] == 0);
-    }
-    return expanded;
-}
-
 // Queries and keys (k null: none), positions and frequencies.
 int fill_rotary(const char *what, const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *positions,
                 const dc_tensor_t *inv_freq, double amplitude, RotaryArgs &a) {
@@ -282,7 +271,8 @@ int dc_cache4_attention(const dc_cache4_t *cache, const dc_tensor_t *q, const dc
         return fail(DC_ERR_VALUE, "cache attention: queries must be (B, H, 1, head dim), H a multiple of the cache's heads");
     if (!usable(out) || out->dtype != q->dtype || !same_sizes(out, q) || overlaps(out))
         return fail(DC_ERR_VALUE, "cache attention: the output must have the queries' shape and type");
-    if (!usable(lse) || lse->dtype != DC_F32 || lse->ndim != 3 || lse->sizes[0] != a.B || lse->sizes[1] != q->sizes[1] || lse->sizes[2] != 1)
+    if (!usable(lse) || lse->dtype != DC_F32 || lse->ndim != 3 || lse->sizes[0] != a.B || lse->sizes[1] != q->sizes[1] || lse->sizes[2] != 1 ||
+        overlaps(lse))
         return fail(DC_ERR_VALUE, "cache attention: the logsumexp must be float32 (B, H, 1)");
     if (window < 0 || sinks < 0) return fail(DC_ERR_VALUE, "cache attention: window and sinks must not be negative");
     a.H = q->sizes[1];

@@ -170,7 +170,8 @@ DC_API int dc_attn_merge(dc_tensor_t *out_acc, dc_tensor_t *lse_acc, const dc_te
  * Keys that no row of a 128-row query tile sees do not touch its results; where a tile sees them, values
  * (and for the gradients keys) are taken as finite, hidden ones too. Shapes the tensor-core kernels do not
  * cover run the CUDA-core kernels. Long windows at head dims above 64 take scratch of the size of key and
- * value, padded to 128 channels, from the library's pool, or do without where there is no room. */
+ * value, padded to 128 channels, from the library's pool, or do without where there is no room.
+ * Null or misaligned tensors and outputs whose elements share memory are refused. */
 
 /* Bytes of scratch dc_sdpa_window_fwd needs (0 unless q_len is 1 and the keys are split). */
 DC_API size_t dc_sdpa_window_fwd_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads,

@@ -273,3 +273,41 @@ def test_expanded_outputs_without_elements_are_taken():
         q.strides[dim] = out.strides[dim] = 0
         pos = fake(shape[2:3], _lib.DC_I64)
         assert L.dc_rotary(r(q), None, r(pos), r(fake((32,), _lib.DC_F64)), 0, 1.0, 0, r(out), None, None) == _lib.DC_OK
+
+
+@without_a_device
+def test_outputs_whose_elements_share_memory_are_refused():
+    L = _lib.load()
+    r = ctypes.byref
+
+    def spread(shape, dim):
+        t = fake(shape)
+        t.strides[dim] = 0
+        return t
+
+    big, small, rows = (2, 4, 8, 64), (2, 2, 9, 64), (2, 4, 8)
+    for dim in range(4):
+        for name, shape in (("gq", big), ("gk", small), ("gv", small)):
+            assert window_backward(**{name: spread(shape, dim)}) == _lib.DC_ERR_VALUE
+            assert "share" in L.dc_last_error().decode()
+    for name, shape in (("go", big), ("q", big), ("k", small), ("v", small), ("out", big)):
+        assert window_backward(**{name: spread(shape, 1)}) == _lib.DC_ERR_CUDA  # inputs may be expanded
+
+    def forward(out, lse):
+        return L.dc_sdpa_window_fwd(r(fake(big)), r(fake(small)), r(fake(small)), None, 4, 0, 1, None, 0, 0.0, 0, r(out), r(lse),
+                                    None, 0, None)
+
+    assert forward(fake(big), fake(rows)) == _lib.DC_ERR_CUDA
+    for dim in range(4):
+        assert forward(spread(big, dim), fake(rows)) == _lib.DC_ERR_VALUE
+    for dim in range(3):
+        assert forward(fake(big), spread(rows, dim)) == _lib.DC_ERR_VALUE
+    cache, one = _lib.DcCache4(0x10000, 4, 2, 64, 16), (2, 4, 1, 64)
+
+    def attention(lse):
+        return L.dc_cache4_attention(r(cache), r(fake(one)), r(fake((2, 3), _lib.DC_I32)), r(fake((2,), _lib.DC_I32)), 0, 0, 0, 0.0,
+                                     r(fake(one)), r(lse), None, 0, None)
+
+    assert attention(fake((2, 4, 1))) == _lib.DC_ERR_CUDA
+    for dim in (0, 1):
+        assert attention(spread((2, 4, 1), dim)) == _lib.DC_ERR_VALUE
