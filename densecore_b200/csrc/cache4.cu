@@ -290,7 +290,12 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bo
     const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
     const int64_t b = blockIdx.z;
     const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes, row0 = threadIdx.x / lanes;
-    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), len = a.lens[b * a.lens_stride];
+    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), capacity = a.P * a.c.page_size;
+    int64_t len = a.lens[b * a.lens_stride];
+    if (len < 0 || len > capacity) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.err, BAD_TABLE);
+        len = len < 0 ? 0 : capacity;
+    }
     block_places(a, b, 0, t0, min(a.T, len), pass * ROWS, which, head, places);
     const int code = code_at(which, r, g, ng);
     uint32_t codes[ROWS], sl[ROWS];

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from densecore_b200 import _native
+import densecore_b200 as dc
+from densecore_b200 import _lib, _native
 from densecore_b200 import functional as F
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +33,25 @@ def test_gradients_without_keys(rows, d, ev, precision):
         y = F.sliding_window_attention(leaf, k, v, 3, 1, attn_mask=mask, enable_gqa=True)
         y.backward(go)
         assert (y == 0).all() and (leaf.grad == 0).all()
+
+
+def test_read_reports_lengths_out_of_range():
+    # Capacity 64; also where fewer positions are read than the table holds.
+    status = _lib.load().dc_device_status
+    cache = dc.KVCache4(4, 2, 64, page_size=32)
+    table = torch.tensor([[0, 1], [2, 3], [1, 0]], dtype=torch.int32, device="cuda")
+    k = torch.randn(3, 2, 64, 64, device="cuda")
+    zeros = torch.zeros(3, dtype=torch.int32, device="cuda")
+    cache.append(k[:2], k[:2], table[:2], zeros[:2])
+    full, _ = cache.read(table, torch.full_like(zeros, 64), 64)
+    status(1)
+    for lengths, seen, bad in (((64, 0, 17), (64, 0, 17), 0), ((64, -7, 17), (64, 0, 17), 3), ((65, 5, 17), (64, 5, 17), 3),
+                               ((2 ** 31 - 1, -2 ** 31, 0), (64, 0, 0), 3)):
+        lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        for positions in (64, 40, 1, 100):
+            key, value = cache.read(table, lens, positions)
+            assert status(1) == bad, (lengths, positions)
+            for b, n in enumerate(seen):
+                n = min(n, positions)
+                assert torch.equal(key[b, :, :n], full[b, :, :n]) and (key[b, :, n:] == 0).all()
+                assert torch.equal(value[b], key[b])
