@@ -210,6 +210,18 @@ def _fwd_path(q, k, v, mask=None, causal=False, precision=None):
     return L.dc_sdpa_fwd_path(*[_lib.ref(x) for x in vs], int(bool(causal)), prec)
 
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _traced(what):
+    """Whether torch.jit.trace is recording: of a call outside an autograd Function it would record the
+    allocations alone, and the trace return them unwritten. make_fx records no Function either: refused."""
+    if (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None
+            or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None):
+        raise RuntimeError(f"{what} cannot be recorded by make_fx")
+    return torch._C._get_tracing_state() is not None
+
+
 _SAME_DEVICE = contextlib.nullcontext()
 
 
@@ -270,8 +282,8 @@ def _sliding_window(q, k, v, window, sinks, offset, scale=None, mask=None, lengt
     ``need_lse``: (out, None)."""
     L = _lib.load()
     dev = _device_of(q, k, v, mask, lengths)
-    B, H, Lq, E = q.shape
-    Hkv, S, Ev = k.shape[1], k.shape[2], v.shape[3]
+    B, H, Lq, E = map(int, q.shape)  # (in a trace they come as tensors)
+    Hkv, S, Ev = int(k.shape[1]), int(k.shape[2]), int(v.shape[3])
     out = torch.empty_like(q) if E == Ev else torch.empty((B, H, Lq, Ev), device=dev, dtype=torch.float32)
     prec = precision_code() if precision is None else precision
     has, sc = _scale_args(scale)

@@ -84,10 +84,16 @@ class KVCache4:
             raise RuntimeError(f"the page table is on {page_table.device}, the cache on {self.device}")
         return page_table.shape[0]
 
+    def _eager(self):
+        """The pages are no tensors of a trace, which would keep nothing of a call."""
+        if _native._traced("a 4-bit cache"):
+            raise RuntimeError("a 4-bit cache cannot be traced")
+
     def append(self, key, value, page_table, start, end=None):
         """Token i of key, value (B, kv_heads, T, head_dim) to position ``start[b] + i``, where that is
         below ``end[b]`` (ragged prompts). Places from ``end`` on keep what they hold. One call must
         not write a slot twice."""
+        self._eager()
         b = self._table(page_table)
         _counts("start", start, b)
         if end is not None:
@@ -106,6 +112,7 @@ class KVCache4:
     def read(self, page_table, lengths, max_length):
         """(key, value) of the first ``max_length`` positions in float32, (B, kv_heads, max_length,
         head_dim), zeros from ``lengths[b]`` on."""
+        self._eager()
         b = self._table(page_table)
         _counts("lengths", lengths, b)
         return _native._cache4_read(self._desc, page_table, lengths, _whole("max_length", max_length, 0))
@@ -116,6 +123,7 @@ class KVCache4:
         kv_heads (grouped queries). With ``window`` the token, standing at the last position, sees the
         positions less than ``window`` back and the first ``sinks``. scale defaults to
         1/sqrt(head_dim). An empty sequence gives 0. No gradient."""
+        self._eager()
         b = self._table(page_table)
         _counts("lengths", lengths, b)
         if not isinstance(query, torch.Tensor):

@@ -190,12 +190,19 @@ def _whole_number(name, value, least=None):
     return int(value)
 
 
+def _through_function(what, *inputs):
+    """Whether a call goes through its autograd Function: an input requires a gradient, or it is traced."""
+    return _native._traced(what) or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs))
+
+
 class _SlidingWindow(torch.autograd.Function):
-    """Attention through a sliding window; saves q, k, v, out, lse."""
+    """Attention through a sliding window; saves q, k, v, out, lse. offset None: the queries are the last keys."""
 
     @staticmethod
-    def forward(ctx, q, k, v, window, sinks, offset, scale, mask):
-        out, lse = _native._sliding_window(q, k, v, window, sinks, offset, scale, mask)
+    def forward(ctx, q, k, v, window, sinks, offset, scale, mask, lengths):
+        if offset is None:  # (here, so that a trace does not keep the traced lengths' difference)
+            offset = int(k.shape[2]) - int(q.shape[2])
+        out, lse = _native._sliding_window(q, k, v, window, sinks, offset, scale, mask, lengths)
         ctx.save_for_backward(q, k, v, out, lse, *(() if mask is None else (mask,)))
         ctx.window, ctx.sinks, ctx.offset, ctx.scale = window, sinks, offset, scale
         return out
@@ -206,7 +213,7 @@ class _SlidingWindow(torch.autograd.Function):
         q, k, v, out, lse, *mask = ctx.saved_tensors
         gq, gk, gv = _native._sliding_window_backward(grad, q, k, v, out, lse, ctx.window, ctx.sinks, ctx.offset,
                                                       ctx.scale, mask[0] if mask else None)
-        return gq, gk, gv, None, None, None, None, None
+        return gq, gk, gv, None, None, None, None, None, None
 
 
 def sliding_window_attention(query, key, value, window, sinks=0, attn_mask=None, lengths=None, offset=None, scale=None,
@@ -251,14 +258,16 @@ def sliding_window_attention(query, key, value, window, sinks=0, attn_mask=None,
             raise ValueError(f"lengths must be ({b},), got {tuple(lengths.shape)}")
         if length != 1 or offset is not None:
             raise ValueError("lengths take a query length of 1 and no offset")
-    offset = source - length if offset is None else _whole_number("offset", offset)
+    if offset is not None:
+        offset = _whole_number("offset", offset)
     mask = _flash_mask(_as_mask(attn_mask, query.device), rank)
-    grad = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)
-    if grad:
-        if lengths is not None:
+    if _through_function("sliding window attention", query, key, value):
+        if lengths is not None and torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
             raise NotImplementedError("sliding window attention with lengths has no gradient")
-        out = _SlidingWindow.apply(q, k, v, window, sinks, offset, float(scale), mask)
+        out = _SlidingWindow.apply(q, k, v, window, sinks, offset, float(scale), mask, lengths)
     else:
+        if offset is None:
+            offset = source - length
         out, _lse = _native._sliding_window(q, k, v, window, sinks, offset, float(scale), mask, lengths, need_lse=False)
     return out.squeeze(1) if rank == 3 else out
 
@@ -352,7 +361,7 @@ def rotary_embedding(query, key, positions, inv_freq, *, interleaved=False, ampl
     channels and the others pass through. Not in DenseCore, whose nanoGPT path adds learned positions.
     """
     q, k = _rotary_args("rotary", query, key, positions, inv_freq, interleaved, amplitude)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _through_function("rotary_embedding", q, k):
         q, k = _Rotary.apply(q, k, positions, inv_freq, interleaved, float(amplitude))
     else:
         q, k = _native._rotary(q, k, positions, inv_freq, interleaved, float(amplitude))
@@ -398,7 +407,7 @@ def qk_norm_rotary(query, key, query_weight, key_weight, positions, inv_freq, *,
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     args = (q, k, query_weight, key_weight, positions, inv_freq, float(eps), interleaved, float(amplitude))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    if _through_function("qk_norm_rotary", *args[:4]):
         q, k = _QKNormRotary.apply(*args)
     else:
         q, k = _native._qk_norm_rotary(*args)

@@ -55,3 +55,37 @@ def test_read_reports_lengths_out_of_range():
                 n = min(n, positions)
                 assert torch.equal(key[b, :, :n], full[b, :, :n]) and (key[b, :, n:] == 0).all()
                 assert torch.equal(value[b], key[b])
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_calls_run_at_other_sizes(grad):
+    freq, _ = F.rotary_frequencies(64, device="cuda")
+    weight = torch.rand(64, device="cuda") + 0.5
+
+    def layer(q, k, v, positions, key_positions):
+        q, _ = F.qk_norm_rotary(q, None, weight, None, positions, freq)
+        k, _ = F.rotary_embedding(k, None, key_positions, freq)
+        return F.sliding_window_attention(q, k, v, 16, 2, enable_gqa=True)
+
+    def inputs(b, rows, keys):
+        q, k, v = (torch.randn(b, h, n, 64, device="cuda") for h, n in ((4, rows), (2, keys), (2, keys)))
+        at = torch.arange(keys, device="cuda")
+        return q.requires_grad_(grad), k.requires_grad_(grad), v, at[keys - rows:], at
+
+    traced = torch.jit.trace(layer, inputs(1, 20, 33), check_trace=False)
+    for sizes in ((1, 20, 33), (2, 70, 90), (1, 1, 40)):
+        args = inputs(*sizes)
+        got, ref = traced(*args), layer(*args)
+        assert torch.equal(got, ref)
+        if grad:
+            go = torch.randn_like(ref)
+            for x, y in zip(torch.autograd.grad(got, args[:2], go), torch.autograd.grad(ref, args[:2], go)):
+                assert torch.equal(x, y)
+    if not grad:
+        one = torch.jit.trace(lambda q, k, n: F.sliding_window_attention(q, k, k, 16, lengths=n),
+                              (torch.randn(2, 2, 1, 64, device="cuda"), torch.randn(2, 2, 50, 64, device="cuda"),
+                               torch.tensor([3, 50], dtype=torch.int32, device="cuda")), check_trace=False)
+        q, k = torch.randn(3, 2, 1, 64, device="cuda"), torch.randn(3, 2, 400, 64, device="cuda")
+        n = torch.tensor([0, 400, 17], dtype=torch.int32, device="cuda")
+        assert torch.equal(one(q, k, n), F.sliding_window_attention(q, k, k, 16, lengths=n))
