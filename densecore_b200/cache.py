@@ -9,6 +9,7 @@ from __future__ import annotations
 import numbers
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, _native
 
@@ -92,7 +93,7 @@ class KVCache4:
     def append(self, key, value, page_table, start, end=None):
         """Token i of key, value (B, kv_heads, T, head_dim) to position ``start[b] + i``, where that is
         below ``end[b]`` (ragged prompts). Places from ``end`` on keep what they hold. One call must
-        not write a slot twice."""
+        not write a slot twice. Keys and values are taken detached: no gradient or tangent passes the cache."""
         self._eager()
         b = self._table(page_table)
         _counts("start", start, b)
@@ -134,7 +135,8 @@ class KVCache4:
             raise ValueError(f"cache attention query must be ({b}, H, 1, {self.head_dim}), got {tuple(query.shape)}")
         if query.shape[1] % self.kv_heads:
             raise ValueError(f"query heads must be a multiple of the cache's {self.kv_heads}")
-        if query.requires_grad and torch.is_grad_enabled():
+        if (query.requires_grad and torch.is_grad_enabled()
+                or forward_ad._current_level >= 0 and forward_ad.unpack_dual(query).tangent is not None):
             raise NotImplementedError("attention over a 4-bit cache has no gradient")
         if scale is not None and (isinstance(scale, bool) or not isinstance(scale, numbers.Real)):
             raise TypeError("scale must be real")

@@ -13,6 +13,7 @@ import numbers
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -191,8 +192,9 @@ def _whole_number(name, value, least=None):
 
 
 def _through_function(what, *inputs):
-    """Whether a call goes through its autograd Function: an input requires a gradient, or it is traced."""
-    return _native._traced(what) or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs))
+    """Whether a call goes through its autograd Function: an input requires a gradient, the call is traced, or
+    an input may have a forward-mode tangent (which the Function refuses and the kernels would drop)."""
+    return _native._traced(what) or forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs))
 
 
 class _SlidingWindow(torch.autograd.Function):

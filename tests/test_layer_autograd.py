@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import densecore_b200 as dc
@@ -94,3 +95,39 @@ def test_a_cache_is_not_traced():
         with pytest.raises(RuntimeError, match="make_fx"):
             make_fx(call)(q)
         call(q)
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad])
+@pytest.mark.parametrize("name", CALLS)
+def test_tangents_are_refused_not_dropped(name, mode):
+    q = torch.randn(1, 2, 3, 8)
+    with mode(), forward_ad.dual_level():
+        assert torch.equal(CALLS[name](q), q)  # no tangent, no refusal
+        with pytest.raises(NotImplementedError, match="jvp"):
+            CALLS[name](forward_ad.make_dual(q, torch.ones_like(q)))
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.jvp(CALLS[name], (q,), (q,))
+
+
+def test_tangents_of_other_inputs_are_refused():
+    q, k, w = torch.randn(1, 2, 1, 8), torch.randn(1, 2, 4, 8), torch.ones(8)
+    at = torch.arange(1)
+    calls = {
+        "key": lambda d: F.sliding_window_attention(q, d(k), k, 4), "value": lambda d: F.sliding_window_attention(q, k, d(k), 4),
+        "value of padded keys": lambda d: F.sliding_window_attention(q, k, d(k), 4, lengths=LENGTHS),
+        "mask": lambda d: F.sliding_window_attention(q, k, k, 4, attn_mask=d(torch.zeros(1, 4))),
+        "weight": lambda d: F.qk_norm_rotary(q, None, d(w), None, at, FREQ),
+        "frequencies": lambda d: F.rotary_embedding(q, None, at, d(FREQ)),
+    }
+    for name, call in calls.items():
+        call(lambda t: t)
+        with forward_ad.dual_level():
+            call(lambda t: t)
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+    cache = dc.KVCache4(2, 2, 64, page_size=16, device="cpu")
+    table, one = torch.zeros(1, 1, dtype=torch.int32), torch.randn(1, 4, 1, 64)
+    with forward_ad.dual_level():
+        assert torch.equal(cache.attention(one, table, LENGTHS), one)
+        with pytest.raises(NotImplementedError, match="gradient"):
+            cache.attention(forward_ad.make_dual(one, one), table, LENGTHS)
