@@ -329,6 +329,8 @@ def _rotary_args(what, query, key, positions, inv_freq, interleaved, amplitude):
         raise TypeError("positions must be an int32 or int64 Tensor")
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64:
         raise TypeError("inv_freq must be a float64 Tensor")
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{what}: frequencies that require grad are not supported")
     if type(interleaved) is not bool:
         raise TypeError("interleaved must be a bool")
     if type(amplitude) is not float and (isinstance(amplitude, (bool, np.bool_)) or not isinstance(amplitude, numbers.Real)):
@@ -360,7 +362,8 @@ def rotary_embedding(query, key, positions, inv_freq, *, interleaved=False, ampl
     float16 or bfloat16, any strides, D even and at most 256; positions int32 or int64, (L) or (B, L);
     inv_freq float64 (:func:`rotary_frequencies`). Pair i of channels, (i, i + len(inv_freq)) or, with
     ``interleaved``, (2i, 2i + 1), turns by positions * inv_freq[i]; ``amplitude`` multiplies the turned
-    channels and the others pass through. Not in DenseCore, whose nanoGPT path adds learned positions.
+    channels and the others pass through. Differentiable in query and key. Not in DenseCore, whose nanoGPT
+    path adds learned positions.
     """
     q, k = _rotary_args("rotary", query, key, positions, inv_freq, interleaved, amplitude)
     if _through_function("rotary_embedding", q, k):

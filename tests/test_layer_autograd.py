@@ -131,3 +131,12 @@ def test_tangents_of_other_inputs_are_refused():
         assert torch.equal(cache.attention(one, table, LENGTHS), one)
         with pytest.raises(NotImplementedError, match="gradient"):
             cache.attention(forward_ad.make_dual(one, one), table, LENGTHS)
+
+
+def test_frequencies_get_no_gradient():
+    q, freq = torch.randn(1, 2, 3, 8), FREQ.clone().requires_grad_()
+    for call in (lambda: F.rotary_embedding(q, None, POS, freq), lambda: F.qk_norm_rotary(q, q, None, None, POS, freq)):
+        with pytest.raises(NotImplementedError, match="frequencies"):
+            call()
+        with torch.no_grad():
+            assert torch.equal(call()[0], q)
