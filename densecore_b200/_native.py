@@ -211,15 +211,16 @@ def _fwd_path(q, k, v, mask=None, causal=False, precision=None):
 
 
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
+_PRE_DISPATCH = torch._ops.mode_stack_state_for_pre_dispatch()
+_mode_count, _is_tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
 
 
 def _traced(what):
     """Whether torch.jit.trace is recording: of a call outside an autograd Function it would record the
     allocations alone, and the trace return them unwritten. make_fx records no Function either: refused."""
-    if (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None
-            or torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None):
+    if _mode_count() and torch._C._get_dispatch_mode(_PROXY) is not None or _PRE_DISPATCH.get(0) is not None:
         raise RuntimeError(f"{what} cannot be recorded by make_fx")
-    return torch._C._get_tracing_state() is not None
+    return _is_tracing()
 
 
 _SAME_DEVICE = contextlib.nullcontext()
@@ -282,8 +283,10 @@ def _sliding_window(q, k, v, window, sinks, offset, scale=None, mask=None, lengt
     ``need_lse``: (out, None)."""
     L = _lib.load()
     dev = _device_of(q, k, v, mask, lengths)
-    B, H, Lq, E = map(int, q.shape)  # (in a trace they come as tensors)
-    Hkv, S, Ev = int(k.shape[1]), int(k.shape[2]), int(v.shape[3])
+    B, H, Lq, E = q.shape
+    Hkv, S, Ev = k.shape[1], k.shape[2], v.shape[3]
+    if type(B) is not int:  # in a trace they come as tensors
+        B, H, Lq, E, Hkv, S, Ev = map(int, (B, H, Lq, E, Hkv, S, Ev))
     out = torch.empty_like(q) if E == Ev else torch.empty((B, H, Lq, Ev), device=dev, dtype=torch.float32)
     prec = precision_code() if precision is None else precision
     has, sc = _scale_args(scale)

@@ -191,10 +191,13 @@ def _whole_number(name, value, least=None):
     return int(value)
 
 
-def _through_function(what, *inputs):
+def _through_function(what, a, b, c=None, d=None):
     """Whether a call goes through its autograd Function: an input requires a gradient, the call is traced, or
     an input may have a forward-mode tangent (which the Function refuses and the kernels would drop)."""
-    return _native._traced(what) or forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs))
+    if _native._traced(what) or forward_ad._current_level >= 0:
+        return True
+    return (a.requires_grad or b is not None and b.requires_grad or c is not None and c.requires_grad
+            or d is not None and d.requires_grad) and torch.is_grad_enabled()
 
 
 class _SlidingWindow(torch.autograd.Function):
