@@ -290,12 +290,7 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bo
     const int which = blockIdx.y & 1, head = blockIdx.y >> 1, lanes = a.c.D / 4, ng = a.c.D / GROUP;
     const int64_t b = blockIdx.z;
     const int quad = threadIdx.x & (lanes - 1), g = quad / 8, r = quad % 8, pass = 256 / lanes, row0 = threadIdx.x / lanes;
-    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), capacity = a.P * a.c.page_size;
-    int64_t len = a.lens[b * a.lens_stride];
-    if (len < 0 || len > capacity) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.err, BAD_TABLE);
-        len = len < 0 ? 0 : capacity;
-    }
+    const int64_t t0 = (int64_t)blockIdx.x * (pass * ROWS), len = a.lens[b * a.lens_stride];
     block_places(a, b, 0, t0, min(a.T, len), pass * ROWS, which, head, places);
     const int code = code_at(which, r, g, ng);
     uint32_t codes[ROWS], sl[ROWS];
@@ -331,6 +326,12 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Args a, bo
             const int64_t st = a.ys[which][3];
             row[0] = y[0].x, row[st] = y[0].y, row[2 * st] = y[1].x, row[3 * st] = y[1].y;
         }
+    }
+    // Tokens past the table have no place; a length out of range is told whether or not they are read. (One
+    // thread of a sequence looks, at the end: there it takes 0.2 us of the kernel's 22, before the loads 0.5 to 1.5.)
+    if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) {
+        const int64_t n = a.lens[b * a.lens_stride];
+        if (n < 0 || n > a.P * a.c.page_size) atomicExch(a.err, BAD_TABLE);
     }
 }
 
