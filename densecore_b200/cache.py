@@ -123,7 +123,11 @@ class KVCache4:
         float32, float16 or bfloat16, over its first ``lengths[b]`` positions; H a multiple of
         kv_heads (grouped queries). With ``window`` the token, standing at the last position, sees the
         positions less than ``window`` back and the first ``sinks``. scale defaults to
-        1/sqrt(head_dim). An empty sequence gives 0. No gradient."""
+        1/sqrt(head_dim). An empty sequence gives 0. No gradient.
+
+        The softmax's weights keep 24 bits for float32 queries and 16 for the others; a query keeps 28 bits
+        below its largest channel, or 22 where several heads share a key head. Scores and sums are held in
+        32 bits. :func:`densecore_b200.set_sdpa_precision` does not apply."""
         self._eager()
         b = self._table(page_table)
         _counts("lengths", lengths, b)

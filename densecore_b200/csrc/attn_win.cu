@@ -670,6 +670,10 @@ bool window_forward_pick(const AttnProblem &p) {
     // window, 32 heads on 8: 160 : 155; 1024 tokens 367 : 481). Heads of 64 gain nothing at any window (16
     // heads, 16384 tokens, window 2048: 661 : 653, 256: 253 : 195): there the softmax, not the products,
     // bounds both.
+    // (These are times of calls without a wide tile. A call with one, seen by any query tile, is done over
+    // whole: the 16 x 16383 one took 875 us, 2440 with one row of v in the first tile of each head scaled by 2^-9,
+    // which every query tile sees among its first tokens, and 2540 with such a row in one head; attn_tc.cu alone
+    // takes 1427.)
     const double most = (double)min(p.window, p.S), L = (double)p.L, first = (double)max(p.offset, (int64_t)0) + 1.0;
     // The mean over the rows of min(position, most), positions rising from `first`.
     const double ramp = min(max(most - first, 0.0), L), mean = most - (most > first ? ramp * (most - first - 0.5 * ramp) / L : 0.0);

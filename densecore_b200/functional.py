@@ -233,7 +233,9 @@ def sliding_window_attention(query, key, value, window, sinks=0, attn_mask=None,
     lets it. ``lengths`` (int32 (B), L == 1, no gradient) are the keys that each sequence of a padded cache holds:
     its row stands at the last of them. A row that sees no key gives 0 and zero gradients, one that sees
     a single key no gradient of query and key. Hidden keys may hold anything in the forward; hidden values,
-    and for the gradients hidden keys, must be finite. scale defaults to 1/sqrt(E). Not in DenseCore; the rules are those of its SDPA (functional.py:276-340).
+    and for the gradients hidden keys, must be finite: rows of a padded batch that nobody wrote may not be.
+    scale defaults to 1/sqrt(E). Products are taken as :func:`densecore_b200.set_sdpa_precision` says; one
+    query row always in float32. Not in DenseCore; the rules are those of its SDPA (functional.py:276-340).
     """
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not isinstance(t, torch.Tensor):
@@ -286,7 +288,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
     interpolated: every frequency over factor); "ntk" (the base raised to base * factor^(d/(d-2)), so
     that the fastest frequency stays and the slowest is interpolated); "yarn" (frequencies that make
     more than ``fast`` turns over ``original_length`` stay, those below ``slow`` are interpolated, linear
-    in between; amplitude 0.1 ln(factor) + 1).
+    in the number of turns in between, as its paper has it; amplitude 0.1 ln(factor) + 1). Checkpoints
+    trained with a ramp linear in the pair's index between those two bounds, as released code has it,
+    need that code's frequencies in between: any float64 tensor serves as ``inv_freq``.
     """
     d = _whole_number("rotary_dim", rotary_dim, 2)
     if d % 2:
@@ -363,7 +367,8 @@ def rotary_embedding(query, key, positions, inv_freq, *, interleaved=False, ampl
 
     query (B, H, L, D) and key (B, Hkv, L, D; or None), or rank 3 without the head dim, in float32,
     float16 or bfloat16, any strides, D even and at most 256; positions int32 or int64, (L) or (B, L);
-    inv_freq float64 (:func:`rotary_frequencies`). Pair i of channels, (i, i + len(inv_freq)) or, with
+    inv_freq float64 (:func:`rotary_frequencies`). Angles are taken in 64 bits: one of a radians is off by
+    up to a * 2^-51. Pair i of channels, (i, i + len(inv_freq)) or, with
     ``interleaved``, (2i, 2i + 1), turns by positions * inv_freq[i]; ``amplitude`` multiplies the turned
     channels and the others pass through. Differentiable in query and key. Not in DenseCore, whose nanoGPT
     path adds learned positions.
