@@ -685,10 +685,7 @@ int window_forward(const AttnProblem &p, cudaStream_t stream) {
     Scratch ws;
     ws.stream = stream;
     int st = pool_alloc(&ws.ptr, sizeof(__half) * (size_t)(4 * nk) + sizeof(float) * (size_t)(4 * fk + 1), stream);
-    if (st) {  // no room for the copies: the kernel that needs none (whose launch check would find this error)
-        cudaGetLastError();
-        return tc_forward(p, DC_PREC_3XTF32, stream);
-    }
+    if (st) return tc_forward(p, DC_PREC_3XTF32, stream);  // no room for the copies: the kernel that needs none
     __half *k16 = static_cast<__half *>(ws.ptr), *v16 = k16 + 2 * nk;
     float *kf = reinterpret_cast<float *>(v16 + 2 * nk), *vf = kf + fk;
     uint8_t *kw = reinterpret_cast<uint8_t *>(vf + fk), *vw = kw + 4 * fk;

@@ -34,6 +34,7 @@ int fail(int status, const std::string &msg) {
 }
 
 int cuda_fail(cudaError_t err, const char *what) {
+    cudaGetLastError();  // a failed allocation is not the next call's launch error
     g_last_error = std::string(what) + ": " + cudaGetErrorString(err);
     return DC_ERR_CUDA;
 }

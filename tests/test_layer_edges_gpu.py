@@ -89,3 +89,65 @@ def test_traced_calls_run_at_other_sizes(grad):
         q, k = torch.randn(3, 2, 1, 64, device="cuda"), torch.randn(3, 2, 400, 64, device="cuda")
         n = torch.tensor([0, 400, 17], dtype=torch.int32, device="cuda")
         assert torch.equal(one(q, k, n), F.sliding_window_attention(q, k, k, 16, lengths=n))
+
+
+WITHOUT_ROOM = """
+import torch
+from densecore_b200 import functional as F
+
+q, k, v = (torch.randn(1, 16, 8192, 128, device="cuda") for _ in range(3))
+small = [t[:, :2, :200].contiguous().requires_grad_() for t in (q, k, v)]
+
+
+def step():
+    out = F.sliding_window_attention(*small, 64)
+    return [out.detach(), *torch.autograd.grad(out.sum(), small)]
+
+
+want = step()
+F.sliding_window_attention(q[:, :1, :700], k[:, :1, :700], v[:, :1, :700], 699)  # loads the kernels
+leaves = [t.requires_grad_() for t in (q, k, v)]
+out = F.sliding_window_attention(*leaves, 64)
+go = torch.ones_like(out)
+torch.cuda.synchronize()
+
+
+def leave(mib):
+    return torch.empty(torch.cuda.mem_get_info()[0] - (mib << 20), dtype=torch.uint8, device="cuda")
+
+
+fill = leave(112)  # 64 for the output, 134 for the copies
+with torch.no_grad():
+    tight = F.sliding_window_attention(q, k, v, 2048)
+assert all(torch.equal(x, y) for x, y in zip(step(), want))  # the next call is a clean one
+del fill
+torch.cuda.empty_cache()
+fill = leave(512)  # 192 for the gradients, 537 for the copies
+for _ in range(2):
+    try:
+        torch.autograd.grad(out, leaves, go, retain_graph=True)
+        raise SystemExit("the backward found room")
+    except torch.OutOfMemoryError:
+        raise
+    except RuntimeError as e:
+        assert "memory" in str(e), e
+    assert all(torch.equal(x, y) for x, y in zip(step(), want))
+del fill, out, go
+torch.cuda.empty_cache()
+with torch.no_grad():
+    roomy = F.sliding_window_attention(q, k, v, 2048)
+err = (tight - roomy).norm() / roomy.norm()
+assert 0 < err < 5e-6, err
+assert all(torch.equal(x, y) for x, y in zip(step(), want))
+print("fine")
+"""
+
+
+def test_a_call_without_room_leaves_the_next_alone():
+    # In a process of its own: the library's pool keeps what earlier calls took.
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", WITHOUT_ROOM], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
