@@ -197,10 +197,11 @@ DC_API int dc_sdpa_window_bwd(const dc_tensor_t *grad_out, const dc_tensor_t *q,
 
 /* ---- Rotary positions, alone or behind a norm of each head (no counterpart in the reference) ----
  * q (B, H, L, D) and k (B, Hkv, L, D; nullable) of one type, float32, float16 or bfloat16, any
- * strides, D even and at most 256; positions int32 or int64, (L) or (B, L); inv_freq float64 (r), the angle per position of the r pairs: channels (i, r + i), or (2 i, 2 i + 1) when
- * interleaved. A pair (a, b) becomes amplitude * (a cos - b sin, b cos + a sin); channels from 2 r on
- * pass through. Arithmetic is in 32 bits (angles in 64: off by up to 2^-51 of themselves), rounded
- * once. Outputs have the inputs' shapes and type, any strides, and may be the inputs themselves. */
+ * strides, D even and at most 256; positions int32 or int64, (L) or (B, L); inv_freq float64 (r), the
+ * angle per position of the r pairs: channels (i, r + i), or (2 i, 2 i + 1) when interleaved. A pair
+ * (a, b) becomes amplitude * (a cos - b sin, b cos + a sin); channels from 2 r on pass through.
+ * Arithmetic is in 32 bits (angles in 64: off by up to 2^-51 of themselves), rounded once. Outputs have
+ * the inputs' shapes and type, any strides, and may be the inputs themselves. */
 
 /* inverse != 0 turns by the negative angles: the gradient of the inputs from the outputs'. */
 DC_API int dc_rotary(const dc_tensor_t *q, const dc_tensor_t *k, const dc_tensor_t *positions,
